@@ -113,6 +113,18 @@ SIGNATURES = {
     "ds_ep_layer_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "ds_ep_layer_forward": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                                  _i, _i, _i, _vp, _i, _i, _vp, _sz, _vp, _vp]),
+    "ds_int8_quantize": (_i, [_vp, _i64, _i, _i, _vp, _vp, _vp]),
+    "ds_int8_linear_workspace_size": (_sz, [_i, _i, _i]),
+    "ds_int8_linear": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "ds_mla_cache4_append": (_i, [_vp, _i64, _vp, _i64, _i64, _i, _vp, _vp, _vp, _i, _f, _vp, _vp,
+                                  _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "ds_mla_cache4_get": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "ds_mla_decode_attention4_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "ds_mla_decode_attention4": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _f,
+                                      _vp, _vp, _sz, _vp]),
+    "ds_mla_cache4_evict_workspace_size": (_sz, [_i, _i]),
+    "ds_mla_cache4_evict": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp,
+                                 _vp, _vp, _i, _vp, _sz, _vp]),
 }
 
 
@@ -755,6 +767,238 @@ def mla_decode_step(x: torch.Tensor, w_dec: torch.Tensor, w_out: torch.Tensor, c
                                        workspace.numel(), ev, _stream(x)), "mla_decode_step")
     cache._advance(1, device_counted=True)
     return out
+
+
+# ---------------------------------------------------------------------- 8-bit integer linear
+def int8_quantize(x: torch.Tensor) -> List[torch.Tensor]:
+    """Rows of x to 8-bit integers, one scale per row (additive): x bf16 [..., K] ->
+    [q int8 [..., K], scale f32 [...]] with a = max |row|, q = rint(127 x / a) (ties to even),
+    scale = a / 127.  A row of zeros gives zeros and scale 0; a row with an infinity or a NaN
+    gives zeros and scale NaN.  Weights [N, K] are quantised per output channel the same way.
+    K: a multiple of 16."""
+    _require(x.is_cuda, "int8_quantize: x must be a CUDA tensor.")
+    _require(x.dtype == torch.bfloat16, "int8_quantize: x must be bfloat16.")
+    _require(x.dim() >= 1 and x.shape[-1] > 0, "int8_quantize: x must be [..., K].")
+    K = x.shape[-1]
+    _require(K % 16 == 0, "int8_quantize: K must be a multiple of 16.")
+    x2 = _rows_2d(x)
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if x.numel() == 0:
+        return [q, scale]
+    with _on_device(x):
+        _check(_lib.ds_int8_quantize(_ptr(x2), x2.stride(0), x2.shape[0], K, _ptr(q), _ptr(scale),
+                                     _stream(x)), "int8_quantize")
+    return [q, scale]
+
+
+def _rows_2d(x: torch.Tensor) -> torch.Tensor:
+    """x [..., K] as [rows, K] whose rows are contiguous and start on 16-byte boundaries (a
+    copy only where the strides do not allow a view)."""
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
+        x2 = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device).copy_(x2)
+    return x2
+
+
+def int8_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
+                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x bf16 [..., K] @ (w_q int8 [N, K] * w_scale f32 [N, 1])^T -> bf16 [..., N] (additive).
+
+    The rows of x are quantised as int8_quantize does, the product of the integers is exact
+    (32 bits) and scaled once: bf16(acc * (scale_row * w_scale)).  K: a multiple of 16, at most
+    131072; N: a multiple of 8.  `workspace` (uint8, at least int8_linear_workspace_size bytes)
+    saves the allocation; calls that overlap need different ones."""
+    _require(x.is_cuda and w_q.is_cuda and w_scale.is_cuda,
+             "int8_linear: x, w_q and w_scale must be CUDA tensors.")
+    _require(x.dtype == torch.bfloat16, "int8_linear: x must be bfloat16.")
+    _require(w_q.dtype == torch.int8 and w_q.dim() == 2 and w_q.is_contiguous(),
+             "int8_linear: w_q must be a contiguous int8 [N, K] tensor.")
+    _require(w_scale.dtype == torch.float32 and tuple(w_scale.shape) == (w_q.shape[0],)
+             and w_scale.is_contiguous(), "int8_linear: w_scale must be a contiguous float32 [N] tensor.")
+    _require(w_q.device == x.device and w_scale.device == x.device,
+             "int8_linear: x, w_q and w_scale must be on one device.")
+    N, K = w_q.shape
+    _require(x.dim() >= 1 and x.shape[-1] == K,
+             f"int8_linear: x last dim must match w_q inner dim {K}.")
+    _require(K > 0 and K % 16 == 0, "int8_linear: K must be a positive multiple of 16.")
+    _require(N % 8 == 0, "int8_linear: N must be a multiple of 8.")
+    out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
+    if out.numel() == 0:
+        return out
+    x2 = _rows_2d(x)
+    need = int8_linear_workspace_size(x2.shape[0], N, K)
+    workspace = _scratch(workspace, need, x.device, "int8_linear")
+    with _on_device(x):
+        _check(_lib.ds_int8_linear(_ptr(x2), x2.stride(0), _ptr(w_q), _ptr(w_scale), _ptr(out),
+                                   x2.shape[0], N, K, _ptr(workspace), workspace.numel(),
+                                   _stream(x)), "int8_linear")
+    return out
+
+
+def int8_linear_workspace_size(rows: int, out_features: int, in_features: int) -> int:
+    return int(_lib.ds_int8_linear_workspace_size(rows, out_features, in_features))
+
+
+def _scratch(workspace: Optional[torch.Tensor], need: int, device: torch.device,
+             op: str) -> torch.Tensor:
+    if workspace is None or workspace.numel() < need:
+        return _workspace(need, device)
+    _require(workspace.dtype == torch.uint8 and workspace.is_contiguous()
+             and workspace.device == device and workspace.data_ptr() % 16 == 0,
+             f"{op}: workspace must be a contiguous, 16-byte aligned uint8 tensor on x's device.")
+    return workspace
+
+
+# ------------------------------------------------------------------- 4-bit latent KV cache
+def _require_cache4(cache, op: str) -> None:
+    _require(cache.codes.is_cuda, f"{op}: the cache must reside on a CUDA device.")
+
+
+def _cache4_ptrs(cache):
+    return (_ptr(cache.codes), _ptr(cache.scales), _ptr(cache.rstd), _ptr(cache.pos),
+            _ptr(cache.mass), _ptr(cache.state))
+
+
+def mla_cache4_append(latent: torch.Tensor, k_pe: torch.Tensor, cache, cos: torch.Tensor,
+                      sin: torch.Tensor, eps: float = 1e-6,
+                      new_lens: Optional[torch.Tensor] = None) -> None:
+    """latent bf16 [bsz, n, 512] (raw), k_pe bf16 [bsz, n, 64] (raw; any row stride with 16-byte
+    aligned rows) -> quantised behind each sequence's last slot of `cache`
+    (mla_cache.LatentKVCache4), k_pe rotated at its position (cos/sin bf16 [positions, 64]).
+    new_lens int32 [bsz] (on the device): only the first new_lens[b] tokens of sequence b (a
+    ragged, padded batch)."""
+    _require(latent.is_cuda and k_pe.is_cuda, "mla_cache4_append: inputs must be CUDA tensors.")
+    _require(latent.dtype == torch.bfloat16 and k_pe.dtype == torch.bfloat16,
+             "mla_cache4_append: latent and k_pe must be bfloat16.")
+    _require(latent.dim() == 3 and latent.shape[2] == 512 and latent.shape[0] == cache.bsz
+             and tuple(k_pe.shape) == (*latent.shape[:2], 64),
+             "mla_cache4_append: latent must be [bsz, n, 512] and k_pe [bsz, n, 64].")
+    _require(latent.device == cache.codes.device and k_pe.device == cache.codes.device,
+             "mla_cache4_append: inputs and cache must be on one device.")
+    _check_tables(cos, sin, cache, "mla_cache4_append")
+    B, n, _ = latent.shape
+    if B * n == 0:
+        return
+    if new_lens is not None:
+        _require(new_lens.is_cuda and new_lens.dtype == torch.int32 and new_lens.is_contiguous()
+                 and tuple(new_lens.shape) == (B,) and new_lens.device == cache.codes.device,
+                 "mla_cache4_append: new_lens must be a contiguous int32 [bsz] tensor on the "
+                 "cache's device.")
+    cache._check_room(n, cos.shape[0])
+    ok = (latent.stride(2) == 1 and k_pe.stride(2) == 1 and latent.stride(1) % 8 == 0
+          and k_pe.stride(1) % 8 == 0 and latent.data_ptr() % 16 == 0 and k_pe.data_ptr() % 16 == 0
+          and latent.stride(1) > 0 and k_pe.stride(1) > 0)
+    rows = latent.stride(0) // latent.stride(1) if ok else 0
+    if not ok or latent.stride(0) != rows * latent.stride(1) or k_pe.stride(0) != rows * k_pe.stride(1):
+        latent = torch.empty(latent.shape, dtype=latent.dtype, device=latent.device).copy_(latent)
+        k_pe = torch.empty(k_pe.shape, dtype=k_pe.dtype, device=k_pe.device).copy_(k_pe)
+        rows = n
+    with _on_device(latent):
+        _check(_lib.ds_mla_cache4_append(_ptr(latent), latent.stride(1), _ptr(k_pe),
+                                         k_pe.stride(1), rows, n, _ptr(new_lens), _ptr(cos),
+                                         _ptr(sin), cos.shape[0], float(eps),
+                                         *_cache4_ptrs(cache), B, cache.slots, _stream(latent)),
+               "mla_cache4_append")
+    cache._advance(n)
+
+
+def _check_tables(cos: torch.Tensor, sin: torch.Tensor, cache, op: str) -> None:
+    for t in (cos, sin):
+        _require(t.is_cuda and t.dtype == torch.bfloat16 and t.is_contiguous() and t.dim() == 2
+                 and t.shape[1] == 64 and t.shape[0] > 0 and t.shape == cos.shape
+                 and t.device == cache.codes.device,
+                 f"{op}: cos and sin must be contiguous bfloat16 [positions, 64] tensors on the "
+                 "cache's device.")
+
+
+def mla_cache4_get(cache, seq_len: Optional[int] = None) -> List[torch.Tensor]:
+    """The cache read back as bf16 values: [raw latent [bsz, seq_len, 512], rotated k_pe
+    [bsz, seq_len, 64]], zeros from a sequence's length on; seq_len defaults to the cache's
+    current_len (its longest sequence's bound)."""
+    _require_cache4(cache, "mla_cache4_get")
+    n = cache.current_len if seq_len is None else int(seq_len)
+    _require(0 <= n <= cache.slots, f"mla_cache4_get: seq_len={n} outside the cache.")
+    dev = cache.codes.device
+    lat = torch.empty((cache.bsz, n, 512), dtype=torch.bfloat16, device=dev)
+    kpe = torch.empty((cache.bsz, n, 64), dtype=torch.bfloat16, device=dev)
+    if lat.numel() == 0:
+        return [lat, kpe]
+    with _on_device(lat):
+        _check(_lib.ds_mla_cache4_get(_ptr(cache.codes), _ptr(cache.scales), _ptr(cache.state),
+                                      cache.bsz, cache.slots, n, _ptr(lat), _ptr(kpe),
+                                      _stream(lat)), "mla_cache4_get")
+    return [lat, kpe]
+
+
+def mla_decode_attention4_workspace_size(batch: int, heads: int, slots: int, max_len: int,
+                                         accumulate: bool = False) -> int:
+    return int(_lib.ds_mla_decode_attention4_workspace_size(batch, heads, slots, max_len,
+                                                            1 if accumulate else 0))
+
+
+def mla_decode_attention4(q: torch.Tensor, cache, softmax_scale: float,
+                          mass_decay: Optional[float] = None,
+                          out: Optional[torch.Tensor] = None,
+                          workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One decode step's attention over a 4-bit cache (mla_cache.LatentKVCache4): q bf16
+    [bsz, heads, 576] (512 absorbed query, 64 rotated q_pe) -> the latent outputs bf16
+    [bsz, heads * 512]; 1 to 128 heads; a sequence without tokens gives zeros.
+
+    With mass_decay the attention weights are accumulated for a later eviction:
+    cache.mass[b, t] = mass_decay * cache.mass[b, t] + sum over heads of p(t)."""
+    _require(q.is_cuda and q.dtype == torch.bfloat16 and q.is_contiguous(),
+             "mla_decode_attention4: q must be a contiguous bfloat16 CUDA tensor.")
+    _require(q.dim() == 3 and q.shape[0] == cache.bsz and q.shape[2] == 576,
+             "mla_decode_attention4: q must be [bsz, heads, 576].")
+    _require(q.device == cache.codes.device,
+             "mla_decode_attention4: q and cache must be on one device.")
+    B, heads, _ = q.shape
+    _require(1 <= heads <= 128, "mla_decode_attention4: heads must be in [1, 128].")
+    _require(mass_decay is None or 0.0 <= mass_decay <= 1.0,
+             "mla_decode_attention4: mass_decay must be in [0, 1].")
+    if out is None:
+        out = torch.empty((B, heads * 512), dtype=torch.bfloat16, device=q.device)
+    else:
+        _check_out(out, B, heads * 512, q.device)
+    if B == 0:
+        return out
+    acc = mass_decay is not None
+    max_len = cache.bound_for_launch
+    need = mla_decode_attention4_workspace_size(B, heads, cache.slots, max_len, acc)
+    workspace = _scratch(workspace, need, q.device, "mla_decode_attention4")
+    with _on_device(q):
+        _check(_lib.ds_mla_decode_attention4(
+            _ptr(q), heads, _ptr(cache.codes), _ptr(cache.scales), _ptr(cache.rstd),
+            _ptr(cache.mass), _ptr(cache.state), B, cache.slots, max_len, float(softmax_scale),
+            1 if acc else 0, float(mass_decay or 0.0), _ptr(out), _ptr(workspace),
+            workspace.numel(), _stream(q)), "mla_decode_attention4")
+    return out
+
+
+def mla_cache4_evict(cache, budget: int, recent: int = 0, out=None):
+    """Evict from a 4-bit cache by accumulated attention weight: every sequence longer than
+    `budget` keeps the `recent` newest positions and, of the rest, those of the largest mass
+    (ties to the lowest slot; NaN last), `budget` slots in all.  In place, or into `out`
+    (another LatentKVCache4 of the same batch with at least `budget` slots, whose contents it
+    replaces).  Survivors behind the budget fill the freed slots before it, both in ascending
+    order; the others stay.  Returns the cache that holds the result."""
+    _require_cache4(cache, "mla_cache4_evict")
+    dst = cache if out is None else out
+    budget, recent = int(budget), int(recent)
+    _require(dst.bsz == cache.bsz and dst.codes.device == cache.codes.device,
+             "mla_cache4_evict: out must have the cache's batch size and device.")
+    _require(1 <= budget <= dst.max_seq,
+             f"mla_cache4_evict: budget must be in [1, {dst.max_seq}].")
+    _require(0 <= recent <= budget, "mla_cache4_evict: recent must be in [0, budget].")
+    need = int(_lib.ds_mla_cache4_evict_workspace_size(cache.bsz, budget))
+    ws = _workspace(need, cache.codes.device)
+    with _on_device(cache.codes):
+        _check(_lib.ds_mla_cache4_evict(*_cache4_ptrs(cache), cache.bsz, cache.slots, budget,
+                                        recent, *_cache4_ptrs(dst), dst.slots, _ptr(ws), need,
+                                        _stream(cache.codes)), "mla_cache4_evict")
+    dst._evicted(cache, budget)
+    return dst
 
 
 def device_status() -> int:

@@ -151,3 +151,152 @@ class LatentKVCache:
         self._side_len = self._len
         if not device_counted:
             self.len_dev.fill_(self._len)
+
+
+class LatentKVCache4:
+    """Latent KV cache held in 4 bits: 310 bytes a token against LatentKVCache's 1156 (with its
+    side arrays).  Filled by ds_kernels.mla_cache4_append (FusedMLA.prefill / decode), read by
+    ds_kernels.mla_decode_attention4, trimmed by ds_kernels.mla_cache4_evict.
+
+    Sequences have their own lengths (device, int32 `lens`) and next positions (`next_pos`: the
+    tokens seen, evicted ones included, so a token keeps its rotary position when others leave).
+    Arrays, per sequence and slot (`slots` = max_seq rounded up to 64):
+
+        codes   uint8 [bsz, slots, 288]  two 4-bit codes a byte, low half first: 512 dimensions
+                                         of the raw latent, then 64 of k_pe rotated at its
+                                         position; value = (code - 8) * scale of its group
+        scales  bf16  [bsz, 5, slots]    four groups of 128 latent dimensions, then k_pe:
+                                         bf16(max |v| / 7)
+        rstd    f32   [bsz, slots]       rsqrt(mean(latent^2) + eps) of the exact latent
+        pos     int32 [bsz, slots]       position of the token in the slot
+        mass    f32   [bsz, slots]       accumulated attention weight
+
+    The host knows only a bound on the lengths (`current_len`: exact for batches that are not
+    ragged), which it advances with every call; no call synchronises.  A call recorded into a
+    CUDA graph takes the whole cache as its bound, so replays may go on to the last slot; replays
+    move the device-side lengths only, and the caller reports them with note_replay()."""
+
+    def __init__(self, bsz: int, max_seq: int, device="cuda"):
+        if not isinstance(bsz, int) or bsz < 1:
+            raise ValueError(f"bsz must be a positive integer, got {bsz}")
+        if not isinstance(max_seq, int) or max_seq < 1:
+            raise ValueError(f"max_seq must be a positive integer, got {max_seq}")
+        self.bsz, self.max_seq = bsz, max_seq
+        self.slots = -(-max_seq // 64) * 64
+        dev = self.device = torch.device(device)
+        self.codes = torch.zeros((bsz, self.slots, 288), dtype=torch.uint8, device=dev)
+        self.scales = torch.zeros((bsz, 5, self.slots), dtype=torch.bfloat16, device=dev)
+        self.rstd = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
+        self.pos = torch.zeros((bsz, self.slots), dtype=torch.int32, device=dev)
+        self.mass = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
+        self.state = torch.zeros((2, bsz), dtype=torch.int32, device=dev)
+        self.lens, self.next_pos = self.state[0], self.state[1]
+        self._bound = 0      # no sequence is longer
+        self._seen = 0       # no next position is larger
+
+    @property
+    def current_len(self) -> int:
+        """A bound on the sequences' lengths (the length itself when they are equal)."""
+        return self._bound
+
+    @property
+    def remaining_capacity(self) -> int:
+        """Tokens that surely still fit into every sequence."""
+        return self.max_seq - self._bound
+
+    @property
+    def memory_bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in
+                   (self.codes, self.scales, self.rstd, self.pos, self.mass, self.state))
+
+    @property
+    def bound_for_launch(self) -> int:
+        """The bound that a launch is sized for: all slots inside a graph capture, because a
+        replay sees later lengths."""
+        if self.codes.is_cuda and torch.cuda.is_current_stream_capturing():
+            return self.max_seq
+        return self._bound
+
+    def reset(self) -> None:
+        """Clear the cache for new sequences (keeps the memory)."""
+        self.state.zero_()
+        self._bound = self._seen = 0
+
+    def get(self, seq_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(raw latent bf16 [bsz, seq_len, 512], rotated k_pe bf16 [bsz, seq_len, 64]) as the
+        codes stand for them; zeros from a sequence's length on."""
+        import ds_kernels
+        lat, kpe = ds_kernels.mla_cache4_get(self, seq_len)
+        return lat, kpe
+
+    def evict(self, budget: int, recent: int = 0, out: "Optional[LatentKVCache4]" = None):
+        """ds_kernels.mla_cache4_evict on this cache."""
+        import ds_kernels
+        return ds_kernels.mla_cache4_evict(self, budget, recent, out)
+
+    def note_replay(self, tokens: int = 1) -> None:
+        """A replayed graph appended `tokens` tokens to every sequence."""
+        self._advance(tokens)
+
+    # ---- saving and restoring ------------------------------------------------------------
+    def state_dict(self) -> dict:
+        """Copies of everything the cache holds."""
+        return {k: getattr(self, k).clone()
+                for k in ("codes", "scales", "rstd", "pos", "mass", "lens", "next_pos")}
+
+    def load_state_dict(self, state: dict) -> None:
+        """Take over saved contents (same batch; the saved slots may be fewer).  `codes`,
+        `scales`, `rstd` and `lens` are needed; without `pos` slot i holds position i, without
+        `next_pos` it is the length, without `mass` the weights are 0.  Synchronises once to
+        read the largest length."""
+        for k in ("codes", "scales", "rstd", "lens"):
+            if k not in state:
+                raise ValueError(f"load_state_dict: {k} is missing")
+        n = state["codes"].shape[1]
+        want = {"codes": (self.bsz, n, 288), "scales": (self.bsz, 5, n), "rstd": (self.bsz, n),
+                "pos": (self.bsz, n), "mass": (self.bsz, n), "lens": (self.bsz,),
+                "next_pos": (self.bsz,)}
+        for k, t in state.items():
+            if k not in want or tuple(t.shape) != want[k]:
+                raise ValueError(f"load_state_dict: unexpected {k} of shape {tuple(t.shape)}")
+        lens = state["lens"].to(self.device, torch.int32)
+        nxt = state["next_pos"].to(self.device, torch.int32) if "next_pos" in state else lens
+        lo, hi, top = (int(v) for v in torch.stack([lens.min(), lens.max(), nxt.max()]).tolist())
+        if n > self.slots or lo < 0 or hi > min(n, self.max_seq):
+            raise ValueError("load_state_dict: the saved sequences do not fit the cache")
+        for k in ("codes", "scales", "rstd"):
+            dst = getattr(self, k)
+            (dst[:, :, :n] if k == "scales" else dst[:, :n]).copy_(state[k])
+        if "pos" in state:
+            self.pos[:, :n].copy_(state["pos"])
+        else:
+            self.pos.copy_(torch.arange(self.slots, dtype=torch.int32, device=self.device)
+                           .expand(self.bsz, -1))
+        if "mass" in state:
+            self.mass[:, :n].copy_(state["mass"])
+        else:
+            self.mass.zero_()
+        self.lens.copy_(lens)
+        self.next_pos.copy_(nxt)
+        self._bound, self._seen = hi, top
+
+    def __repr__(self) -> str:
+        return (f"LatentKVCache4(bsz={self.bsz}, tokens<={self._bound}/{self.max_seq}, "
+                f"memory={self.memory_bytes / 2 ** 20:.2f}MB, device={self.device})")
+
+    # ---- bookkeeping of the fused calls --------------------------------------------------
+    def _check_room(self, n: int, table_rows: int) -> None:
+        if self._bound + n > self.max_seq:
+            raise RuntimeError(
+                f"KV cache overflow: current_len={self._bound}, new_tokens={n}, "
+                f"max_seq={self.max_seq}. Increase max_seq, evict or reset the cache.")
+        if self._seen + n > table_rows:
+            raise RuntimeError(f"LatentKVCache4: position {self._seen + n - 1} is beyond the RoPE "
+                               f"tables ({table_rows} positions)")
+
+    def _advance(self, n: int) -> None:
+        self._bound = min(self._bound + n, self.max_seq)
+        self._seen += n
+
+    def _evicted(self, src: "LatentKVCache4", budget: int) -> None:
+        self._bound, self._seen = min(src._bound, budget), src._seen

@@ -481,6 +481,73 @@ DS_API int ds_ep_layer_forward(const void* x_bf16, int num_tokens,
                                void** events, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Matrix product in 8-bit integers with one scale per token and per output channel (new,
+ * additive).  ds_int8_quantize: each row x (bf16, `row_stride` elements apart) to q = rint(127 x
+ * / a) (ties to even), scale = a / 127 with a = max |x|; a = 0 gives zeros, a row with an
+ * infinity or a NaN gives zeros and scale NaN.  ds_int8_linear quantises the rows of x so and
+ * writes out[m, n] = bf16((sum_k q[m,k] w[n,k]) * (scale[m] * w_scale[n])), the sum exact.
+ * cols / in_features: a multiple of 16, at most 131072; out_features: a multiple of 8. */
+DS_API int ds_int8_quantize(const void* x_bf16, int64_t row_stride, int rows, int cols,
+                            void* q_int8, float* scale, void* stream);
+DS_API size_t ds_int8_linear_workspace_size(int rows, int out_features, int in_features);
+DS_API int ds_int8_linear(const void* x_bf16, int64_t row_stride, const void* w_int8,
+                          const float* w_scale, void* out_bf16, int rows, int out_features,
+                          int in_features, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Latent KV cache held in 4 bits (new, additive; beside the bf16 cache of
+ * src/kernels/mla_cache.py:29-219).  Arrays, with slots a multiple of 64: codes u8 [batch,
+ * slots, 288] (512 latent then 64 rotated k_pe dimensions, two a byte, low half first, value =
+ * (code - 8) * scale), scales bf16 [batch, 5, slots] (four groups of 128 latent dimensions,
+ * then k_pe), rstd f32, pos i32 and mass f32 [batch, slots], state i32 [2, batch] (lengths in
+ * slots, next positions).
+ *
+ * ds_mla_cache4_append: new_tokens tokens of every sequence (token i of sequence b at row
+ *   b * src_rows_per_seq + i of latent / kpe; only the first new_lens[b] when given) quantised
+ *   behind its last slot, k_pe rotated at its position (table rows cos/sin [table_rows, 64];
+ *   positions past the table take its last row); mass 0.  Lengths and positions move on.
+ *   Tokens past the last slot are dropped.
+ * ds_mla_cache4_get: slots 0 .. seq_len-1 as bf16 values (raw latent [batch, seq_len, 512],
+ *   rotated k_pe [batch, seq_len, 64]); zeros from a sequence's length on.
+ * ds_mla_decode_attention4: one query token per sequence: q bf16 [batch, heads, 576] (absorbed
+ *   query, rotated q_pe) over slots 0 .. length-1 (at most max_len, a host-side bound on the
+ *   lengths) -> out bf16 [batch, heads * 512]; a sequence without slots gives zeros.
+ *   accumulate != 0: mass[b, t] = mass_decay * mass[b, t] + sum_h p_h(t) for t < length
+ *   (mass_decay 0: the old values are not read).  1 <= heads <= 128.
+ * ds_mla_cache4_evict: a sequence longer than `budget` keeps `budget` slots: those of the
+ *   `recent` newest positions (pos >= next position - recent), then by mass, largest first (NaN
+ *   last), ties to the lowest slot.  Kept slots below the budget stay where they are; the
+ *   others move, in ascending order, into the evicted ones below it.  The result goes to the
+ *   dst arrays (all the same as the source's: in place; or all others, [batch, dst_slots,
+ *   ...]); slots behind the result's length are left as they were.
+ * The calls read lengths on the device, so they can be captured into a graph and replayed. */
+DS_API int ds_mla_cache4_append(const void* latent_bf16, int64_t latent_ld, const void* kpe_bf16,
+                                int64_t kpe_ld, int64_t src_rows_per_seq, int new_tokens,
+                                const int32_t* new_lens, const void* cos_bf16,
+                                const void* sin_bf16, int table_rows, float eps, void* codes,
+                                void* scales_bf16, float* rstd, int32_t* pos, float* mass,
+                                int32_t* state, int batch, int slots, void* stream);
+DS_API int ds_mla_cache4_get(const void* codes, const void* scales_bf16, const int32_t* state,
+                             int batch, int slots, int seq_len, void* latent_out_bf16,
+                             void* kpe_out_bf16, void* stream);
+DS_API size_t ds_mla_decode_attention4_workspace_size(int batch, int heads, int slots,
+                                                      int max_len, int accumulate);
+DS_API int ds_mla_decode_attention4(const void* q_bf16, int heads, const void* codes,
+                                    const void* scales_bf16, const float* rstd, float* mass,
+                                    const int32_t* state, int batch, int slots, int max_len,
+                                    float softmax_scale, int accumulate, float mass_decay,
+                                    void* out_bf16, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+DS_API size_t ds_mla_cache4_evict_workspace_size(int batch, int budget);
+DS_API int ds_mla_cache4_evict(void* codes, void* scales_bf16, float* rstd, int32_t* pos,
+                               float* mass, int32_t* state, int batch, int slots, int budget,
+                               int recent, void* dst_codes, void* dst_scales_bf16,
+                               float* dst_rstd, int32_t* dst_pos, float* dst_mass,
+                               int32_t* dst_state, int dst_slots, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Failure-detection probe (no reference counterpart): launches one CTA that waits on an
  * mbarrier nothing arrives on, through the same bounded-wait routine the GEMM pipeline
  * uses, with a limit of `timeout_cycles` SM clock cycles.  The wait runs out, the kernel

@@ -1,0 +1,145 @@
+"""Refusals of the quantised decode operators and the 4-bit cache's host side (no GPU needed)."""
+import ctypes
+
+import pytest
+import torch
+
+import ds_kernels
+from mla_cache import LatentKVCache4
+
+bf16 = torch.bfloat16
+P = ctypes.c_void_p
+F = ctypes.c_float
+
+
+def lib():
+    return ds_kernels.library()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ds_kernels.int8_quantize(torch.zeros(2, 16, dtype=bf16)),
+    lambda: ds_kernels.int8_linear(torch.zeros(2, 16, dtype=bf16), torch.zeros(8, 16, dtype=torch.int8), torch.ones(8)),
+    lambda: ds_kernels.mla_cache4_append(torch.zeros(1, 1, 512, dtype=bf16), torch.zeros(1, 1, 64, dtype=bf16),
+                                         LatentKVCache4(1, 4, "cpu"), torch.zeros(4, 64, dtype=bf16),
+                                         torch.zeros(4, 64, dtype=bf16)),
+    lambda: ds_kernels.mla_decode_attention4(torch.zeros(1, 16, 576, dtype=bf16), LatentKVCache4(1, 4, "cpu"), 1.0),
+    lambda: ds_kernels.mla_cache4_get(LatentKVCache4(1, 4, "cpu"), 1),
+    lambda: ds_kernels.mla_cache4_evict(LatentKVCache4(1, 4, "cpu"), 2),
+])
+def test_cpu_tensors_are_refused(call):
+    with pytest.raises(RuntimeError, match="CUDA"):
+        call()
+
+
+C = [P(256 * i) for i in range(1, 16)]
+
+
+@pytest.mark.parametrize("call,code", [
+    # int8: K a multiple of 16 up to 131072, N of 8, aligned rows, a workspace
+    (lambda L: L.ds_int8_quantize(C[0], 24, 2, 24, C[1], C[2], None), 1),
+    (lambda L: L.ds_int8_quantize(C[0], 8, 2, 16, C[1], C[2], None), 1),
+    (lambda L: L.ds_int8_quantize(C[0], 20, 2, 16, C[1], C[2], None), 1),
+    (lambda L: L.ds_int8_quantize(P(258), 16, 2, 16, C[1], C[2], None), 1),
+    (lambda L: L.ds_int8_quantize(None, 16, 2, 16, C[1], C[2], None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 24, C[1], C[2], C[3], 2, 8, 24, C[4], 1 << 20, None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], 2, 12, 16, C[4], 1 << 20, None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 131088, C[1], C[2], C[3], 2, 8, 131088, C[4], 1 << 20, None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 16, None, C[2], C[3], 2, 8, 16, C[4], 1 << 20, None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], 2, 8, 16, None, 0, None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], -1, 8, 16, C[4], 1 << 20, None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 16, P(520), C[2], C[3], 2, 8, 16, C[4], 1 << 20, None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], 2, 8, 16, C[4], 31, None), 5),
+    # append: slots a multiple of 64, room, aligned rows
+    (lambda L: L.ds_mla_cache4_append(C[0], 512, C[1], 64, 1, 1, None, C[2], C[3], 4, F(1e-6), C[4], C[5], C[6], C[7],
+                                      C[8], C[9], 1, 63, None), 1),
+    (lambda L: L.ds_mla_cache4_append(C[0], 512, C[1], 64, 1, 65, None, C[2], C[3], 4, F(1e-6), C[4], C[5], C[6], C[7],
+                                      C[8], C[9], 1, 64, None), 1),
+    (lambda L: L.ds_mla_cache4_append(C[0], 510, C[1], 64, 1, 1, None, C[2], C[3], 4, F(1e-6), C[4], C[5], C[6], C[7],
+                                      C[8], C[9], 1, 64, None), 1),
+    (lambda L: L.ds_mla_cache4_append(C[0], 512, C[1], 64, 1, 1, None, C[2], C[3], 0, F(1e-6), C[4], C[5], C[6], C[7],
+                                      C[8], C[9], 1, 64, None), 1),
+    (lambda L: L.ds_mla_cache4_append(C[0], 512, C[1], 64, 1, 1, None, C[2], C[3], 4, F(1e-6), C[4], None, C[6], C[7],
+                                      C[8], C[9], 1, 64, None), 1),
+    (lambda L: L.ds_mla_cache4_append(C[0], 512, C[1], 64, 1, 1, None, C[2], C[3], 4, F(1e-6), C[4], C[5], C[6], C[7],
+                                      C[8], C[9], 65536, 64, None), 1),
+    # get
+    (lambda L: L.ds_mla_cache4_get(C[0], C[1], C[2], 1, 64, 65, C[3], C[4], None), 1),
+    (lambda L: L.ds_mla_cache4_get(C[0], C[1], C[2], 1, 64, 4, None, C[4], None), 1),
+    # attention: heads, bounds, pointers
+    (lambda L: L.ds_mla_decode_attention4(C[0], 0, C[1], C[2], C[3], C[4], C[5], 1, 64, 4, F(1), 0, F(0), C[6], C[7],
+                                          1 << 20, None), 1),
+    (lambda L: L.ds_mla_decode_attention4(C[0], 129, C[1], C[2], C[3], C[4], C[5], 1, 64, 4, F(1), 0, F(0), C[6], C[7],
+                                          1 << 20, None), 1),
+    (lambda L: L.ds_mla_decode_attention4(C[0], 16, C[1], C[2], C[3], C[4], C[5], 1, 64, 65, F(1), 0, F(0), C[6], C[7],
+                                          1 << 20, None), 1),
+    (lambda L: L.ds_mla_decode_attention4(C[0], 16, C[1], C[2], C[3], C[4], C[5], 1, 64, 4, F(1), 0, F(0), C[6], None,
+                                          0, None), 1),
+    (lambda L: L.ds_mla_decode_attention4(P(260), 16, C[1], C[2], C[3], C[4], C[5], 1, 64, 4, F(1), 0, F(0), C[6], C[7],
+                                          1 << 20, None), 1),
+    # evict: budget, recent, the result shares all or nothing
+    (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 0, 0, *C[:6], 64, C[12], 1 << 20, None), 1),
+    (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 65, 0, *C[:6], 64, C[12], 1 << 20, None), 1),
+    (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 8, 9, *C[:6], 64, C[12], 1 << 20, None), 1),
+    (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 8, -1, *C[:6], 64, C[12], 1 << 20, None), 1),
+    (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 8, 0, C[0], *C[7:12], 64, C[12], 1 << 20, None), 1),
+    (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 8, 0, *C[6:11], C[5], 64, C[12], 1 << 20, None), 1),
+    (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 8, 0, *C[:6], 128, C[12], 1 << 20, None), 1),
+    (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 8, 0, *C[:6], 64, C[12], 16, None), 5),
+])
+def test_the_c_entries_refuse_before_any_launch(call, code):
+    assert call(lib()) == code
+    assert lib().ds_last_error().decode()
+
+
+def test_zero_size_calls_are_no_ops():
+    L = lib()
+    assert L.ds_int8_quantize(None, 16, 0, 16, None, None, None) == 0
+    assert L.ds_int8_linear(None, 16, None, None, None, 0, 8, 16, None, 0, None) == 0
+    assert L.ds_mla_cache4_get(None, None, None, 1, 64, 0, None, None, None) == 0
+
+
+def test_cache_construction_and_host_bounds():
+    for bad in (0, -1, 1.5):
+        with pytest.raises(ValueError):
+            LatentKVCache4(bad, 4, "cpu")
+        with pytest.raises(ValueError):
+            LatentKVCache4(1, bad, "cpu")
+    c = LatentKVCache4(2, 100, "cpu")
+    assert c.slots == 128 and c.codes.shape == (2, 128, 288) and c.scales.shape == (2, 5, 128)
+    assert c.memory_bytes == 2 * 128 * 310 + 16
+    assert c.current_len == 0 and c.remaining_capacity == 100
+    c._check_room(100, 100)
+    with pytest.raises(RuntimeError, match="overflow"):
+        c._check_room(101, 1000)
+    with pytest.raises(RuntimeError, match="RoPE"):
+        c._check_room(10, 9)
+    c._advance(60)
+    with pytest.raises(RuntimeError, match="overflow"):
+        c._check_room(41, 1000)
+    d = LatentKVCache4(2, 32, "cpu")
+    d._evicted(c, 32)
+    assert d.current_len == 32 and d._seen == 60
+    d.reset()
+    assert d.current_len == 0 and d._seen == 0
+
+
+def test_load_state_dict_checks_what_it_takes():
+    c = LatentKVCache4(2, 64, "cpu")
+    c.state.copy_(torch.tensor([[3, 64], [5, 64]]))
+    sd = c.state_dict()
+    d = LatentKVCache4(2, 200, "cpu")
+    d.load_state_dict(sd)
+    assert d.lens.tolist() == [3, 64] and d.next_pos.tolist() == [5, 64] and d.current_len == 64
+    e = LatentKVCache4(2, 200, "cpu")
+    e.load_state_dict({k: sd[k] for k in ("codes", "scales", "rstd", "lens")})
+    assert e.next_pos.tolist() == [3, 64] and e.pos[0, 190] == 190
+    for key in ("codes", "scales", "rstd", "lens"):
+        with pytest.raises(ValueError, match=key):
+            LatentKVCache4(2, 64, "cpu").load_state_dict({k: v for k, v in sd.items() if k != key})
+    with pytest.raises(ValueError, match="shape"):
+        LatentKVCache4(3, 64, "cpu").load_state_dict(sd)
+    with pytest.raises(ValueError, match="fit"):
+        LatentKVCache4(2, 63, "cpu").load_state_dict(sd)       # 64 tokens do not fit 63
+    sd["lens"] = torch.tensor([-1, 3], dtype=torch.int32)
+    with pytest.raises(ValueError, match="fit"):
+        LatentKVCache4(2, 64, "cpu").load_state_dict(sd)
