@@ -13,7 +13,11 @@
 // scale multiplies one probability instead of 128 values.  A group holding an infinity or a
 // NaN gets scale NaN.  state[0..batch) holds the sequences' lengths in slots,
 // state[batch..2 batch) their next positions (tokens seen, evicted ones included).
+#include <cuda_fp16.h>
+
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "kernels.cuh"
 #include "ptx.cuh"
@@ -213,141 +217,758 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- attention ------------------------------------------------------------------------------
-// Partials of (sequence, split): o f32 [batch][nsplit][heads][512], then maximum (log2 domain)
-// and sum f32 [batch][nsplit][2][heads].  With scores set, s * log2(e) of every slot goes to
-// scores [batch][heads][slots].
+// One query token per sequence over its slots, 16 heads (an MMA's M) at a time.
+//
+// Work is cut into units of (sequence, head tile, chunk of 128 slots), in that order, and CTA i
+// of G takes the units [i U / G, (i + 1) U / G): every CTA does the same number of chunks, whatever
+// the lengths, and none needs them on the host.  A CTA walks its range in segments of one
+// (sequence, head tile).  A segment that holds all its chunks writes the output; one that does not
+// (at most the first and the last of a CTA) leaves a partial, and merge_kernel joins those.
+//
+// Products run on mma.sync m16n8k16 (f16, f32 accumulators) with the 16 heads as M: tcgen05 would
+// take the heads as N = 16, where an instruction costs the same ~75 cycles as at N = 64 and the
+// cache as its M operand from shared memory, 68 of them a chunk, so about 40 cycles a slot and
+// SM against 17 here; and the operand would have to be written back to shared memory as 16 bits.
+// Here the codes go from shared memory to the fragments:
+//   * a nibble c in bits 0-3 of a half, under the exponent of 1024, is 1024 + c; in bits 4-7, under
+//     that of 64, 64 + c.  One AND-OR and one subtraction (1032, 72) make two operands code - 8,
+//     exactly, and one shift by 8 a word serves its other four codes: 9 instructions for 8
+//     codes.  (The nibble as it stands is the f16 subnormal c 2^-24 and would need no subtraction
+//     but the products then lose about ten bits when the tensor core aligns them; an offset left
+//     in the operands costs f32 bits of every sum.)
+//   * a group's scale multiplies the accumulator of its 128 dimensions (S) or the probability
+//     (O; warp w has the dimensions of group w), never the 128 values.
+//   * any bijection of an MMA's K index and of its N index serves, if both operands use it: K of
+//     S is the order in which a word's nibbles come out, and slot T(c, m) = (c ^ 2(m&1)) + 4m of
+//     16 sits at the m-th column pair of thread c, so that S fragments are P fragments after one
+//     16-byte store and every shared load is free of bank conflicts (288 bytes a row = 8 banks
+//     modulo 32: four slots that differ modulo 4 meet all banks).
+// q is scaled by a power of two per head, P by one per group and CTA, into f16's range (2^29 of
+// normal numbers below the largest), so P carries 11 bits where bf16 would carry 8.
+// The running maximum of a head is raised, and O rescaled, only when it grows by more than 2^4.
+constexpr int kChunk = 128;
+constexpr int kAttnThreads = 128;
+constexpr int kMergeParts = 1024;  // CTAs of the attention kernel, at most
+constexpr int kPLd = 144;  // floats; 16 modulo 32: conflict-free 16-byte rows
+constexpr uint32_t kStageBytes = kChunk * kRowBytes;                 // 36,864
+constexpr uint32_t kQLd = 2 * kQCols * 2 + 64;  // two heads; 64 modulo 128: conflict-free
+constexpr uint32_t kQBytes = 8 * kQLd;                               // 18,944
+constexpr uint32_t kPBytes = 16 * kPLd * 4;                          // 9,216
+constexpr uint32_t kFacBytes = kGroups * kChunk * 4;                 // 2,560, twice
+constexpr uint32_t kOffQ = 2 * kStageBytes;
+constexpr uint32_t kOffP = kOffQ + kQBytes;
+constexpr uint32_t kOffFac = kOffP + kPBytes;
+constexpr uint32_t kOffSmall = kOffFac + 2 * kFacBytes;
+struct AttnSmall {  // behind the tiles
+  unsigned long long bar[2];
+  float row[16];            // accumulator -> log2 of a weight
+  float wmax[4][16];
+  float wsum[4][16];
+  int scan[4];
+  int abort_flag;
+  int never_flag;
+};
+constexpr size_t kAttnSmem = kOffSmall + sizeof(AttnSmall);
+constexpr long long kTimeoutCycles = 4000000000LL;
+
 struct AttnParams {
   Cache c;
   const __nv_bfloat16* q;  // [batch, heads, 576]
-  int heads, nsplit, split_tokens;
+  __nv_bfloat16* out;      // [batch, heads * 512]
+  int heads, tiles;        // head tiles of 16
+  int max_chunks;          // of any sequence, as the host knows it
   float scale_log2;
-  float* part_o;
-  float* part_ml;
-  float* scores;
+  float* part_o;           // [G][2][16][512]
+  float* part_ml;          // [G][2][2][16]: maximum (log2), sum
+  float* lse;              // [batch, tiles * 16]: of the segments that held all their chunks
+  float* scores;           // [batch, tiles, max_chunks, 16, 128] (slots in fragment order) or null
+  int* status;
 };
 
-__global__ void __launch_bounds__(256) attend4_kernel(const AttnParams p) {
-  const Cache& c = p.c;
-  __shared__ float so[8][kLatent];
-  __shared__ float sm[8], sl[8];
-  const int bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads;
-  const int split = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int len = min(c.state[b], c.slots);
-  const int t0 = split * p.split_tokens, t1 = min(len, t0 + p.split_tokens);
-  const __nv_bfloat16* q = p.q + static_cast<int64_t>(bh) * kQCols;
-  float ql[16], qr[2], o[16];
+__device__ __forceinline__ int chunks_of(const Cache& c, int b, int max_chunks) {
+  const int len = min(max(__ldg(c.state + b), 0), c.slots);
+  return min((len + kChunk - 1) / kChunk, max_chunks);
+}
+// First unit of CTA i of n.
+__device__ __forceinline__ int64_t unit_start(int64_t units, int i, int n) { return units * i / n; }
+// Position of slot t (0..15) of a 16-slot group in fragment order, and back.
+__device__ __forceinline__ int frag_pos(int t) {
+  const int m = (t >> 2) & 3;
+  return (t & ~15) | (((t & 3) ^ (2 * (m & 1))) * 4 + m);
+}
+__device__ __forceinline__ int frag_slot(int pos) {
+  const int m = pos & 3, c = (pos >> 2) & 3;
+  return (pos & ~15) | ((c ^ (2 * (m & 1))) + 4 * m);
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The eight codes of a word, less 8, as four f16 pairs: pair j = nibbles j and j + 4.
+struct Masks {  // constants kept in registers, so that the AND-OR is one instruction
+  uint32_t m0, e0, s0, m1, e1, s1;
+};
+__device__ __forceinline__ Masks masks() {
+  Masks k;
+  asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(k.m0));
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(k.e0));  // 1024
+  asm volatile("mov.b32 %0, 0xE408E408;" : "=r"(k.s0));  // -1032
+  asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(k.m1));
+  asm volatile("mov.b32 %0, 0x54005400;" : "=r"(k.e1));  // 64
+  asm volatile("mov.b32 %0, 0xD480D480;" : "=r"(k.s1));  // -72
+  return k;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t e) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(m), "r"(e));
+  return r;
+}
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t x, uint32_t y) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+__device__ __forceinline__ void codes_f16(uint32_t w, const Masks& k, uint32_t (&o)[4]) {
+  const uint32_t v = w >> 8;
+  o[0] = add_f16x2(and_or(w, k.m0, k.e0), k.s0);
+  o[1] = add_f16x2(and_or(w, k.m1, k.e1), k.s1);
+  o[2] = add_f16x2(and_or(v, k.m0, k.e0), k.s0);
+  o[3] = add_f16x2(and_or(v, k.m1, k.e1), k.s1);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds_u2(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint4 lds_u4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+  const uint4 v = lds_u4(a);
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z),
+                     __uint_as_float(v.w));
+}
+
+// The sum of chunks over all sequences (times head tiles) and, for `unit` >= 0, the (sequence,
+// head tile, chunk) it is.  All threads of the block.
+__device__ __forceinline__ int64_t count_units(const AttnParams& p, int* scan) {
+  int64_t n = 0;
+  for (int b = threadIdx.x; b < p.c.batch; b += kAttnThreads) n += chunks_of(p.c, b, p.max_chunks);
+  int v = static_cast<int>(n);  // at most 65535 sequences of 2^26 / 128 chunks over 128 threads
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    ql[i] = __bfloat162float(q[16 * lane + i]) * p.scale_log2;
-    o[i] = 0.f;
-  }
-  qr[0] = __bfloat162float(q[kLatent + 2 * lane]) * p.scale_log2;
-  qr[1] = __bfloat162float(q[kLatent + 2 * lane + 1]) * p.scale_log2;
-  float m = -INFINITY, l = 0.f;
-  const __nv_bfloat16* sc = c.scales + static_cast<int64_t>(b) * kGroups * c.slots;
-  for (int t = t0 + warp; t < t1; t += 8) {
-    const int64_t row = static_cast<int64_t>(b) * c.slots + t;
-    const uint2 w = *reinterpret_cast<const uint2*>(c.codes + row * kRowBytes + 8 * lane);
-    const uint32_t wr = c.codes[row * kRowBytes + kLatent / 2 + lane];
-    const float sg = __bfloat162float(sc[static_cast<int64_t>(lane >> 3) * c.slots + t]) *
-                     c.rstd[row];
-    const float sr = __bfloat162float(sc[static_cast<int64_t>(4) * c.slots + t]);
-    float v[16], dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t x = ((i < 8 ? w.x : w.y) >> (4 * (i & 7))) & 15u;
-      v[i] = static_cast<float>(static_cast<int>(x) - 8) * sg;
-      dot = fmaf(v[i], ql[i], dot);
-    }
-    dot += sr * (static_cast<float>(static_cast<int>(wr & 15u) - 8) * qr[0] +
-                 static_cast<float>(static_cast<int>(wr >> 4) - 8) * qr[1]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    if (p.scores != nullptr && lane == 0)
-      p.scores[static_cast<int64_t>(bh) * c.slots + t] = dot;
-    const float mn = fmaxf(m, dot);
-    const float ref = mn == -INFINITY ? 0.f : mn;  // a NaN score stays one
-    const float f = exp2f(m - ref);
-    const float pr = exp2f(dot - ref);
-    l = l * f + pr;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = fmaf(pr, v[i], o[i] * f);
-    m = mn;
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) so[warp][16 * lane + i] = o[i];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   __syncthreads();
-  float M = -INFINITY, L = 0.f, f[8];
+  if ((threadIdx.x & 31) == 0) scan[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return (static_cast<int64_t>(scan[0]) + scan[1] + scan[2] + scan[3]) * p.tiles;
+}
+
+// The scales of slot t0 + threadIdx.x as they multiply the accumulators: scale * rstd for the
+// latent groups; 0 outside the segment, whatever the memory there holds.
+struct Factors {
+  uint32_t s[kGroups];
+  float rstd;
+};
+__device__ __forceinline__ Factors load_factors(const Cache& c, int b, int t, int t_end) {
+  Factors f;
+  const bool in = t < t_end;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) M = fmaxf(M, sm[i]);
+  for (int g = 0; g < kGroups; ++g)
+    f.s[g] = in ? __ldg(reinterpret_cast<const unsigned short*>(c.scales) +
+                        (static_cast<int64_t>(b) * kGroups + g) * c.slots + t)
+                : 0u;
+  f.rstd = in ? __ldg(c.rstd + static_cast<int64_t>(b) * c.slots + t) : 0.f;
+  return f;
+}
+__device__ __forceinline__ void store_factors(float* fac, const Factors& f) {
+  const int pos = frag_pos(threadIdx.x);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    f[i] = exp2f(sm[i] - (M == -INFINITY ? 0.f : M));
-    L += sl[i] * f[i];
-  }
-  const int64_t part = static_cast<int64_t>(b) * p.nsplit + split;
-  for (int d = threadIdx.x; d < kLatent; d += 256) {
-    float a = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a += so[i][d] * f[i];
-    p.part_o[(part * p.heads + h) * kLatent + d] = a;
-  }
+  for (int g = 0; g < 4; ++g) fac[g * kChunk + pos] = __uint_as_float(f.s[g] << 16) * f.rstd;
+  fac[4 * kChunk + pos] = __uint_as_float(f.s[4] << 16);
+}
+
+__global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const Cache& c = p.c;
+  AttnSmall& sm = *reinterpret_cast<AttnSmall*>(smem + kOffSmall);
+  const uint32_t s0 = ptx::smem_u32(smem);
+  const uint32_t sQ = s0 + kOffQ, sP = s0 + kOffP;
+  const uint32_t bar0 = ptx::smem_u32(sm.bar);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, cc = lane & 3;  // fragment row (or column) and column pair
   if (threadIdx.x == 0) {
-    p.part_ml[(part * 2) * p.heads + h] = M;
-    p.part_ml[(part * 2 + 1) * p.heads + h] = L;
+    ptx::mbar_init(bar0, 1);
+    ptx::mbar_init(bar0 + 8, 1);
+    sm.abort_flag = 0;
+    sm.never_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  const int64_t units = count_units(p, sm.scan);
+  int64_t u = unit_start(units, blockIdx.x, gridDim.x);
+  const int64_t u_end = unit_start(units, blockIdx.x + 1, gridDim.x);
+  if (u >= u_end) return;
+  // the sequence of unit u (a serial walk in blocks of 32 sequences, all warps alike)
+  int b = 0;
+  int64_t before = 0;  // units of the sequences before b
+  for (int base = 0;; base += 32) {
+    int n = base + lane < c.batch ? chunks_of(c, base + lane, p.max_chunks) : 0;
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + static_cast<int64_t>(incl) * p.tiles > u);
+    if (hit != 0u) {
+      const int l = __ffs(hit) - 1;
+      b = base + l;
+      before += static_cast<int64_t>(__shfl_sync(0xffffffffu, incl - n, l)) * p.tiles;
+      break;
+    }
+    before += static_cast<int64_t>(__shfl_sync(0xffffffffu, incl, 31)) * p.tiles;
+    if (base + 32 >= c.batch) return;  // not reached: u < units
+  }
+  const Masks km = masks();
+  uint32_t it = 0;  // chunks taken so far: stage it & 1, phase (it >> 1) & 1
+  bool first = true;
+  while (u < u_end) {
+    const int nch = chunks_of(c, b, p.max_chunks);
+    if (before + static_cast<int64_t>(nch) * p.tiles <= u) {  // on to the next sequence
+      before += static_cast<int64_t>(nch) * p.tiles;
+      ++b;
+      continue;
+    }
+    const int tile = static_cast<int>((u - before) / nch);
+    const int c0 = static_cast<int>((u - before) - static_cast<int64_t>(tile) * nch);
+    const int seg = static_cast<int>(min(static_cast<int64_t>(nch - c0), u_end - u));
+    const bool whole = c0 == 0 && seg == nch;
+    const int len = min(__ldg(c.state + b), c.slots);
+    const int nh = min(16, p.heads - tile * 16);
+    const uint8_t* codes = c.codes + static_cast<int64_t>(b) * c.slots * kRowBytes;
+    // the last chunk may reach past the slots: copy the rows that exist
+    auto load_chunk = [&](int i, uint32_t at) {
+      const int t0 = (c0 + i) * kChunk;
+      const uint32_t bytes = static_cast<uint32_t>(min(kChunk, c.slots - t0)) * kRowBytes;
+      const uint32_t bar = bar0 + 8 * (at & 1);
+      ptx::mbar_arrive_expect_tx(bar, bytes);
+      ptx::bulk_load_1d(s0 + (at & 1) * kStageBytes, codes + static_cast<int64_t>(t0) * kRowBytes,
+                        bytes, bar);
+    };
+    __syncthreads();  // the last segment is done with the tiles (and the barriers are set up)
+    if (threadIdx.x == 0) {
+      load_chunk(0, it);
+      if (seg > 1) load_chunk(1, it + 1);
+    }
+    Factors nf = load_factors(c, b, c0 * kChunk + threadIdx.x, len);
+    // Q as f16 fragments: warp w makes the heads r and r + 8 of rows r = 2w, 2w + 1, whose words
+    // lie side by side as an MMA takes them.  Lane l holds dimensions 16 l .. (and 2 of q_pe);
+    // k-step s of a quad of 64 dimensions takes pairs j = 2 (s & 1), + 1 of word s / 2.
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      const int r = warp * 2 + i;
+      uint32_t f[2][8], fr[2][2];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int h = r + 8 * hh;
+        const __nv_bfloat16* q =
+            p.q + (static_cast<int64_t>(b) * p.heads + tile * 16 + (h < nh ? h : 0)) * kQCols;
+        const uint4 x0 = __ldg(reinterpret_cast<const uint4*>(q) + 2 * lane);
+        const uint4 x1 = __ldg(reinterpret_cast<const uint4*>(q) + 2 * lane + 1);
+        const uint32_t x2 = __ldg(reinterpret_cast<const uint32_t*>(q + kLatent) + lane);
+        const uint32_t w[9] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w, x2};
+        float v[18];
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < 9; ++j) {
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+          amax = fmaxf(amax, fmaxf(fabsf(v[2 * j]), fabsf(v[2 * j + 1])));
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        // largest magnitude into [2^14, 2^15), by two factors: their product may pass 2^127
+        int e = 0;
+        if (amax > 0.f && amax <= 3.4e38f) e = 14 - ilogbf(amax);
+        const float fa = __int_as_float((127 + e / 2) << 23);
+        const float fb = h < nh ? __int_as_float((127 + e - e / 2) << 23) : 0.f;
+#pragma unroll
+        for (int n = 0; n < 18; ++n) v[n] = v[n] * fa * fb;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int n = (j & 3) + 8 * (j >> 2);
+          f[hh][j] = pack_f16(v[n], v[n + 4]);
+        }
+        // q_pe dimensions 2 l and 2 l + 1; their partners are two lanes up
+        fr[hh][0] = pack_f16(v[16], __shfl_down_sync(0xffffffffu, v[16], 2));
+        fr[hh][1] = pack_f16(v[17], __shfl_down_sync(0xffffffffu, v[17], 2));
+        if (lane == 0) sm.row[h] = ldexpf(p.scale_log2, -e);
+      }
+      uint8_t* row = smem + kOffQ + r * kQLd;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        *reinterpret_cast<uint4*>(row + (lane >> 2) * 256 + s * 64 + (lane & 3) * 16) =
+            make_uint4(f[0][2 * s], f[1][2 * s], f[0][2 * s + 1], f[1][2 * s + 1]);
+      if ((lane & 2) == 0)
+        *reinterpret_cast<uint4*>(row + 8 * 256 + ((lane & 4) >> 1 | (lane & 1)) * 64 +
+                                  (lane >> 3) * 16) =
+            make_uint4(fr[0][0], fr[1][0], fr[0][1], fr[1][1]);
+    }
+    store_factors(reinterpret_cast<float*>(smem + kOffFac) + (it & 1) * (kFacBytes / 4), nf);
+    __syncthreads();
+
+    float o[16][4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[j][k] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float pmax = 0.f, pscale = 1.f;  // of this warp's group: largest factor seen, power of two
+    const float row0 = sm.row[g], row1 = sm.row[g + 8];
+    for (int i = 0; i < seg; ++i, ++it) {
+      const int t0 = (c0 + i) * kChunk;
+      const bool ok = ptx::mbar_wait(bar0 + 8 * (it & 1), (it >> 1) & 1, &sm.abort_flag, p.status,
+                                     kTimeoutCycles, DS_ERR_TIMEOUT);
+      const uint32_t st = s0 + (it & 1) * kStageBytes;
+      const uint32_t sFac = s0 + kOffFac + (it & 1) * kFacBytes;
+      const bool more = i + 1 < seg;
+      if (more) nf = load_factors(c, b, t0 + kChunk + threadIdx.x, len);
+      // ---- S: this warp's 32 slots (four blocks of 8 columns) against 16 heads
+      float sc[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[k][j] = 0.f;
+      {
+        // column n = g of block k: slot T(g / 2, g & 1 | 2 (k & 1)) of 16-slot group 2 warp + k / 2
+        const int te = (((g >> 1) ^ (2 * (g & 1))) + 4 * (g & 1)) + warp * 32;
+        const uint32_t base = st + te * kRowBytes + cc * 8;
+        const uint32_t q0 = sQ + g * kQLd + cc * 16;
+        const uint32_t fac0 = sFac + (warp * 32 + 4 * cc) * 4;
+#pragma unroll 1
+        for (int gr = 0; gr < kGroups; ++gr) {
+          float acc[4][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[k][j] = 0.f;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (half == 1 && gr == 4) break;  // 64 dimensions of k_pe
+            const int qd = 2 * gr + half;
+            uint4 a[4];
+            uint2 x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = lds_u2(base + (k * 8) * kRowBytes + qd * 32);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) a[s] = lds_u4(q0 + qd * 256 + s * 64);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t v[4], w[4];
+              codes_f16(x[k].x, km, v);
+              mma_f16(acc[k], a[0].x, a[0].y, a[0].z, a[0].w, v[0], v[1]);
+              mma_f16(acc[k], a[1].x, a[1].y, a[1].z, a[1].w, v[2], v[3]);
+              codes_f16(x[k].y, km, w);
+              mma_f16(acc[k], a[2].x, a[2].y, a[2].z, a[2].w, w[0], w[1]);
+              mma_f16(acc[k], a[3].x, a[3].y, a[3].z, a[3].w, w[2], w[3]);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // the group is complete: times its slots' factors
+            const float2 f = lds_f2(fac0 + (gr * kChunk + (k >> 1) * 16 + 2 * (k & 1)) * 4);
+            sc[k][0] = fmaf(acc[k][0], f.x, sc[k][0]);
+            sc[k][1] = fmaf(acc[k][1], f.y, sc[k][1]);
+            sc[k][2] = fmaf(acc[k][2], f.x, sc[k][2]);
+            sc[k][3] = fmaf(acc[k][3], f.y, sc[k][3]);
+          }
+        }
+      }
+      // column pair cc of block k: slots T(cc, 2 (k & 1)) and T(cc, 2 (k & 1) + 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        sc[k][0] *= row0;
+        sc[k][1] *= row0;
+        sc[k][2] *= row1;
+        sc[k][3] *= row1;
+      }
+      if (t0 + kChunk > len) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (t0 + warp * 32 + k * 8 + (cc ^ (2 * j)) + 4 * j >= len)
+              sc[k][j] = sc[k][2 + j] = -INFINITY;
+      }
+      float mx0 = sc[0][0], mx1 = sc[0][2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        mx0 = fmaxf(mx0, fmaxf(sc[k][0], sc[k][1]));
+        mx1 = fmaxf(mx1, fmaxf(sc[k][2], sc[k][3]));
+      }
+      mx0 = fmaxf(mx0, -INFINITY);  // (all NaN: a maximum must not be one)
+      mx1 = fmaxf(mx1, -INFINITY);
+      if (p.scores != nullptr) {
+        float* dst = p.scores +
+                     ((static_cast<int64_t>(b) * p.tiles + tile) * p.max_chunks + c0 + i) * 16 * kChunk +
+                     warp * 32 + 4 * cc;
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          *reinterpret_cast<float4*>(dst + g * kChunk + 8 * k) =
+              make_float4(sc[k][0], sc[k][1], sc[k + 1][0], sc[k + 1][1]);
+          *reinterpret_cast<float4*>(dst + (g + 8) * kChunk + 8 * k) =
+              make_float4(sc[k][2], sc[k][3], sc[k + 1][2], sc[k + 1][3]);
+        }
+      }
+#pragma unroll
+      for (int d = 2; d > 0; d >>= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+      }
+      if (cc == 0) {
+        sm.wmax[warp][g] = mx0;
+        sm.wmax[warp][g + 8] = mx1;
+      }
+      // barrier A: the maxima are there; every warp is done with the last chunk's P and codes
+      if (!__syncthreads_and(ok)) {  // a load did not arrive in time: wait (bounded) and leave
+        if (threadIdx.x == 0) {
+          ptx::mbar_wait(bar0 + 8 * (it & 1), (it >> 1) & 1, &sm.never_flag, p.status,
+                         kTimeoutCycles, DS_ERR_TIMEOUT);
+          if (more && i == 0)  // (later chunks are asked for behind this barrier)
+            ptx::mbar_wait(bar0 + 8 * ((it + 1) & 1), ((it + 1) >> 1) & 1, &sm.never_flag, p.status,
+                           kTimeoutCycles, DS_ERR_TIMEOUT);
+        }
+        return;
+      }
+      if (threadIdx.x == 0 && i >= 1 && more) load_chunk(i + 1, it + 1);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        mx0 = fmaxf(mx0, sm.wmax[w][g]);
+        mx1 = fmaxf(mx1, sm.wmax[w][g + 8]);
+      }
+      const float n0 = mx0 > m0 + 4.f ? mx0 : m0, n1 = mx1 > m1 + 4.f ? mx1 : m1;
+      if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
+        const float f0 = ptx::ex2(m0 - (n0 == -INFINITY ? 0.f : n0));
+        const float f1 = ptx::ex2(m1 - (n1 == -INFINITY ? 0.f : n1));
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          o[j][0] *= f0;
+          o[j][1] *= f0;
+          o[j][2] *= f1;
+          o[j][3] *= f1;
+        }
+        l0 *= f0;
+        l1 *= f1;
+        m0 = n0;
+        m1 = n1;
+      }
+      const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+#pragma unroll
+      for (int k = 0; k < 4; k += 2) {
+        float4 a, bb;
+        a.x = ptx::ex2(sc[k][0] - r0);
+        a.y = ptx::ex2(sc[k][1] - r0);
+        a.z = ptx::ex2(sc[k + 1][0] - r0);
+        a.w = ptx::ex2(sc[k + 1][1] - r0);
+        bb.x = ptx::ex2(sc[k][2] - r1);
+        bb.y = ptx::ex2(sc[k][3] - r1);
+        bb.z = ptx::ex2(sc[k + 1][2] - r1);
+        bb.w = ptx::ex2(sc[k + 1][3] - r1);
+        l0 += (a.x + a.y) + (a.z + a.w);
+        l1 += (bb.x + bb.y) + (bb.z + bb.w);
+        float* dst = reinterpret_cast<float*>(smem + kOffP) + warp * 32 + 8 * k + 4 * cc;
+        *reinterpret_cast<float4*>(dst + g * kPLd) = a;
+        *reinterpret_cast<float4*>(dst + (g + 8) * kPLd) = bb;
+      }
+      if (more)
+        store_factors(reinterpret_cast<float*>(smem + kOffFac) + ((it + 1) & 1) * (kFacBytes / 4), nf);
+      __syncthreads();  // barrier B: P and the next chunk's factors are there
+      // ---- O += P V over the 128 dimensions of group `warp`
+      {
+        const uint32_t fw = sFac + warp * kChunk * 4;
+        const float4 fl = lds_f4(fw + lane * 16);
+        float fm = fmaxf(fmaxf(fl.x, fl.y), fmaxf(fl.z, fl.w));
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) fm = fmaxf(fm, __shfl_xor_sync(0xffffffffu, fm, d));
+        if (fm > 16.f * pmax && fm <= 3.4e38f) {  // (warp-uniform) largest factor to [2^6, 2^7)
+          const float ns = ldexpf(1.f, max(-100, min(100, 6 - ilogbf(fm))));
+          if (pmax > 0.f) {
+            const float f = ns / pscale;  // powers of two
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) o[j][k] *= f;
+          }
+          pscale = ns;
+          pmax = fm;
+        }
+        // this group's factors, scaled, back in place: no other warp reads them any more
+        __syncwarp();
+        *reinterpret_cast<float4*>(smem + (fw - s0) + lane * 16) =
+            make_float4(fl.x * pscale, fl.y * pscale, fl.z * pscale, fl.w * pscale);
+        __syncwarp();
+        // B: slots T(cc, 0..3) of the 16, dimensions 128 warp + 16 g + 0..15
+        const uint32_t v0 = st + cc * kRowBytes + warp * 64 + g * 8;
+        const uint32_t v1 = st + ((cc ^ 2) + 4) * kRowBytes + warp * 64 + g * 8;
+        const uint32_t pr = sP + (g * kPLd + 4 * cc) * 4;
+#pragma unroll 2
+        for (int kk = 0; kk < 8; ++kk) {
+          const float4 p0 = lds_f4(pr + kk * 64);
+          const float4 p1 = lds_f4(pr + 8 * kPLd * 4 + kk * 64);
+          const float4 f = lds_f4(fw + (kk * 16 + 4 * cc) * 4);
+          const uint2 x0 = lds_u2(v0 + (kk * 16) * kRowBytes);
+          const uint2 x1 = lds_u2(v1 + (kk * 16) * kRowBytes);
+          const uint2 x2 = lds_u2(v0 + (kk * 16 + 8) * kRowBytes);
+          const uint2 x3 = lds_u2(v1 + (kk * 16 + 8) * kRowBytes);
+          const uint32_t a0 = pack_f16(p0.x * f.x, p0.y * f.y), a1 = pack_f16(p1.x * f.x, p1.y * f.y);
+          const uint32_t a2 = pack_f16(p0.z * f.z, p0.w * f.w), a3 = pack_f16(p1.z * f.z, p1.w * f.w);
+#pragma unroll
+          for (int wi = 0; wi < 2; ++wi) {
+            const uint32_t y0 = wi ? x0.y : x0.x, y1 = wi ? x1.y : x1.x;
+            const uint32_t y2 = wi ? x2.y : x2.x, y3 = wi ? x3.y : x3.x;
+#pragma unroll
+            for (int up = 0; up < 2; ++up) {
+              uint32_t b0[4], b1[4];
+              codes_f16(__byte_perm(y0, y1, up ? 0x7632 : 0x5410), km, b0);
+              codes_f16(__byte_perm(y2, y3, up ? 0x7632 : 0x5410), km, b1);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                mma_f16(o[8 * wi + 4 * up + j], a0, a1, a2, a3, b0[j], b1[j]);
+            }
+          }
+        }
+      }
+    }
+    // ---- the segment's result
+#pragma unroll
+    for (int d = 2; d > 0; d >>= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+    }
+    if (cc == 0) {
+      sm.wsum[warp][g] = l0;
+      sm.wsum[warp][g + 8] = l1;
+    }
+    __syncthreads();
+    l0 = (sm.wsum[0][g] + sm.wsum[1][g]) + (sm.wsum[2][g] + sm.wsum[3][g]);
+    l1 = (sm.wsum[0][g + 8] + sm.wsum[1][g + 8]) + (sm.wsum[2][g + 8] + sm.wsum[3][g + 8]);
+    const float unit = 1.f / pscale;
+    const int slot = blockIdx.x * 2 + (first ? 0 : 1);
+    float f0 = unit, f1 = unit;
+    if (whole) {
+      f0 = l0 == 0.f ? 0.f : unit / l0;
+      f1 = l1 == 0.f ? 0.f : unit / l1;
+    }
+    if (warp == 0 && cc == 0) {
+      if (whole) {
+        if (p.lse != nullptr) {
+          float* lse = p.lse + (static_cast<int64_t>(b) * p.tiles + tile) * 16;
+          lse[g] = m0 + log2f(l0);
+          lse[g + 8] = m1 + log2f(l1);
+        }
+      } else {
+        float* ml = p.part_ml + static_cast<int64_t>(slot) * 32;
+        ml[g] = m0;
+        ml[g + 8] = m1;
+        ml[16 + g] = l0;
+        ml[16 + g + 8] = l1;
+      }
+    }
+    // block j holds dimensions 128 warp + 16 (2 cc) + j and 16 (2 cc + 1) + j
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int h = g + 8 * r;
+      const float f = r ? f1 : f0;
+      if (whole && h >= nh) continue;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int d = 128 * warp + 16 * (2 * cc + k);
+        if (whole) {
+          __nv_bfloat16* dst =
+              p.out + (static_cast<int64_t>(b) * p.heads + tile * 16 + h) * kLatent + d;
+#pragma unroll
+          for (int j = 0; j < 16; j += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const __nv_bfloat162 v = __floats2bfloat162_rn(o[j + 2 * x][2 * r + k] * f,
+                                                             o[j + 2 * x + 1][2 * r + k] * f);
+              w[x] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            *reinterpret_cast<uint4*>(dst + j) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+          float* dst = p.part_o + (static_cast<int64_t>(slot) * 16 + h) * kLatent + d;
+#pragma unroll
+          for (int j = 0; j < 16; j += 4)
+            *reinterpret_cast<float4*>(dst + j) =
+                make_float4(o[j][2 * r + k] * f, o[j + 1][2 * r + k] * f,
+                            o[j + 2][2 * r + k] * f, o[j + 3][2 * r + k] * f);
+        }
+      }
+    }
+    u += seg;
+    first = false;
   }
 }
 
-// Merge the splits of each (sequence, head); lse[b, h] = M + log2 L for the weights.
-__global__ void __launch_bounds__(128)
-    merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int nsplit,
-                 int heads, __nv_bfloat16* __restrict__ out, float* __restrict__ lse) {
-  const int64_t b = blockIdx.x / heads;
-  const int h = blockIdx.x - static_cast<int>(b) * heads;
+// The CTAs that hold the units of (sequence b, head tile): first and last, and the unit range.
+struct Owners {
+  int64_t units, u0, u1;
+  int first, last;
+};
+__device__ __forceinline__ Owners owners_of(const AttnParams& p, int b, int tile, int ctas,
+                                            int* scan) {
+  int64_t mine = 0;
+  int n = 0;
+  for (int x = threadIdx.x; x < p.c.batch; x += kAttnThreads) {
+    const int k = chunks_of(p.c, x, p.max_chunks);
+    mine += k;
+    if (x < b) n += k;
+  }
+  int v = static_cast<int>(mine);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    v += __shfl_xor_sync(0xffffffffu, v, d);
+    n += __shfl_xor_sync(0xffffffffu, n, d);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    scan[threadIdx.x >> 5] = v;
+    scan[4 + (threadIdx.x >> 5)] = n;
+  }
+  __syncthreads();
+  Owners w;
+  w.units = (static_cast<int64_t>(scan[0]) + scan[1] + scan[2] + scan[3]) * p.tiles;
+  const int64_t before =
+      (static_cast<int64_t>(scan[4]) + scan[5] + scan[6] + scan[7]) * p.tiles;
+  const int nch = chunks_of(p.c, b, p.max_chunks);
+  w.u0 = before + static_cast<int64_t>(tile) * nch;
+  w.u1 = w.u0 + nch;
+  w.first = w.last = 0;
+  if (nch > 0) {
+    // CTA of unit u: the largest i with floor(units i / ctas) <= u
+    w.first = static_cast<int>(((w.u0 + 1) * ctas - 1) / w.units);
+    w.last = static_cast<int>((w.u1 * ctas - 1) / w.units);
+  }
+  return w;
+}
+// The partial of CTA i that belongs to units [u0, ..): its first segment if it starts inside.
+// -1: a CTA without units (fewer units than CTAs).
+__device__ __forceinline__ int part_slot(const Owners& w, int i, int ctas) {
+  const int64_t u = unit_start(w.units, i, ctas);
+  if (u == unit_start(w.units, i + 1, ctas)) return -1;
+  return 2 * i + (u >= w.u0 ? 0 : 1);
+}
+
+// Joins the partials of one (sequence, head) a block: output, and lse (log2 of the weights' sum)
+// where it is wanted; zeros for a sequence without slots.
+__global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p, int ctas) {
+  __shared__ int scan[8];
+  __shared__ float sw[kMergeParts], sred[8];
+  __shared__ int sslot[kMergeParts];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = static_cast<int>(blockIdx.x) / p.heads;
+  const int h = static_cast<int>(blockIdx.x) - b * p.heads;
+  const int r = h & 15;
+  const Owners w = owners_of(p, b, h >> 4, ctas, scan);
+  __nv_bfloat16* o = p.out + static_cast<int64_t>(blockIdx.x) * kLatent;
+  if (w.u1 == w.u0) {
+    reinterpret_cast<uint2*>(o)[tid] = make_uint2(0u, 0u);
+    return;
+  }
+  if (w.first == w.last) return;  // written by the attention kernel
+  const int n = w.last - w.first + 1;  // at most kMergeParts: the grid's CTAs
   float M = -INFINITY;
-  for (int s = 0; s < nsplit; ++s)
-    M = fmaxf(M, __ldg(part_ml + (b * nsplit + s) * 2 * heads + h));
+  for (int i = tid; i < n; i += kAttnThreads) {
+    const int s = part_slot(w, w.first + i, ctas);
+    sslot[i] = s;
+    const float m = s >= 0 ? __ldg(p.part_ml + static_cast<int64_t>(s) * 32 + r) : -INFINITY;
+    sw[i] = m;
+    M = fmaxf(M, m);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  if (lane == 0) sred[warp] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(sred[0], sred[1]), fmaxf(sred[2], sred[3]));
   const float ref = M == -INFINITY ? 0.f : M;
   float L = 0.f;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < nsplit; ++s) {
-    const float* ml = part_ml + (b * nsplit + s) * 2 * heads;
-    const float ls = __ldg(ml + heads + h);
-    if (ls == 0.f) continue;
-    const float w = ptx::ex2(__ldg(ml + h) - ref);
-    L = fmaf(w, ls, L);
-    const float* po = part_o + ((b * nsplit + s) * heads + h) * kLatent;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] = fmaf(w, __ldg(po + k * 128 + threadIdx.x), acc[k]);
+  for (int i = tid; i < n; i += kAttnThreads) {
+    const int s = sslot[i];
+    const float f = s >= 0 ? ptx::ex2(sw[i] - ref) : 0.f;
+    sw[i] = f;
+    if (s >= 0) L = fmaf(f, __ldg(p.part_ml + static_cast<int64_t>(s) * 32 + 16 + r), L);
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;  // no slot: zeros
-  __nv_bfloat16* o = out + (b * heads + h) * kLatent;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) o[k * 128 + threadIdx.x] = __float2bfloat16_rn(acc[k] * inv);
-  if (lse != nullptr && threadIdx.x == 0) lse[b * heads + h] = M + log2f(L);
+  for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+  if (lane == 0) sred[4 + warp] = L;
+  __syncthreads();
+  L = (sred[4] + sred[5]) + (sred[6] + sred[7]);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const int s = sslot[i];
+    if (s < 0) continue;
+    const float f = sw[i];
+    const float4 v = __ldg(
+        reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(s) * 16 + r) * kLatent) + tid);
+    a.x = fmaf(f, v.x, a.x);
+    a.y = fmaf(f, v.y, a.y);
+    a.z = fmaf(f, v.z, a.z);
+    a.w = fmaf(f, v.w, a.w);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv);
+  const __nv_bfloat162 y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+  reinterpret_cast<uint2*>(o)[tid] = make_uint2(*reinterpret_cast<const uint32_t*>(&x),
+                                                *reinterpret_cast<const uint32_t*>(&y));
+  if (p.lse != nullptr && tid == 0)
+    p.lse[(static_cast<int64_t>(b) * p.tiles + (h >> 4)) * 16 + r] = M + log2f(L);
 }
 
-// mass[b, t] = decay * mass[b, t] + sum_h 2^(s_h(t) - lse_h) (decay 0: not read), t < length.
-__global__ void __launch_bounds__(256)
-    mass_kernel(Cache c, const float* __restrict__ scores, const float* __restrict__ lse,
-                int heads, float decay) {
-  __shared__ float sl[kMaxHeads];
-  const int b = blockIdx.y;
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  const int len = min(c.state[b], c.slots);
-  if (blockIdx.x * 256 >= len) return;
-  for (int h = threadIdx.x; h < heads; h += 256) sl[h] = lse[static_cast<int64_t>(b) * heads + h];
+// mass[t] = decay mass[t] + sum_h 2^(s_h(t) - lse_h); one chunk of one sequence a block.
+__global__ void __launch_bounds__(kChunk) mass_kernel(const AttnParams p, float decay) {
+  __shared__ float slse[kMaxHeads];
+  const int tid = threadIdx.x, b = blockIdx.y, chunk = blockIdx.x;
+  const int len = min(__ldg(p.c.state + b), p.c.slots);
+  if (chunk * kChunk >= len) return;
+  if (tid < p.heads) slse[tid] = p.lse[static_cast<int64_t>(b) * p.tiles * 16 + tid];
   __syncthreads();
-  if (t >= len) return;
-  const float* s = scores + static_cast<int64_t>(b) * heads * c.slots + t;
+  const int t = chunk * kChunk + frag_slot(tid);
   float a = 0.f;
-  for (int h = 0; h < heads; ++h) a += ptx::ex2(__ldg(s + static_cast<int64_t>(h) * c.slots) - sl[h]);
-  float* m = c.mass + static_cast<int64_t>(b) * c.slots + t;
+  for (int tile = 0; tile < p.tiles; ++tile) {
+    const float* s = p.scores +
+                     ((static_cast<int64_t>(b) * p.tiles + tile) * p.max_chunks + chunk) * 16 * kChunk + tid;
+    if (p.heads >= 16 * tile + 16) {
+      float v[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = __ldg(s + r * kChunk);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) a += ptx::ex2(v[r] - slse[tile * 16 + r]);
+    } else {
+      for (int r = 0; r < p.heads - 16 * tile; ++r)
+        a += ptx::ex2(__ldg(s + r * kChunk) - slse[tile * 16 + r]);
+    }
+  }
+  if (t >= len) return;
+  float* m = p.c.mass + static_cast<int64_t>(b) * p.c.slots + t;
   *m = decay != 0.f ? fmaf(decay, *m, a) : a;
 }
 
@@ -503,15 +1124,6 @@ int check_cache(const Cache& c, const char* op) {
   return DS_OK;
 }
 
-int split_count(int batch, int heads, int max_len, int num_sms, int* tokens) {
-  (void)batch;
-  (void)heads;
-  (void)num_sms;
-  *tokens = 1024;
-  const int n = (max_len + *tokens - 1) / *tokens;
-  return n < 1 ? 1 : n;
-}
-
 struct AttnBuffers {
   float* part_o;
   float* part_ml;
@@ -519,13 +1131,26 @@ struct AttnBuffers {
   float* lse;
 };
 
-void carve_attn(Carve& w, AttnBuffers* b, int batch, int heads, int slots, int nsplit,
-                bool mass) {
-  b->part_o = w.take<float>(static_cast<size_t>(batch) * nsplit * heads * kLatent);
-  b->part_ml = w.take<float>(static_cast<size_t>(batch) * nsplit * 2 * heads);
-  b->scores = mass ? w.take<float>(static_cast<size_t>(batch) * heads * slots) : nullptr;
-  b->lse = mass ? w.take<float>(static_cast<size_t>(batch) * heads) : nullptr;
+// CTAs of the attention kernel: two per SM, no more than there can be chunks.
+int attn_ctas(int batch, int tiles, int max_chunks, int num_sms) {
+  const int64_t units = static_cast<int64_t>(batch) * tiles * max_chunks;
+  const int most = std::min(2 * num_sms, kMergeParts);
+  return static_cast<int>(units < most ? (units < 1 ? 1 : units) : most);
 }
+
+void carve_attn(Carve& w, AttnBuffers* b, int batch, int heads, int max_len, int num_sms,
+                bool mass) {
+  const int tiles = (heads + 15) / 16, chunks = (max_len + kChunk - 1) / kChunk;
+  const size_t parts = 2 * static_cast<size_t>(attn_ctas(batch, tiles, chunks, num_sms));
+  b->part_o = w.take<float>(parts * 16 * kLatent);
+  b->part_ml = w.take<float>(parts * 32);
+  b->lse = mass ? w.take<float>(static_cast<size_t>(batch) * tiles * 16) : nullptr;
+  b->scores =
+      mass ? w.take<float>(static_cast<size_t>(batch) * tiles * chunks * 16 * kChunk) : nullptr;
+}
+
+bool g_attr_set[64] = {};
+std::mutex g_attr_mutex;
 
 int launch_append(const Cache& c, const void* lat, int64_t lat_ld, const void* kpe,
                   int64_t kpe_ld, int64_t src_bstride, int n_new, const int32_t* new_lens,
@@ -552,27 +1177,41 @@ int launch_attention(const Cache& c, const void* q, int heads, int max_len, floa
   DeviceInfo di;
   DS_TRY(device_info(&di));
   AttnParams p{};
-  p.nsplit = split_count(c.batch, heads, max_len, di.num_sms, &p.split_tokens);
-  Carve w(workspace, ws_bytes);
-  AttnBuffers b{};
-  carve_attn(w, &b, c.batch, heads, c.slots, p.nsplit, accumulate != 0);
-  if (!w.ok())
-    return fail(DS_ERR_WORKSPACE, "mla_decode_attention4: workspace needs %zu bytes", w.used);
   p.c = c;
   p.q = static_cast<const __nv_bfloat16*>(q);
+  p.out = static_cast<__nv_bfloat16*>(out);
   p.heads = heads;
+  p.tiles = (heads + 15) / 16;
+  p.max_chunks = (max_len + kChunk - 1) / kChunk;
   p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
+  Carve w(workspace, ws_bytes);
+  AttnBuffers b{};
+  carve_attn(w, &b, c.batch, heads, max_len, di.num_sms, accumulate != 0);
+  if (!w.ok())
+    return fail(DS_ERR_WORKSPACE, "mla_decode_attention4: workspace needs %zu bytes", w.used);
   p.part_o = b.part_o;
   p.part_ml = b.part_ml;
   p.scores = b.scores;
-  attend4_kernel<<<dim3(c.batch * heads, p.nsplit), 256, 0, s>>>(p);
-  DS_LAUNCH_CHECK("attend4_kernel");
-  merge_kernel<<<c.batch * heads, 128, 0, s>>>(b.part_o, b.part_ml, p.nsplit, heads,
-                                               static_cast<__nv_bfloat16*>(out), b.lse);
+  p.lse = b.lse;
+  p.status = device_status_ptr();
+  if (p.status == nullptr) return fail(DS_ERR_CUDA, "device status word unavailable");
+  {
+    std::lock_guard<std::mutex> lock(g_attr_mutex);
+    if (!g_attr_set[di.device]) {
+      DS_CUDA(cudaFuncSetAttribute(attend4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(kAttnSmem)));
+      g_attr_set[di.device] = true;
+    }
+  }
+  const int ctas = attn_ctas(c.batch, p.tiles, p.max_chunks, di.num_sms);
+  if (max_len > 0) {
+    attend4_kernel<<<ctas, kAttnThreads, kAttnSmem, s>>>(p);
+    DS_LAUNCH_CHECK("attend4_kernel");
+  }
+  merge_kernel<<<c.batch * heads, kAttnThreads, 0, s>>>(p, ctas);
   DS_LAUNCH_CHECK("merge_kernel");
   if (accumulate && max_len > 0) {
-    mass_kernel<<<dim3((max_len + 255) / 256, c.batch), 256, 0, s>>>(c, b.scores, b.lse, heads,
-                                                                     decay);
+    mass_kernel<<<dim3(p.max_chunks, c.batch), kChunk, 0, s>>>(p, decay);
     DS_LAUNCH_CHECK("mass_kernel");
   }
   return DS_OK;
@@ -630,14 +1269,13 @@ int ds_mla_cache4_get(const void* codes, const void* scales_bf16, const int32_t*
 
 size_t ds_mla_decode_attention4_workspace_size(int batch, int heads, int slots, int max_len,
                                                int accumulate) {
+  (void)slots;
   if (batch <= 0 || heads <= 0 || max_len < 0) return 0;
   ds::DeviceInfo di;
   if (ds::device_info(&di) != DS_OK) return 0;
-  int tokens;
-  const int ns = ds::c4::split_count(batch, heads, max_len, di.num_sms, &tokens);
   ds::Carve w(nullptr, 0);
   ds::c4::AttnBuffers b{};
-  ds::c4::carve_attn(w, &b, batch, heads, slots, ns, accumulate != 0);
+  ds::c4::carve_attn(w, &b, batch, heads, max_len, di.num_sms, accumulate != 0);
   return ds::align_up(w.used, 256);
 }
 

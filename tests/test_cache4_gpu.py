@@ -3,8 +3,12 @@ their definitions in 64 bits on the CPU.
 
 Codes, scales, positions and what eviction keeps are exact and compared bit for bit.
 
-Attention: with A = sum_t p |v| (per output), the probabilities times a group's scale are rounded
-once to bf16 (2^-8 of A) and the output once (2^-8 |o|).  A score is a sum of 576 products, exact
+Attention: with A = sum_t p |v| (per output), the probabilities times a group's factor (scale *
+rstd) are rounded once to 16 bits (2^-8 of A at most) and the output once (2^-8 |o|).  In f16 that
+first rounding has a floor: the products are scaled so that the group's largest factor F meets [2^6,
+2^7) when it is set, and weights are taken against a maximum that the largest weight reaches, so a
+weight p (of a sum of 1 or more) becomes p f 2^6 / F or more, and below 2^-14 its error is 2^-25:
+2^-31 F of a value's factor, 7 of them a code at most: n 7 F 2^-31 for n slots.  A score is a sum of 576 products, exact
 one by one, added up in f32 by at most 40 dependent additions of 2^-23 relative to sum |q k|; it
 and the exponentials (2^-21) move a probability by twice that at most (numerator and sum).
 """
@@ -95,7 +99,9 @@ def attend64(st, q, lens, scale=SCALE):
         size = scale * qd.abs() @ k.abs().t()
         moved = 2 * (40 * 2.0 ** -23 * size.amax(1, keepdim=True) + 2.0 ** -21)
         o, a = p @ lat, p @ lat.abs()
-        out[b], tol[b] = o.flatten(), (2.0 ** -8 * (o.abs() + a) + moved * a).flatten()
+        fac = (st["scales"][b, :4, :n].double() * st["rstd"][b, :n].double()).amax(1).repeat_interleave(128)
+        out[b] = o.flatten()
+        tol[b] = (2.0 ** -8 * (o.abs() + a) + moved * a + n * 7 * fac * 2.0 ** -31).flatten()
         mass[b, :n], mtol[b, :n] = p.sum(0), (p * moved).sum(0) + 2.0 ** -23 * p.sum(0) * H
     return out, tol, mass, mtol
 
