@@ -9,7 +9,12 @@
 // of a candidate n, which decides the neighbour and the ties (x = a/2 is one: 63.5).
 // Product: out_mn = bf16((sum_k q_mk w_nk) * (s_m * ws_n)); the sum is exact in 32 bits
 // (K <= 131072), so no split or order of it changes the result.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "kernels.cuh"
 #include "ptx.cuh"
@@ -32,105 +37,641 @@ __device__ __forceinline__ int quant1(float x, float a, float r) {
   return static_cast<int>(n);
 }
 
-// One warp per row when rows are short, one block otherwise (rows of 16-byte vectors).
+__device__ __forceinline__ float abs_max8(const uint4& v, float a) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float lo = fabsf(__uint_as_float(w[i] << 16)), hi = fabsf(__uint_as_float(w[i] & 0xFFFF0000u));
+    // a NaN counts as infinity: fmaxf would pass it over
+    a = fmaxf(a, fmaxf(lo <= 3.4e38f ? lo : INFINITY, hi <= 3.4e38f ? hi : INFINITY));
+  }
+  return a;
+}
+
+struct RowScale {
+  float up, au, r;  // x up / au * 127; r ~ 127 / au, 0 for an empty or non-finite row
+};
+__device__ __forceinline__ RowScale row_scale(float a) {
+  RowScale s;
+  // subnormal and tiny rows are scaled up by a power of two, so that 127 / a stays finite,
+  // huge ones down, so that 127 x does
+  s.up = a < 1e-30f ? 0x1p100f : a > 1e30f ? 0x1p-100f : 1.f;
+  s.au = a * s.up;
+  s.r = a <= 3.4e38f && s.au > 0.f ? 127.f / s.au : 0.f;
+  return s;
+}
+__device__ __forceinline__ uint2 quant8(const uint4& v, const RowScale& s) {
+  if (s.r == 0.f) return make_uint2(0u, 0u);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int lo = quant1(__uint_as_float(w[i] << 16) * s.up, s.au, s.r);
+    const int hi = quant1(__uint_as_float(w[i] & 0xFFFF0000u) * s.up, s.au, s.r);
+    o[i >> 1] |= ((lo & 0xFF) | ((hi & 0xFF) << 8)) << (16 * (i & 1));
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+// TPR threads a row (a warp, or the block of 256); a row of at most TPR * V 16-byte vectors
+// stays in registers between the maximum and the quotients, a longer one is read twice.
+template <int TPR, int V>
 __global__ void __launch_bounds__(256)
     quantize_kernel(const uint4* __restrict__ x, int64_t ld8, int rows, int k8,
                     uint2* __restrict__ q, float* __restrict__ scale) {
   __shared__ float red[8];
-  const int row = blockIdx.x;
+  ptx::pdl_launch_dependents();
+  const int row = TPR == 32 ? static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5)
+                            : static_cast<int>(blockIdx.x);
+  if (TPR == 32 && row >= rows) return;
+  const int t = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
   const uint4* src = x + static_cast<int64_t>(row) * ld8;
-  float a = 0.f;
-  bool bad = false;
-  for (int c = threadIdx.x; c < k8; c += 256) {
-    const uint4 v = __ldg(src + c);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint2* dst = q + static_cast<int64_t>(row) * k8;
+  uint4 v[V];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float lo = __uint_as_float(w[i] << 16), hi = __uint_as_float(w[i] & 0xFFFF0000u);
-      bad |= !(fabsf(lo) <= 3.4e38f) || !(fabsf(hi) <= 3.4e38f);
-      a = fmaxf(a, fmaxf(fabsf(lo), fabsf(hi)));
-    }
-  }
-  if (bad) a = INFINITY;
+  for (int i = 0; i < V; ++i)
+    v[i] = t + i * TPR < k8 ? __ldg(src + t + i * TPR) : make_uint4(0, 0, 0, 0);
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) a = abs_max8(v[i], a);
+  for (int c = t + V * TPR; c < k8; c += TPR) a = abs_max8(__ldg(src + c), a);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+  if (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = fmaxf(a, red[i]);
+  }
+  if (t == 0) scale[row] = a <= 3.4e38f ? a / 127.f : __uint_as_float(0x7FC00000u);
+  const RowScale s = row_scale(a);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (t + i * TPR < k8) dst[t + i * TPR] = quant8(v[i], s);
+  for (int c = t + V * TPR; c < k8; c += TPR) dst[c] = quant8(__ldg(src + c), s);
+}
+
+// ---- the product ----------------------------------------------------------------------------
+// tcgen05.mma kind::i8 (K = 32 an instruction, 32-bit integer accumulators in TMEM), operands
+// by TMA in k-blocks of 128 bytes, 128-byte swizzle.  Every wait is bounded.
+constexpr int kBK = 128;
+constexpr uint32_t kTileBytes = 128 * kBK;  // 128 rows of a k-block
+constexpr long long kTimeoutCycles = 4000000000LL;
+
+// Instruction descriptor, kind::i8: signed 8-bit A and B (K-major), 32-bit integer D.
+__host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Few rows: the weights are the M operand, so a tile is 128 output channels x NT rows of x and
+// the kernel streams the weights once, whatever the rows (bound: the weights' bytes).  To have
+// enough CTAs streaming, a cluster of `splits` CTAs shares a tile, each with a part of K; the
+// partial sums are integers and meet through distributed shared memory, exactly.  The weight
+// loads of the first stages go out before the kernel waits for the quantised rows (programmatic
+// dependent launch behind quantize_kernel).
+constexpr int kFewStages = 4;
+constexpr int kFewThreads = 128;
+template <int NT>
+struct FewTile {
+  static constexpr uint32_t stage = kTileBytes + NT * kBK;
+  static constexpr uint32_t tmem_cols = NT < 32 ? 32 : NT;
+  static constexpr size_t smem = 1024 + kFewStages * stage + 256;
+  static_assert(NT * 128 * 4 <= kFewStages * stage, "the partial sums reuse the ring");
+};
+struct FewParams {
+  const float* sa;
+  const float* sw;
+  __nv_bfloat16* out;
+  int M, N, k_blocks, splits, kb_per_split;
+  int* status;
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kFewThreads)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                    const FewParams p) {
+  using T = FewTile<NT>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const uint32_t s0 = ptx::smem_u32(smem);
+  uint8_t* tail = smem + kFewStages * T::stage;
+  const uint32_t full0 = ptx::smem_u32(tail), empty0 = full0 + 8 * kFewStages;
+  const uint32_t done = empty0 + 8 * kFewStages;
+  uint32_t* holder = reinterpret_cast<uint32_t*>(tail + 8 * (2 * kFewStages + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
+  volatile int* never_flag = abort_flag + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % p.splits;
+  const int n0 = static_cast<int>(blockIdx.x) / p.splits * 128;
+  const int m0 = static_cast<int>(blockIdx.y) * NT;
+  const int kb0 = rank * p.kb_per_split;
+  const int nkb = min(p.k_blocks, kb0 + p.kb_per_split) - kb0;  // >= 1: no split is empty
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kFewStages; ++i) {
+      ptx::mbar_init(full0 + 8 * i, 1);
+      ptx::mbar_init(empty0 + 8 * i, 1);
+    }
+    ptx::mbar_init(done, 1);
+    *abort_flag = 0;
+    *never_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(holder), T::tmem_cols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
   __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *holder;
+  if (warp == 0) {
+    if (lane == 0) {
+      ptx::prefetch_tmap(&tmX);
+      const int pre = min(nkb, kFewStages);
+      for (int i = 0; i < pre; ++i) {
+        ptx::mbar_arrive_expect_tx(full0 + 8 * i, T::stage);
+        ptx::tma_load_2d(s0 + i * T::stage, &tmW, full0 + 8 * i, (kb0 + i) * kBK, n0);
+      }
+      ptx::pdl_wait();
+      for (int i = 0; i < pre; ++i)
+        ptx::tma_load_2d(s0 + i * T::stage + kTileBytes, &tmX, full0 + 8 * i, (kb0 + i) * kBK, m0);
+      bool ok = true;
+      int issued = pre;
+      for (int i = pre; ok && i < nkb; ++i) {
+        const int st = i % kFewStages;
+        ok = ptx::mbar_wait(empty0 + 8 * st, (i / kFewStages - 1) & 1, abort_flag, p.status,
+                            kTimeoutCycles, DS_ERR_TIMEOUT);
+        if (!ok) break;
+        ptx::mbar_arrive_expect_tx(full0 + 8 * st, T::stage);
+        ptx::tma_load_2d(s0 + st * T::stage, &tmW, full0 + 8 * st, (kb0 + i) * kBK, n0);
+        ptx::tma_load_2d(s0 + st * T::stage + kTileBytes, &tmX, full0 + 8 * st, (kb0 + i) * kBK, m0);
+        issued = i + 1;
+      }
+      // every load has landed before this CTA goes on: the last fill of each stage
+      for (int i = max(0, issued - kFewStages); i < issued; ++i)
+        ptx::mbar_wait(full0 + 8 * (i % kFewStages), (i / kFewStages) & 1, never_flag, p.status,
+                       kTimeoutCycles, DS_ERR_TIMEOUT);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8(128, NT);
+      for (int i = 0; i < nkb; ++i) {
+        const int st = i % kFewStages;
+        if (!ptx::mbar_wait(full0 + 8 * st, (i / kFewStages) & 1, abort_flag, p.status,
+                            kTimeoutCycles, DS_ERR_TIMEOUT))
+          break;
+        ptx::tc_fence_after();
+        const uint32_t a = s0 + st * T::stage, b = a + kTileBytes;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = fmaxf(a, red[i]);
-  const bool finite = a <= 3.4e38f;
-  if (threadIdx.x == 0) scale[row] = finite ? a / 127.f : __uint_as_float(0x7FC00000u);
-  // subnormal and tiny rows are scaled up by a power of two, so that 127 / a stays finite,
-  // huge ones down, so that 127 x does
-  const float up = a < 1e-30f ? 1.2676506e30f : a > 1e30f ? 7.8886091e-31f : 1.f;  // 2^100, 2^-100
-  const float au = a * up;
-  const float r = finite && au > 0.f ? 127.f / au : 0.f;
-  uint2* dst = q + static_cast<int64_t>(row) * k8;
-  for (int c = threadIdx.x; c < k8; c += 256) {
-    uint32_t o[2] = {0u, 0u};
-    if (r != 0.f) {
-      const uint4 v = __ldg(src + c);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        for (int k = 0; k < 4; ++k)
+          umma_i8(tmem, ptx::sw128_kmajor_desc(a + 32u * k), ptx::sw128_kmajor_desc(b + 32u * k),
+                  idesc, i != 0 || k != 0);
+        ptx::umma_commit(empty0 + 8 * st);
+      }
+      ptx::umma_commit(done);
+    }
+  }
+  __syncwarp();
+  int ok = 1;
+  if (lane == 0)
+    ok = ptx::mbar_wait(done, 0, never_flag, p.status, kTimeoutCycles, DS_ERR_TIMEOUT) &&
+         !*abort_flag;
+  ok = __syncthreads_and(__shfl_sync(0xffffffffu, ok, 0));
+  ptx::tc_fence_after();
+  // D (lane = channel, column = row of x) -> shared memory [row][128 channels]
+  int32_t* part = reinterpret_cast<int32_t*>(smem);
+  const uint32_t tb = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+  const int mrows = min(NT, p.M - m0);
+#pragma unroll 1
+  for (int c = 0; c < NT; c += 32) {
+    if (c >= mrows) break;
+    uint32_t v[32];
+    ptx::tmem_ld32(tb + c, v);
+    ptx::tmem_wait_ld(v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int lo = quant1(__uint_as_float(w[i] << 16) * up, au, r);
-        const int hi = quant1(__uint_as_float(w[i] & 0xFFFF0000u) * up, au, r);
-        o[i >> 1] |= ((lo & 0xFF) | ((hi & 0xFF) << 8)) << (16 * (i & 1));
+    for (int i = 0; i < 32; ++i)
+      if (i < NT) part[(c + i) * 128 + threadIdx.x] = static_cast<int32_t>(v[i]);
+  }
+  ptx::tc_fence_before();
+  __syncwarp();
+  if (p.splits > 1) ptx::cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, T::tmem_cols);
+  }
+  ptx::pdl_wait();  // the rows' scales
+  if (ok) {
+    // CTA `rank` finishes its share of the rows: 16 threads a row, 8 channels each
+    const int per = (mrows + p.splits - 1) / p.splits;
+    const int r1 = min(mrows, (rank + 1) * per);
+    const int n = n0 + (threadIdx.x & 15) * 8;
+    float sw[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sw[j] = n < p.N ? __ldg(p.sw + n + j) : 0.f;
+    for (int r = rank * per + (threadIdx.x >> 4); r < r1; r += kFewThreads / 16) {
+      const uint32_t at = s0 + (r * 128 + (threadIdx.x & 15) * 8) * 4;
+      int4 x = make_int4(0, 0, 0, 0), y = x;
+      for (int k = 0; k < p.splits; ++k) {
+        const uint32_t src = p.splits > 1 ? ptx::mapa_shared(at, k) : at;
+        int4 u, v;
+        asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(src));
+        asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src + 16));
+        x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+        y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
+      }
+      if (n < p.N) {  // (N is a multiple of 8)
+        const float sa = __ldg(p.sa + m0 + r);
+        const uint4 o = make_uint4(
+            pack2(static_cast<float>(x.x) * (sa * sw[0]), static_cast<float>(x.y) * (sa * sw[1])),
+            pack2(static_cast<float>(x.z) * (sa * sw[2]), static_cast<float>(x.w) * (sa * sw[3])),
+            pack2(static_cast<float>(y.x) * (sa * sw[4]), static_cast<float>(y.y) * (sa * sw[5])),
+            pack2(static_cast<float>(y.z) * (sa * sw[6]), static_cast<float>(y.w) * (sa * sw[7])));
+        *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(m0 + r) * p.N + n) = o;
       }
     }
-    dst[c] = make_uint2(o[0], o[1]);
+  }
+  __syncwarp();
+  if (p.splits > 1) ptx::cluster_sync();  // no CTA leaves while another reads its sums
+}
+
+// Many rows: tiles of 256 rows x 256 channels by pairs of CTAs (cta_group::2), persistent over
+// the tiles, as grouped_gemm_kernel's pair mode: each CTA loads its own 128 rows and its half of
+// the channels (32 KB a k-block, 6 stages), two accumulators of 256 columns let the epilogue of
+// a tile run under the products of the next.  A last tile of fewer channels runs narrower MMAs.
+constexpr int kManyStages = 6;
+constexpr int kManyThreads = 192;
+constexpr uint32_t kSlabBytes = 32 * 128;
+constexpr size_t kManySmem = 1024 + kManyStages * 2 * kTileBytes + 4 * kSlabBytes + 256 + 2 * 256 * 4;
+struct ManyParams {
+  const float* sa;
+  const float* sw;
+  int M, N, k_blocks, n_tiles, tiles;
+  int* status;
+};
+
+__global__ void __launch_bounds__(kManyThreads, 1)
+    many_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                     const __grid_constant__ CUtensorMap tmO, const ManyParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const uint32_t sX = ptx::smem_u32(smem), sW = sX + kManyStages * kTileBytes;
+  const uint32_t sOut = sW + kManyStages * kTileBytes;
+  uint8_t* tail = smem + kManyStages * 2 * kTileBytes + 4 * kSlabBytes;
+  float* sw = reinterpret_cast<float*>(tail + 256);  // [2][256] channel scales of a tile
+  const uint32_t full0 = ptx::smem_u32(tail), empty0 = full0 + 8 * kManyStages;
+  const uint32_t tfull0 = empty0 + 8 * kManyStages, tempty0 = tfull0 + 16, drain = tempty0 + 16;
+  uint32_t* holder = reinterpret_cast<uint32_t*>(tail + 8 * (2 * kManyStages + 5));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
+  volatile int* never_flag = abort_flag + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kManyStages; ++i) {
+      ptx::mbar_init(full0 + 8 * i, 1);
+      ptx::mbar_init(empty0 + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(tfull0 + 8 * i, 1);
+      ptx::mbar_init(tempty0 + 8 * i, 8);
+    }
+    ptx::mbar_init(drain, 1);
+    *abort_flag = 0;
+    *never_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_u32(holder), 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::pdl_wait();
+  ptx::tc_fence_before();
+  __syncwarp();
+  ptx::cluster_sync();  // both CTAs' barriers are set up before either signals the other's
+  ptx::tc_fence_after();
+  const uint32_t tmem = *holder;
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0;
+      uint32_t phase = 0, used = 0, phases = 0;
+      bool ok = true;
+      for (int t = unit; ok && t < p.tiles; t += units) {
+        const int m0 = t / p.n_tiles * 256 + rank * 128, n0 = t % p.n_tiles * 256;
+        const int half = (min(256, p.N - n0) + 31) / 32 * 16;  // channels of this CTA's half
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!ptx::mbar_wait(empty0 + 8 * st, phase ^ 1u, abort_flag, p.status, kTimeoutCycles,
+                              DS_ERR_TIMEOUT)) {
+            ok = false;
+            break;
+          }
+          // the leader's barrier counts both CTAs' bytes
+          const uint32_t lead = ptx::mapa_shared(full0 + 8 * st, 0);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(full0 + 8 * st, 4 * kTileBytes);
+          ptx::tma_load_2d_pair(sX + st * kTileBytes, &tmX, lead, kb * kBK, m0);
+          ptx::tma_load_2d_pair(sW + st * kTileBytes, &tmW, lead, kb * kBK, n0 + rank * half);
+          used |= 1u << st;
+          phases = (phases & ~(1u << st)) | (phase << st);
+          if (++st == kManyStages) {
+            st = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // every load has landed before the CTA may exit (the peer sees the leader's stages as
+      // consumed by the MMAs)
+      for (int i = 0; i < kManyStages; ++i)
+        if (used & (1u << i))
+          ptx::mbar_wait((rank != 0 ? empty0 : full0) + 8 * i, (phases >> i) & 1u, never_flag,
+                         p.status, kTimeoutCycles, DS_ERR_TIMEOUT);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int st = 0, acc = 0;
+      uint32_t phase = 0, aphase = 0;
+      bool ok = true;
+      for (int t = unit; ok && t < p.tiles; t += units) {
+        if (!ptx::mbar_wait(tempty0 + 8 * acc, aphase ^ 1u, abort_flag, p.status, kTimeoutCycles,
+                            DS_ERR_TIMEOUT))
+          break;
+        ptx::tc_fence_after();
+        const int n0 = t % p.n_tiles * 256;
+        const uint32_t idesc = idesc_i8(256, (min(256, p.N - n0) + 31) / 32 * 32);
+        const uint32_t d = tmem + acc * 256;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!ptx::mbar_wait(full0 + 8 * st, phase, abort_flag, p.status, kTimeoutCycles,
+                              DS_ERR_TIMEOUT)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t a = sX + st * kTileBytes, b = sW + st * kTileBytes;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_i8_pair(d, ptx::sw128_kmajor_desc(a + 32u * k),
+                         ptx::sw128_kmajor_desc(b + 32u * k), idesc, kb != 0 || k != 0);
+          ptx::umma_commit_pair(empty0 + 8 * st);  // the stage is free in both CTAs
+          ptx::umma_commit_pair(ptx::mapa_shared(empty0 + 8 * st, 1));
+          if (++st == kManyStages) {
+            st = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        ptx::umma_commit_pair(tfull0 + 8 * acc);
+        ptx::umma_commit_pair(ptx::mapa_shared(tfull0 + 8 * acc, 1));
+        if (++acc == 2) {
+          acc = 0;
+          aphase ^= 1u;
+        }
+      }
+      ptx::umma_commit_pair(drain);  // no MMA may still write when TMEM is released
+      ptx::mbar_wait(drain, 0, never_flag, p.status, kTimeoutCycles, DS_ERR_TIMEOUT);
+    }
+  } else {
+    const int q = warp & 3, r = q * 32 + lane;  // TMEM lane quarter of this warp
+    const int et = threadIdx.x - 64;
+    const uint32_t slab = sOut + (warp - 2) * kSlabBytes;
+    int acc = 0;
+    uint32_t aphase = 0;
+    for (int t = unit; t < p.tiles; t += units) {
+      const int m0 = t / p.n_tiles * 256 + rank * 128, n0 = t % p.n_tiles * 256;
+      const int cols = min(256, p.N - n0);
+      float* swt = sw + acc * 256;
+      swt[et] = n0 + et < p.N ? __ldg(p.sw + n0 + et) : 0.f;
+      swt[et + 128] = n0 + et + 128 < p.N ? __ldg(p.sw + n0 + et + 128) : 0.f;
+      const float sa = m0 + r < p.M ? __ldg(p.sa + m0 + r) : 0.f;
+      ptx::named_bar_sync(1, 128);
+      int ok = 1;
+      if (lane == 0)
+        ok = ptx::mbar_wait(tfull0 + 8 * acc, aphase, abort_flag, p.status, kTimeoutCycles,
+                            DS_ERR_TIMEOUT);
+      // (all four epilogue warps leave together: the named barrier above counts them)
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (ok) {
+        ptx::tc_fence_after();
+        const uint32_t tb = tmem + acc * 256 + (static_cast<uint32_t>(q * 32) << 16);
+#pragma unroll 1
+        for (int c = 0; c < 256; c += 64) {
+          if (c >= cols || m0 + q * 32 >= p.M) break;
+          uint32_t a[32], b[32];
+          ptx::tmem_ld32(tb + c, a);
+          ptx::tmem_ld32(tb + c + 32, b);
+          ptx::tmem_wait_ld2(a, b);
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = *reinterpret_cast<const float2*>(swt + c + 2 * i);
+            const float2 g = *reinterpret_cast<const float2*>(swt + c + 32 + 2 * i);
+            w[i] = pack2(static_cast<float>(static_cast<int>(a[2 * i])) * (sa * f.x),
+                         static_cast<float>(static_cast<int>(a[2 * i + 1])) * (sa * f.y));
+            w[16 + i] = pack2(static_cast<float>(static_cast<int>(b[2 * i])) * (sa * g.x),
+                              static_cast<float>(static_cast<int>(b[2 * i + 1])) * (sa * g.y));
+          }
+          if (lane == 0) ptx::bulk_wait_read0();  // the slab's last store has read it
+          __syncwarp();
+          // 128-byte rows, 16-byte chunks swizzled as the output's tensor map expects
+          const uint32_t row = slab + lane * 128u;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             row + ((static_cast<uint32_t>(j) ^ (lane & 7u)) << 4)),
+                         "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                         : "memory");
+          ptx::fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {  // rows and channels outside the output are not stored
+            ptx::tma_store_2d(&tmO, slab, n0 + c, m0 + q * 32);
+            ptx::bulk_commit();
+          }
+        }
+        ptx::tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0 && ok) {
+        if (rank != 0) ptx::mbar_arrive_remote(ptx::mapa_shared(tempty0 + 8 * acc, 0));
+        else ptx::mbar_arrive(tempty0 + 8 * acc);
+      }
+      if (++acc == 2) {
+        acc = 0;
+        aphase ^= 1u;
+      }
+    }
+    if (lane == 0) ptx::bulk_wait0();
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem, 512);
   }
 }
 
-// out[m, n] = bf16(acc * (sa[m] * sw[n])).  64 x 64 outputs a block, 4 x 4 a thread, 64
-// bytes of K at a time through shared memory, __dp4a.
-__global__ void __launch_bounds__(256)
-    gemm_dp4a_kernel(const int8_t* __restrict__ a, const float* __restrict__ sa,
-                     const int8_t* __restrict__ w, const float* __restrict__ sw,
-                     __nv_bfloat16* __restrict__ out, int M, int N, int K) {
-  __shared__ int ta[64][17], tw[64][17];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += 64) {
-    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
-    int4 va = make_int4(0, 0, 0, 0), vw = va;
-    if (k0 + c < K) {
-      if (m0 + r < M)
-        va = *reinterpret_cast<const int4*>(a + static_cast<int64_t>(m0 + r) * K + k0 + c);
-      if (n0 + r < N)
-        vw = *reinterpret_cast<const int4*>(w + static_cast<int64_t>(n0 + r) * K + k0 + c);
-    }
-    __syncthreads();
-    ta[r][c / 4] = va.x; ta[r][c / 4 + 1] = va.y; ta[r][c / 4 + 2] = va.z; ta[r][c / 4 + 3] = va.w;
-    tw[r][c / 4] = vw.x; tw[r][c / 4 + 1] = vw.y; tw[r][c / 4 + 2] = vw.z; tw[r][c / 4 + 3] = vw.w;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      int x[4], y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = ta[ty + 16 * i][k];
-        y[i] = tw[tx + 16 * i][k];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(x[i], y[j], acc[i][j]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty + 16 * i;
-    if (m >= M) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx + 16 * j;
-      if (n < N)
-        out[static_cast<int64_t>(m) * N + n] =
-            __float2bfloat16_rn(static_cast<float>(acc[i][j]) * (__ldg(sa + m) * __ldg(sw + n)));
-    }
-  }
+// ---- host side ------------------------------------------------------------------------------
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::once_flag g_encode_once;
+
+int tmap(CUtensorMap* m, const void* ptr, CUtensorMapDataType type, int bytes, int64_t rows,
+         int64_t cols, uint32_t box_cols, uint32_t box_rows) {
+  std::call_once(g_encode_once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  if (g_encode == nullptr) return fail(DS_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * bytes};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1u, 1u};
+  const CUresult r = g_encode(m, type, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return DS_OK;
+}
+
+bool g_attr_set[64] = {};
+std::mutex g_attr_mutex;
+int g_pairs[64] = {};  // co-resident CTA pairs of the many-rows kernel
+
+template <int NT>
+int few_attr() {
+  DS_CUDA(cudaFuncSetAttribute(few_rows_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(FewTile<NT>::smem)));
+  return DS_OK;
+}
+
+int set_attrs(const DeviceInfo& di) {
+  std::lock_guard<std::mutex> lock(g_attr_mutex);
+  if (g_attr_set[di.device]) return DS_OK;
+  DS_TRY(few_attr<16>());
+  DS_TRY(few_attr<32>());
+  DS_TRY(few_attr<64>());
+  DS_TRY(few_attr<128>());
+  DS_CUDA(cudaFuncSetAttribute(many_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(kManySmem)));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(2 * (di.num_sms / 2));
+  cfg.blockDim = dim3(kManyThreads);
+  cfg.dynamicSmemBytes = kManySmem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  DS_CUDA(cudaOccupancyMaxActiveClusters(&n, many_rows_kernel, &cfg));
+  g_pairs[di.device] = n;
+  g_attr_set[di.device] = true;
+  return DS_OK;
+}
+
+template <int NT>
+int launch_few(const void* a, const float* sa, const void* w, const float* sw, void* out, int M,
+               int N, int K, const DeviceInfo& di, cudaStream_t s) {
+  CUtensorMap tmW, tmX;
+  DS_TRY(tmap(&tmW, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, N, K, kBK, 128));
+  DS_TRY(tmap(&tmX, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M, K, kBK, NT));
+  FewParams p{};
+  p.sa = sa;
+  p.sw = sw;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.M = M;
+  p.N = N;
+  p.k_blocks = (K + kBK - 1) / kBK;
+  const int tiles = (N + 127) / 128, mt = (M + NT - 1) / NT;
+  // enough CTAs for the SMs to stream, at least two k-blocks each; clusters of at most 8
+  int splits = 1;
+  while (splits < 8 && tiles * mt * splits < di.num_sms && p.k_blocks >= 4 * splits) splits *= 2;
+  p.kb_per_split = (p.k_blocks + splits - 1) / splits;
+  p.splits = (p.k_blocks + p.kb_per_split - 1) / p.kb_per_split;  // none is empty
+  p.status = device_status_ptr();
+  if (p.status == nullptr) return fail(DS_ERR_CUDA, "device status word unavailable");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(tiles * p.splits, mt);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = FewTile<NT>::smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  DS_CUDA(cudaLaunchKernelEx(&cfg, few_rows_kernel<NT>, tmW, tmX, p));
+  return DS_OK;
+}
+
+int launch_many(const void* a, const float* sa, const void* w, const float* sw, void* out, int M,
+                int N, int K, const DeviceInfo& di, cudaStream_t s) {
+  CUtensorMap tmX, tmW, tmO;
+  DS_TRY(tmap(&tmX, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M, K, kBK, 128));
+  DS_TRY(tmap(&tmW, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, N, K, kBK, 128));
+  DS_TRY(tmap(&tmO, out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, M, N, 64, 32));
+  ManyParams p{};
+  p.sa = sa;
+  p.sw = sw;
+  p.M = M;
+  p.N = N;
+  p.k_blocks = (K + kBK - 1) / kBK;
+  p.n_tiles = (N + 255) / 256;
+  const int64_t tiles = static_cast<int64_t>(p.n_tiles) * ((M + 255) / 256);
+  DS_REQUIRE(tiles < (1LL << 31), "int8_linear: too many tiles");
+  p.tiles = static_cast<int>(tiles);
+  p.status = device_status_ptr();
+  if (p.status == nullptr) return fail(DS_ERR_CUDA, "device status word unavailable");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(2 * std::min(p.tiles, g_pairs[di.device]));
+  cfg.blockDim = dim3(kManyThreads);
+  cfg.dynamicSmemBytes = kManySmem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  DS_CUDA(cudaLaunchKernelEx(&cfg, many_rows_kernel, tmX, tmW, tmO, p));
+  return DS_OK;
 }
 
 int check_shape(int64_t M, int N, int K) {
@@ -146,22 +687,38 @@ int check_shape(int64_t M, int N, int K) {
 int launch_quantize(const void* x, int64_t ld, int64_t rows, int K, void* q, float* scale,
                     cudaStream_t s) {
   if (rows == 0) return DS_OK;
-  quantize_kernel<<<static_cast<unsigned>(rows), 256, 0, s>>>(
-      static_cast<const uint4*>(x), ld / 8, static_cast<int>(rows), K / 8, static_cast<uint2*>(q),
-      scale);
+  const uint4* src = static_cast<const uint4*>(x);
+  uint2* dst = static_cast<uint2*>(q);
+  const int k8 = K / 8, n = static_cast<int>(rows);
+  const unsigned r = static_cast<unsigned>(rows), r8 = static_cast<unsigned>((rows + 7) / 8);
+  if (rows >= 1024 && k8 <= 256) {  // a warp a row once there are rows enough to fill the SMs
+    if (k8 <= 128) quantize_kernel<32, 4><<<r8, 256, 0, s>>>(src, ld / 8, n, k8, dst, scale);
+    else quantize_kernel<32, 8><<<r8, 256, 0, s>>>(src, ld / 8, n, k8, dst, scale);
+  } else if (k8 <= 256) {
+    quantize_kernel<256, 1><<<r, 256, 0, s>>>(src, ld / 8, n, k8, dst, scale);
+  } else {
+    quantize_kernel<256, 4><<<r, 256, 0, s>>>(src, ld / 8, n, k8, dst, scale);
+  }
   DS_LAUNCH_CHECK("quantize_kernel");
   return DS_OK;
 }
 
 int launch_gemm(const void* a, const float* sa, const void* w, const float* sw, void* out,
-                int64_t M, int N, int K, cudaStream_t s) {
-  if (M == 0 || N == 0) return DS_OK;
-  const int64_t my = (M + 63) / 64;
-  DS_REQUIRE(my <= 65535, "int8_linear: too many rows");
-  gemm_dp4a_kernel<<<dim3((N + 63) / 64, static_cast<unsigned>(my)), 256, 0, s>>>(
-      static_cast<const int8_t*>(a), sa, static_cast<const int8_t*>(w), sw,
-      static_cast<__nv_bfloat16*>(out), static_cast<int>(M), N, K);
-  DS_LAUNCH_CHECK("gemm_dp4a_kernel");
+                int64_t M64, int N, int K, cudaStream_t s) {
+  if (M64 == 0 || N == 0) return DS_OK;
+  const int M = static_cast<int>(M64);
+  DeviceInfo di;
+  DS_TRY(device_info(&di));
+  DS_TRY(set_attrs(di));
+  int st;
+  if (M <= 16) st = launch_few<16>(a, sa, w, sw, out, M, N, K, di, s);
+  else if (M <= 32) st = launch_few<32>(a, sa, w, sw, out, M, N, K, di, s);
+  else if (M <= 64) st = launch_few<64>(a, sa, w, sw, out, M, N, K, di, s);
+  else if (M <= 512 || g_pairs[di.device] < 1)
+    st = launch_few<128>(a, sa, w, sw, out, M, N, K, di, s);
+  else st = launch_many(a, sa, w, sw, out, M, N, K, di, s);
+  DS_TRY(st);
+  DS_LAUNCH_CHECK("int8 product");
   return DS_OK;
 }
 
