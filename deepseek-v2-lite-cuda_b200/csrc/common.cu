@@ -1,5 +1,6 @@
 // Library-wide host state: error messages, per-device facts and side streams, the device
 // status word, the hello stub and the bounded-wait probe.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -99,8 +100,15 @@ void add_pdl_attr(cudaLaunchAttribute* attrs, unsigned int& n) {
 }
 
 int* device_status_ptr() {
+  // looked up once per device: the address does not change while the library is loaded
+  static std::atomic<int*> known[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
+  int* at = known[dev].load(std::memory_order_acquire);
+  if (at != nullptr) return at;
   void* p = nullptr;
   if (cudaGetSymbolAddress(&p, g_ds_device_status) != cudaSuccess) return nullptr;
+  known[dev].store(static_cast<int*>(p), std::memory_order_release);
   return static_cast<int*>(p);
 }
 }  // namespace ds

@@ -4,9 +4,10 @@
 // Quantisation of a row x (bf16, K values), a = max |x|:
 //   q_k = rint(127 x_k / a), ties to even;  s = a / 127  (x_k stands as q_k s)
 // a = 0 gives q = 0, s = 0; a row holding an infinity or a NaN gives q = 0, s = NaN, so its
-// whole output row is NaN and no other row is touched.  The quotient is exact to its side of
-// every border: 127 x has 15 significant bits, so fmaf(-n, a, 127 x) is the exact remainder
-// of a candidate n, which decides the neighbour and the ties (x = a/2 is one: 63.5).
+// whole output row is NaN and no other row is touched.  Every quotient goes to its own side: with
+// 127 / a = rh + rl to twice f32's bits, fmaf(x, rh, x rl) is 127 x / a rounded once, so a tie (x
+// = a / 2 is one: 63.5) stays one, and no other quotient of two 8-bit significands is nearer to
+// a tie than 2^-15 of itself.
 // Product: out_mn = bf16((sum_k q_mk w_nk) * (s_m * ws_n)); the sum is exact in 32 bits
 // (K <= 131072), so no split or order of it changes the result.
 #include <cuda.h>
@@ -25,52 +26,46 @@ namespace {
 
 constexpr int kMaxK = 131072;
 
-// rint(127 x / a) for finite |x| <= a, a > 0; r ~ 127 / a, both scaled alike.
-__device__ __forceinline__ int quant1(float x, float a, float r) {
-  const float x127 = x * 127.f;  // exact: 8 + 7 significant bits
-  float n = rintf(x * r);
-  const float e = fmaf(-n, a, x127);  // exact: |n| <= 128 has 8 bits, a has 8
-  const float e2 = 2.f * fabsf(e);
-  const float step = copysignf(1.f, e);
-  const bool odd = (static_cast<int>(n) & 1) != 0;
-  if (e2 > a || (e2 == a && odd)) n += step;
-  return static_cast<int>(n);
-}
-
-__device__ __forceinline__ float abs_max8(const uint4& v, float a) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float lo = fabsf(__uint_as_float(w[i] << 16)), hi = fabsf(__uint_as_float(w[i] & 0xFFFF0000u));
-    // a NaN counts as infinity: fmaxf would pass it over
-    a = fmaxf(a, fmaxf(lo <= 3.4e38f ? lo : INFINITY, hi <= 3.4e38f ? hi : INFINITY));
-  }
-  return a;
+// The larger magnitudes of eight bf16 values, two to a word, as bit patterns: those of finite
+// values order as the values do, infinities and NaN lie above them.
+__device__ __forceinline__ uint32_t abs_max8(const uint4& v, uint32_t a) {
+  a = __vmaxu2(a, __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu));
+  return __vmaxu2(a, __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
 }
 
 struct RowScale {
-  float up, au, r;  // x up / au * 127; r ~ 127 / au, 0 for an empty or non-finite row
+  float up, rh, rl;  // quotient = x up (rh + rl); all 0 for an empty or non-finite row
 };
-__device__ __forceinline__ RowScale row_scale(float a) {
+__device__ __forceinline__ RowScale row_scale(float a, bool finite) {
   RowScale s;
   // subnormal and tiny rows are scaled up by a power of two, so that 127 / a stays finite,
-  // huge ones down, so that 127 x does
+  // huge ones down, so that its lower part does not vanish
   s.up = a < 1e-30f ? 0x1p100f : a > 1e30f ? 0x1p-100f : 1.f;
-  s.au = a * s.up;
-  s.r = a <= 3.4e38f && s.au > 0.f ? 127.f / s.au : 0.f;
+  const float au = a * s.up;
+  const bool some = finite && au > 0.f;
+  s.rh = some ? 127.f / au : 0.f;
+  s.rl = some ? fmaf(-s.rh, au, 127.f) / au : 0.f;
   return s;
 }
+// rint into the low byte: adding 1.5 * 2^23 rounds to a whole number, ties to even.
+__device__ __forceinline__ uint32_t quant1(float x, const RowScale& s) {
+  return __float_as_uint(fmaf(x, s.rh, x * s.rl) + 12582912.f);
+}
 __device__ __forceinline__ uint2 quant8(const uint4& v, const RowScale& s) {
-  if (s.r == 0.f) return make_uint2(0u, 0u);
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  uint32_t o[2] = {0u, 0u};
+  uint32_t h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int lo = quant1(__uint_as_float(w[i] << 16) * s.up, s.au, s.r);
-    const int hi = quant1(__uint_as_float(w[i] & 0xFFFF0000u) * s.up, s.au, s.r);
-    o[i >> 1] |= ((lo & 0xFF) | ((hi & 0xFF) << 8)) << (16 * (i & 1));
+    float lo = __uint_as_float(w[i] << 16), hi = __uint_as_float(w[i] & 0xFFFF0000u);
+    if (s.up != 1.f) {
+      lo *= s.up;
+      hi *= s.up;
+    }
+    h[i] = __byte_perm(quant1(lo, s), quant1(hi, s), 0x0040);
   }
-  return make_uint2(o[0], o[1]);
+  const bool some = s.rh != 0.f;  // (a non-finite row's products are not numbers)
+  return make_uint2(some ? __byte_perm(h[0], h[1], 0x5410) : 0u,
+                    some ? __byte_perm(h[2], h[3], 0x5410) : 0u);
 }
 
 // TPR threads a row (a warp, or the block of 256); a row of at most TPR * V 16-byte vectors
@@ -79,7 +74,7 @@ template <int TPR, int V>
 __global__ void __launch_bounds__(256)
     quantize_kernel(const uint4* __restrict__ x, int64_t ld8, int rows, int k8,
                     uint2* __restrict__ q, float* __restrict__ scale) {
-  __shared__ float red[8];
+  __shared__ uint32_t red[8];
   ptx::pdl_launch_dependents();
   const int row = TPR == 32 ? static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5)
                             : static_cast<int>(blockIdx.x);
@@ -91,20 +86,22 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int i = 0; i < V; ++i)
     v[i] = t + i * TPR < k8 ? __ldg(src + t + i * TPR) : make_uint4(0, 0, 0, 0);
-  float a = 0.f;
+  uint32_t m2 = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) a = abs_max8(v[i], a);
-  for (int c = t + V * TPR; c < k8; c += TPR) a = abs_max8(__ldg(src + c), a);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+  for (int i = 0; i < V; ++i) m2 = abs_max8(v[i], m2);
+  for (int c = t + V * TPR; c < k8; c += TPR) m2 = abs_max8(__ldg(src + c), m2);
+  uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
+  m = __reduce_max_sync(0xffffffffu, m);
   if (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a = fmaxf(a, red[i]);
+    for (int i = 0; i < 8; ++i) m = max(m, red[i]);
   }
-  if (t == 0) scale[row] = a <= 3.4e38f ? a / 127.f : __uint_as_float(0x7FC00000u);
-  const RowScale s = row_scale(a);
+  const bool finite = m < 0x7F80u;
+  const float a = __uint_as_float(m << 16);
+  if (t == 0) scale[row] = finite ? a / 127.f : __uint_as_float(0x7FC00000u);
+  const RowScale s = row_scale(a, finite);
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (t + i * TPR < k8) dst[t + i * TPR] = quant8(v[i], s);
@@ -152,14 +149,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // partial sums are integers and meet through distributed shared memory, exactly.  The weight
 // loads of the first stages go out before the kernel waits for the quantised rows (programmatic
 // dependent launch behind quantize_kernel).
-constexpr int kFewStages = 4;
 constexpr int kFewThreads = 128;
 template <int NT>
 struct FewTile {
+  static constexpr int stages = NT <= 16 ? 6 : NT <= 32 ? 5 : NT <= 64 ? 4 : 3;  // two CTAs an SM
   static constexpr uint32_t stage = kTileBytes + NT * kBK;
   static constexpr uint32_t tmem_cols = NT < 32 ? 32 : NT;
-  static constexpr size_t smem = 1024 + kFewStages * stage + 256;
-  static_assert(NT * 128 * 4 <= kFewStages * stage, "the partial sums reuse the ring");
+  static constexpr size_t smem = 1024 + stages * stage + 256;
+  // [splits][ceil(NT / splits)][128] sums, splits <= 8
+  static_assert((NT + 7) * 128 * 4 <= stages * stage, "the sums reuse the ring");
 };
 struct FewParams {
   const float* sa;
@@ -174,6 +172,7 @@ __global__ void __launch_bounds__(kFewThreads)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                     const FewParams p) {
   using T = FewTile<NT>;
+  constexpr int kFewStages = T::stages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -262,10 +261,16 @@ __global__ void __launch_bounds__(kFewThreads)
          !*abort_flag;
   ok = __syncthreads_and(__shfl_sync(0xffffffffu, ok, 0));
   ptx::tc_fence_after();
-  // D (lane = channel, column = row of x) -> shared memory [row][128 channels]
-  int32_t* part = reinterpret_cast<int32_t*>(smem);
+  // D (lane = channel, column = row of x): each CTA finishes `per` of the rows and takes the
+  // others' sums for them into its ring, [CTA][row][128 channels].  Stores travel without a
+  // reply, so one barrier pays for all of them (remote loads in the sum cost 2-5 us).
+  __syncwarp();
+  if (p.splits > 1) ptx::cluster_sync();  // every CTA's ring is free
   const uint32_t tb = tmem + (static_cast<uint32_t>(warp * 32) << 16);
   const int mrows = min(NT, p.M - m0);
+  const int per = (mrows + p.splits - 1) / p.splits;
+  int owner = 0, in_owner = 0;
+  uint32_t to = (p.splits > 1 ? ptx::mapa_shared(s0, 0) : s0) + (rank * per * 128 + threadIdx.x) * 4;
 #pragma unroll 1
   for (int c = 0; c < NT; c += 32) {
     if (c >= mrows) break;
@@ -273,52 +278,49 @@ __global__ void __launch_bounds__(kFewThreads)
     ptx::tmem_ld32(tb + c, v);
     ptx::tmem_wait_ld(v);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < NT) part[(c + i) * 128 + threadIdx.x] = static_cast<int32_t>(v[i]);
+    for (int i = 0; i < 32; ++i) {
+      if (i >= NT || c + i >= mrows) break;
+      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(v[i]) : "memory");
+      to += 128 * 4;
+      if (++in_owner == per && p.splits > 1) {
+        in_owner = 0;
+        to = ptx::mapa_shared(s0, min(++owner, p.splits - 1)) + (rank * per * 128 + threadIdx.x) * 4;
+      }
+    }
   }
   ptx::tc_fence_before();
   __syncwarp();
-  if (p.splits > 1) ptx::cluster_sync();
+  if (p.splits > 1) ptx::cluster_sync();  // all sums have arrived; no remote access follows
   else __syncthreads();
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, T::tmem_cols);
   }
   ptx::pdl_wait();  // the rows' scales
-  if (ok) {
-    // CTA `rank` finishes its share of the rows: 16 threads a row, 8 channels each
-    const int per = (mrows + p.splits - 1) / p.splits;
-    const int r1 = min(mrows, (rank + 1) * per);
-    const int n = n0 + (threadIdx.x & 15) * 8;
-    float sw[8];
+  if (!ok) return;
+  // 16 threads a row, 8 channels each
+  const int r0 = rank * per, rn = min(mrows, r0 + per) - r0;
+  const int n = n0 + (threadIdx.x & 15) * 8;
+  if (n >= p.N) return;  // (N is a multiple of 8)
+  float sw[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sw[j] = n < p.N ? __ldg(p.sw + n + j) : 0.f;
-    for (int r = rank * per + (threadIdx.x >> 4); r < r1; r += kFewThreads / 16) {
-      const uint32_t at = s0 + (r * 128 + (threadIdx.x & 15) * 8) * 4;
-      int4 x = make_int4(0, 0, 0, 0), y = x;
-      for (int k = 0; k < p.splits; ++k) {
-        const uint32_t src = p.splits > 1 ? ptx::mapa_shared(at, k) : at;
-        int4 u, v;
-        asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(src));
-        asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src + 16));
-        x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
-        y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
-      }
-      if (n < p.N) {  // (N is a multiple of 8)
-        const float sa = __ldg(p.sa + m0 + r);
-        const uint4 o = make_uint4(
-            pack2(static_cast<float>(x.x) * (sa * sw[0]), static_cast<float>(x.y) * (sa * sw[1])),
-            pack2(static_cast<float>(x.z) * (sa * sw[2]), static_cast<float>(x.w) * (sa * sw[3])),
-            pack2(static_cast<float>(y.x) * (sa * sw[4]), static_cast<float>(y.y) * (sa * sw[5])),
-            pack2(static_cast<float>(y.z) * (sa * sw[6]), static_cast<float>(y.w) * (sa * sw[7])));
-        *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(m0 + r) * p.N + n) = o;
-      }
+  for (int j = 0; j < 8; ++j) sw[j] = __ldg(p.sw + n + j);
+  for (int r = threadIdx.x >> 4; r < rn; r += kFewThreads / 16) {
+    const float sa = __ldg(p.sa + m0 + r0 + r);
+    const int4* src = reinterpret_cast<const int4*>(smem) + r * 32 + (threadIdx.x & 15) * 2;
+    int4 x = src[0], y = src[1];
+    for (int k = 1; k < p.splits; ++k) {
+      const int4 u = src[k * per * 32], v = src[k * per * 32 + 1];
+      x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+      y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
     }
+    const uint4 o = make_uint4(
+        pack2(static_cast<float>(x.x) * (sa * sw[0]), static_cast<float>(x.y) * (sa * sw[1])),
+        pack2(static_cast<float>(x.z) * (sa * sw[2]), static_cast<float>(x.w) * (sa * sw[3])),
+        pack2(static_cast<float>(y.x) * (sa * sw[4]), static_cast<float>(y.y) * (sa * sw[5])),
+        pack2(static_cast<float>(y.z) * (sa * sw[6]), static_cast<float>(y.w) * (sa * sw[7])));
+    *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(m0 + r0 + r) * p.N + n) = o;
   }
-  __syncwarp();
-  if (p.splits > 1) ptx::cluster_sync();  // no CTA leaves while another reads its sums
 }
 
 // Many rows: tiles of 256 rows x 256 channels by pairs of CTAs (cta_group::2), persistent over
@@ -613,9 +615,9 @@ int launch_few(const void* a, const float* sa, const void* w, const float* sw, v
   p.N = N;
   p.k_blocks = (K + kBK - 1) / kBK;
   const int tiles = (N + 127) / 128, mt = (M + NT - 1) / NT;
-  // enough CTAs for the SMs to stream, at least two k-blocks each; clusters of at most 8
   int splits = 1;
-  while (splits < 8 && tiles * mt * splits < di.num_sms && p.k_blocks >= 4 * splits) splits *= 2;
+  while (splits < 8 && tiles * mt * splits * 10 <= di.num_sms * 8 && p.k_blocks >= 4 * splits)
+    splits *= 2;
   p.kb_per_split = (p.k_blocks + splits - 1) / splits;
   p.splits = (p.k_blocks + p.kb_per_split - 1) / p.kb_per_split;  // none is empty
   p.status = device_status_ptr();

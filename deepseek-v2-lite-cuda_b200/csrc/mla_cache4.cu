@@ -11,8 +11,9 @@
 //   scale_g = bf16(max_g |v| / 7);  code = 8 + clamp(rint(v / scale_g), -7, 7), ties to even
 // Symmetric 15-level codes: the tensor cores then take code - 8, an exact bf16, and a group's
 // scale multiplies one probability instead of 128 values.  A group holding an infinity or a
-// NaN gets scale NaN.  state[0..batch) holds the sequences' lengths in slots,
-// state[batch..2 batch) their next positions (tokens seen, evicted ones included).
+// NaN gets scale NaN.  state[0..batch) holds the sequences' lengths in slots, state[batch..2
+// batch) their next positions (tokens seen, evicted ones included), the third row counters that
+// are zero between calls.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -39,21 +40,46 @@ struct Cache {
   float* rstd;            // [batch, slots]
   int32_t* pos;           // [batch, slots]
   float* mass;            // [batch, slots]
-  int32_t* state;         // [2, batch]
+  int32_t* state;         // [3, batch]
   int batch, slots;
 };
 
-// 8 + clamp(rint(v / sigma), -7, 7) for bf16 v and sigma > 0; r ~ 1 / sigma.  v - n sigma is
-// exact in f32 (8 and 4 + 8 significant bits of nearby size), so it decides borders and ties.
-__device__ __forceinline__ uint32_t code1(float v, float sigma, float r) {
-  float n = rintf(v * r);
-  n = fminf(fmaxf(n, -8.f), 8.f);
-  const float e = fmaf(-n, sigma, v);
-  const float e2 = 2.f * fabsf(e);
-  const bool odd = (static_cast<int>(n) & 1) != 0;
-  if (e2 > sigma || (e2 == sigma && odd)) n += copysignf(1.f, e);
-  n = fminf(fmaxf(n, -7.f), 7.f);
-  return static_cast<uint32_t>(static_cast<int>(n) + 8);
+// Codes 8 + clamp(rint(v / sigma), -7, 7) of bf16 values.  With 1 / sigma = rh + rl to twice
+// f32's bits, fmaf(v, rh, v rl) is v / sigma rounded once: a tie stays a tie, and no other quotient
+// of two 8-bit significands comes near one.  Adding 1.5 * 2^23 + 8 rounds (ties to even) into
+// the low bits.  The clamp is for scales that lost bits to underflow: otherwise |v| / sigma is at
+// most 7 (1 + 2^-8).
+struct Quant {
+  float up, rh, rl;  // 0 where all codes are 8: an empty or non-finite group
+};
+__device__ __forceinline__ Quant quant_of(float sigma) {
+  Quant q;
+  q.up = sigma < 1e-30f ? 0x1p64f : 1.f;  // a subnormal scale's reciprocal would overflow
+  const float s = sigma * q.up;
+  q.rh = s > 0.f ? 1.f / s : 0.f;
+  q.rl = s > 0.f ? fmaf(-q.rh, s, 1.f) * q.rh : 0.f;
+  return q;
+}
+constexpr float kRound8 = 12582920.f;          // 1.5 * 2^23 + 8
+constexpr uint32_t kRoundBits = 0x4B400000u;   // its bits, less 8
+template <bool TINY>
+__device__ __forceinline__ uint32_t code_bits(float v, const Quant& q) {  // kRoundBits + code
+  if (TINY) v *= q.up;
+  float t = fmaf(v, q.rh, v * q.rl);
+  if (TINY) t = fminf(fmaxf(t, -7.f), 7.f);
+  return __float_as_uint(t + kRound8);
+}
+// Eight codes, the first in the low nibble: one shifted addition each; what kRoundBits adds is
+// known, and taken off at the end.
+template <bool TINY>
+__device__ __forceinline__ uint32_t codes8(const float* v, const Quant& q) {
+  uint32_t w = 0, off = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w += code_bits<TINY>(v[i], q) << (4 * i);
+    off += kRoundBits << (4 * i);
+  }
+  return q.rh == 0.f ? 0x88888888u : w - off;
 }
 
 // The bf16 scale of a group with largest magnitude a (a NaN or infinity inside: NaN).
@@ -72,40 +98,47 @@ __device__ __forceinline__ float usable(__nv_bfloat16 sc) {
 
 // One warp quantises one token into (b, slot): lane l holds latent dimensions 16 l .. 16 l +
 // 15 (a group of 128 = 8 lanes) and the rotation pair l of k_pe.
-__device__ __forceinline__ void put_token(const Cache& c, int b, int slot, int position,
-                                          const __nv_bfloat16* lat, const __nv_bfloat16* kpe,
-                                          const __nv_bfloat16* cos_t, const __nv_bfloat16* sin_t,
-                                          int table_rows, float eps) {
+struct Token {
+  uint4 a0, a1;
+  __nv_bfloat162 kp;
+};
+__device__ __forceinline__ Token load_token(const __nv_bfloat16* lat, const __nv_bfloat16* kpe) {
   const int lane = threadIdx.x & 31;
-  const uint4* l4 = reinterpret_cast<const uint4*>(lat) + 2 * lane;
-  const uint4 a0 = l4[0], a1 = l4[1];
-  const __nv_bfloat162 kp = reinterpret_cast<const __nv_bfloat162*>(kpe)[lane];
+  Token t;
+  t.a0 = __ldg(reinterpret_cast<const uint4*>(lat) + 2 * lane);
+  t.a1 = __ldg(reinterpret_cast<const uint4*>(lat) + 2 * lane + 1);
+  t.kp = __ldg(reinterpret_cast<const __nv_bfloat162*>(kpe) + lane);
+  return t;
+}
+__device__ __forceinline__ void put_token(const Cache& c, int b, int slot, int position,
+                                          const Token& tok, const __nv_bfloat16* cos_t,
+                                          const __nv_bfloat16* sin_t, int table_rows, float eps) {
+  const int lane = threadIdx.x & 31;
+  const uint4 a0 = tok.a0, a1 = tok.a1;
+  const __nv_bfloat162 kp = tok.kp;
   const uint32_t w[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
   float v[16];
-  float amax = 0.f, ss = 0.f;
+  float ss = 0.f;
+  uint32_t m2 = 0;  // the largest magnitudes as bit patterns, two to a word
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     v[2 * i] = __uint_as_float(w[i] << 16);
     v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    amax = fmaxf(amax, fmaxf(abs_or_inf(v[2 * i]), abs_or_inf(v[2 * i + 1])));
     ss = fmaf(v[2 * i], v[2 * i], fmaf(v[2 * i + 1], v[2 * i + 1], ss));
+    m2 = __vmaxu2(m2, w[i] & 0x7FFF7FFFu);
   }
 #pragma unroll
-  for (int d = 4; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+  for (int d = 4; d > 0; d >>= 1) m2 = __vmaxu2(m2, __shfl_xor_sync(0xffffffffu, m2, d));
+  const float amax = __uint_as_float(max(m2 & 0xFFFFu, m2 >> 16) << 16);  // (NaN, inf: not finite)
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
   const __nv_bfloat16 sc = group_scale(amax);
-  const float sg = usable(sc);
-  // a subnormal scale's reciprocal would overflow: scale both by 2^64
-  const float up = sg < 1e-30f ? 1.8446744e19f : 1.f;
-  const float r = sg > 0.f ? 1.f / (sg * up) : 0.f;
-  uint2 packed = make_uint2(0u, 0u);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t n = r > 0.f ? code1(v[i] * up, sg * up, r) : 8u;
-    if (i < 8) packed.x |= n << (4 * i);
-    else packed.y |= n << (4 * (i - 8));
-  }
+  const Quant qs = quant_of(usable(sc));
+  uint2 packed;
+  if (__any_sync(0xffffffffu, qs.up != 1.f))  // (rare)
+    packed = make_uint2(codes8<true>(v, qs), codes8<true>(v + 8, qs));
+  else
+    packed = make_uint2(codes8<false>(v, qs), codes8<false>(v + 8, qs));
   // k_pe at its position: the interleave -> half RoPE of src/reference/mla.py:176-206
   const int prow = min(position, table_rows - 1);
   const __nv_bfloat16* cr = cos_t + static_cast<int64_t>(prow) * kRope;
@@ -120,11 +153,9 @@ __device__ __forceinline__ void put_token(const Cache& c, int b, int slot, int p
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) ka = fmaxf(ka, __shfl_xor_sync(0xffffffffu, ka, d));
   const __nv_bfloat16 ksc = group_scale(ka);
-  const float kg = usable(ksc);
-  const float kup = kg < 1e-30f ? 1.8446744e19f : 1.f;
-  const float kr = kg > 0.f ? 1.f / (kg * kup) : 0.f;
-  const uint32_t c0 = kr > 0.f ? code1(r0 * kup, kg * kup, kr) : 8u;
-  const uint32_t c1 = kr > 0.f ? code1(r1 * kup, kg * kup, kr) : 8u;
+  const Quant kq = quant_of(usable(ksc));
+  const uint32_t c0 = kq.rh == 0.f ? 8u : code_bits<true>(r0, kq) - kRoundBits;
+  const uint32_t c1 = kq.rh == 0.f ? 8u : code_bits<true>(r1, kq) - kRoundBits;
   const uint32_t n0 = __shfl_down_sync(0xffffffffu, c0, 1);
   const uint32_t n1 = __shfl_down_sync(0xffffffffu, c1, 1);
   const int64_t row = static_cast<int64_t>(b) * c.slots + slot;
@@ -144,76 +175,88 @@ __device__ __forceinline__ void put_token(const Cache& c, int b, int slot, int p
   }
 }
 
-// n_new tokens of each sequence (new_lens[b] of them when given) behind its last slot; a warp
-// per token.  `advance`: one block holds all of a sequence's tokens and moves its length on.
-__global__ void __launch_bounds__(256)
+// n_new tokens of each sequence (new_lens[b] of them when given) behind its last slot; a warp a
+// token, whose loads are on their way while the lengths are read.  The block that finishes last
+// of a sequence moves its length on: by then every other one has read it (state's third row
+// counts them, and is zero between calls).  Prompts run in blocks of 1024 threads: the blocks
+// meet at that counter, one address a sequence, and with 256 threads a block their arrivals took
+// longer than the tokens (4 x 4096: 22 us).
+__global__ void __launch_bounds__(1024)
     append_kernel(Cache c, const __nv_bfloat16* __restrict__ lat, int64_t lat_ld,
                   const __nv_bfloat16* __restrict__ kpe, int64_t kpe_ld, int64_t src_bstride,
                   int n_new, const int32_t* __restrict__ new_lens,
                   const __nv_bfloat16* __restrict__ cos_t, const __nv_bfloat16* __restrict__ sin_t,
-                  int table_rows, float eps, int advance) {
+                  int table_rows, float eps) {
   const int b = blockIdx.y;
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  Token tok{};
+  if (i < n_new) {
+    const int64_t src = static_cast<int64_t>(b) * src_bstride + i;
+    tok = load_token(lat + src * lat_ld, kpe + src * kpe_ld);
+  }
   const int len = c.state[b], next = c.state[c.batch + b];
   const int n = new_lens != nullptr ? min(n_new, __ldg(new_lens + b)) : n_new;
-  if (i < n && len >= 0 && len + i < c.slots) {
-    const int64_t src = static_cast<int64_t>(b) * src_bstride + i;
-    put_token(c, b, len + i, next + i, lat + src * lat_ld, kpe + src * kpe_ld, cos_t, sin_t,
-              table_rows, eps);
-  }
-  if (advance) {
-    __syncthreads();  // every warp has read the length
-    if (threadIdx.x == 0) {
-      const int add = max(0, min(n, c.slots - len));
-      c.state[b] = len + add;
-      c.state[c.batch + b] = next + add;
-    }
+  if (i < n && len >= 0 && len + i < c.slots)
+    put_token(c, b, len + i, next + i, tok, cos_t, sin_t, table_rows, eps);
+  __syncthreads();  // every warp has read the length
+  if (threadIdx.x == 0 &&
+      (gridDim.x == 1 ||
+       atomicAdd(c.state + 2 * c.batch + b, 1) == static_cast<int>(gridDim.x) - 1)) {
+    const int add = max(0, min(n, c.slots - len));
+    c.state[b] = len + add;
+    c.state[c.batch + b] = next + add;
+    c.state[2 * c.batch + b] = 0;
   }
 }
 
-__global__ void advance_kernel(Cache c, int n_new, const int32_t* __restrict__ new_lens) {
-  const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  if (b >= c.batch) return;
-  const int n = new_lens != nullptr ? min(n_new, __ldg(new_lens + b)) : n_new;
-  const int add = max(0, min(n, c.slots - c.state[b]));
-  c.state[b] += add;
-  c.state[c.batch + b] += add;
-}
-
-// Eight codes of one word -> eight bf16 values code * scale (rounded once).
-__device__ __forceinline__ uint4 values8(uint32_t w, float s) {
-  uint4 o;
-  uint32_t* u = reinterpret_cast<uint32_t*>(&o);
+// Eight codes of one word -> eight bf16 values (code - 8) * scale, rounded once: 128 + code is a
+// bf16 pair under a mask, 136 off it is exact, and the product rounds.
+__device__ __forceinline__ uint4 values8(uint32_t w, uint32_t scale2) {
+  uint32_t p[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float lo = static_cast<float>(static_cast<int>((w >> (8 * i)) & 15u) - 8) * s;
-    const float hi = static_cast<float>(static_cast<int>((w >> (8 * i + 4)) & 15u) - 8) * s;
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    u[i] = *reinterpret_cast<const uint32_t*>(&h);
+  for (int j = 0; j < 4; ++j) {  // nibbles j and j + 4
+    const uint32_t x = ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p[j]) : "r"(x), "r"(0x43084308u));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(p[j]) : "r"(p[j]), "r"(scale2));
   }
-  return o;
+  return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
+                    __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
 }
 
-// Slots 0 .. n-1 of every sequence as bf16 values, zeros from its length on; a warp per slot.
+// Slots 0 .. n-1 of every sequence as bf16 values, zeros from its length on; four slots a warp,
+// so that their loads are in flight together.
+constexpr int kGetSlots = 4;
 __global__ void __launch_bounds__(256)
     get_kernel(Cache c, int n, uint4* __restrict__ lat, uint4* __restrict__ kpe) {
   const int lane = threadIdx.x & 31;
-  const int64_t i = blockIdx.x * static_cast<int64_t>(8) + (threadIdx.x >> 5);
-  if (i >= static_cast<int64_t>(c.batch) * n) return;
-  const int b = static_cast<int>(i / n), t = static_cast<int>(i - static_cast<int64_t>(b) * n);
-  uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0, v2 = v0;
-  if (t < c.state[b]) {
-    const int64_t row = static_cast<int64_t>(b) * c.slots + t;
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(c.codes + row * kRowBytes);
-    const __nv_bfloat16* s = c.scales + static_cast<int64_t>(b) * kGroups * c.slots + t;
-    v0 = values8(w[lane], __bfloat162float(s[static_cast<int64_t>(lane >> 4) * c.slots]));
-    v1 = values8(w[32 + lane], __bfloat162float(s[static_cast<int64_t>(2 + (lane >> 4)) * c.slots]));
-    if (lane < 8)
-      v2 = values8(w[64 + lane], __bfloat162float(s[static_cast<int64_t>(4) * c.slots]));
+  const int b = blockIdx.y;
+  const int t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kGetSlots;
+  if (t0 >= n) return;
+  const int len = __ldg(c.state + b);
+  const int64_t row0 = static_cast<int64_t>(b) * c.slots + t0;
+  const unsigned short* sc = reinterpret_cast<const unsigned short*>(c.scales) +
+                             static_cast<int64_t>(b) * kGroups * c.slots + t0;
+  uint32_t w[kGetSlots][3], s[kGetSlots][3];
+#pragma unroll
+  for (int k = 0; k < kGetSlots; ++k) {  // (slots are a multiple of 64: all four exist)
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(c.codes + (row0 + k) * kRowBytes);
+    w[k][0] = __ldg(src + lane);
+    w[k][1] = __ldg(src + 32 + lane);
+    w[k][2] = lane < 8 ? __ldg(src + 64 + lane) : 0u;
+    s[k][0] = __ldg(sc + static_cast<int64_t>(lane >> 4) * c.slots + k);
+    s[k][1] = __ldg(sc + static_cast<int64_t>(2 + (lane >> 4)) * c.slots + k);
+    s[k][2] = __ldg(sc + static_cast<int64_t>(4) * c.slots + k);
   }
-  lat[i * 64 + lane] = v0;
-  lat[i * 64 + 32 + lane] = v1;
-  if (lane < 8) kpe[i * 8 + lane] = v2;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int k = 0; k < kGetSlots; ++k) {
+    if (t0 + k >= n) break;
+    const bool in = t0 + k < len;
+    const int64_t o = static_cast<int64_t>(b) * n + t0 + k;
+    lat[o * 64 + lane] = in ? values8(w[k][0], s[k][0] * 0x00010001u) : zero;
+    lat[o * 64 + 32 + lane] = in ? values8(w[k][1], s[k][1] * 0x00010001u) : zero;
+    if (lane < 8) kpe[o * 8 + lane] = in ? values8(w[k][2], s[k][2] * 0x00010001u) : zero;
+  }
 }
 
 // ---- attention ------------------------------------------------------------------------------
@@ -996,16 +1039,250 @@ __device__ __forceinline__ int block_rank(bool flag, int* warp_sum, int* total) 
   return base + __popc(m & ((1u << lane) - 1u));
 }
 
-// One block per sequence: the budget-th largest key by four 8-bit radix passes, ties to the
-// lowest slots, then src_of[b, j] = the slot whose row result slot j takes: itself where slot
-// j < budget stays, else the next survivor from behind the budget, both in ascending order.
+// Result slots j0 .. j0 + 3 (below n) of sequence b take the rows src[j0 ..]: a warp's work, all
+// loads before the stores.  Lanes: 18 16-byte pieces of codes a row, and for the small fields one
+// (field, row) each.  In place, rows that stay are skipped: sources lie at or behind the budget
+// and targets before it, so no row is both.
+constexpr int kMoveRows = 4;
+__device__ __forceinline__ void move_rows(const Cache& s, const Cache& d, int b, int j0, int n,
+                                          const int32_t* src, bool in_place) {
+  const int lane = threadIdx.x & 31;
+  const int mine = lane & 3;
+  int t = -1;
+  if (j0 + mine < n) t = __ldcg(src + j0 + mine);
+  if (in_place && t == j0 + mine) t = -1;
+  uint4 v[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const int i = lane + 32 * k, row = i / 18;
+    const int tr = __shfl_sync(0xffffffffu, t, row & 3);
+    if (row < kMoveRows && tr >= 0)
+      v[k] = __ldcg(reinterpret_cast<const uint4*>(
+                        s.codes + (static_cast<int64_t>(b) * s.slots + tr) * kRowBytes) + i % 18);
+  }
+  const int f = lane >> 2;  // field: 0-4 scales, 5 rstd, 6 position, 7 mass
+  const int64_t ss = static_cast<int64_t>(b) * s.slots + t, ds = static_cast<int64_t>(b) * d.slots + j0 + mine;
+  const int64_t gs = (static_cast<int64_t>(b) * kGroups + f) * s.slots + t;
+  const int64_t gd = (static_cast<int64_t>(b) * kGroups + f) * d.slots + j0 + mine;
+  __nv_bfloat16 g = __float2bfloat16_rn(0.f);
+  uint32_t w = 0u;
+  if (t >= 0) {
+    if (f < 5) g = s.scales[gs];
+    else w = __ldcg((f == 5   ? reinterpret_cast<const uint32_t*>(s.rstd)
+                     : f == 6 ? reinterpret_cast<const uint32_t*>(s.pos)
+                              : reinterpret_cast<const uint32_t*>(s.mass)) + ss);
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const int i = lane + 32 * k, row = i / 18;
+    const int tr = __shfl_sync(0xffffffffu, t, row & 3);
+    if (row < kMoveRows && tr >= 0)
+      reinterpret_cast<uint4*>(d.codes + (static_cast<int64_t>(b) * d.slots + j0 + row) * kRowBytes)[i % 18] = v[k];
+  }
+  if (t >= 0) {
+    if (f < 5) d.scales[gd] = g;
+    else (f == 5   ? reinterpret_cast<uint32_t*>(d.rstd)
+          : f == 6 ? reinterpret_cast<uint32_t*>(d.pos)
+                   : reinterpret_cast<uint32_t*>(d.mass))[ds] = w;
+  }
+}
+
+// Sum of v over the block (1024 threads); `red`: 32 words, not in use by an earlier call any more
+// (callers alternate between two).
+__device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t* red) {
+  const uint32_t w = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = w;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, red[threadIdx.x & 31]);
+}
+// Exclusive prefix of v over the block's threads.
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t incl = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 31) red[warp] = incl;
+  __syncthreads();
+  const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? red[lane] : 0u);
+  return before + incl - v;
+}
+
+// One block per sequence: which slots stay, and src_of[b, j] = the slot whose row result slot j
+// takes: itself where slot j < budget stays, else the next survivor from behind the budget,
+// both in ascending order.  Up to 1024 * IPT slots, whose keys stay in registers (thread i has
+// slots IPT i ..): the budget-th largest key is found two bits a round, by counting the keys at
+// or above three candidates, so no histogram's atomics collide however alike the weights are
+// (four 8-bit histogram passes: 23 us for 333 slots and 68 us for 8192; this: see evict_plan_long).
+// `rows_here`: the block moves the rows itself.
+template <int IPT>
 __global__ void __launch_bounds__(1024)
-    evict_plan_kernel(Cache c, int32_t* __restrict__ dst_state, int budget, int recent,
+    evict_plan_kernel(Cache c, Cache dst, int budget, int recent, int32_t* __restrict__ src_of,
+                      int32_t* __restrict__ holes, int rows_here, int in_place) {
+  __shared__ uint32_t red[6][32];
+  __shared__ uint32_t list[IPT == 1 ? 1 : 1024];
+  ptx::pdl_launch_dependents();
+  const int b = blockIdx.x;
+  const int len = min(max(c.state[b], 0), c.slots), next = c.state[c.batch + b];
+  int32_t* src = src_of + static_cast<int64_t>(b) * budget;
+  int32_t* hole = holes + static_cast<int64_t>(b) * budget;
+  const int kept_n = min(len, budget);
+  const int t0 = threadIdx.x * IPT;
+  if (len > budget) {
+    const float* mass = c.mass + static_cast<int64_t>(b) * c.slots;
+    const int32_t* pos = c.pos + static_cast<int64_t>(b) * c.slots;
+    const int from = next - recent;
+    uint32_t key[IPT];
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) key[i] = 0u;
+    if (IPT >= 4) {
+#pragma unroll
+      for (int i = 0; i < IPT; i += 4)
+        if (t0 + i < c.slots) {  // (slots are a multiple of 64)
+          const float4 m = *reinterpret_cast<const float4*>(mass + t0 + i);
+          const int4 p = *reinterpret_cast<const int4*>(pos + t0 + i);
+          key[i] = evict_key(m.x, p.x, from);
+          key[i + (IPT > 1 ? 1 : 0)] = evict_key(m.y, p.y, from);
+          key[i + (IPT > 2 ? 2 : 0)] = evict_key(m.z, p.z, from);
+          key[i + (IPT > 3 ? 3 : 0)] = evict_key(m.w, p.w, from);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < IPT; ++i)
+        if (t0 + i < len) key[i] = evict_key(mass[t0 + i], pos[t0 + i], from);
+    }
+#pragma unroll
+    for (int i = 0; i < IPT; ++i)
+      if (t0 + i >= len) key[i] = 0u;  // below every candidate
+    // the largest v with at least `budget` keys >= v
+    uint32_t v = 0;
+    int want = budget;          // keys still to be found among those that are compared
+    uint32_t one = 0;           // this thread's key once 1024 or fewer can still decide
+    bool few = IPT == 1;
+    if (IPT == 1) one = key[0];
+    uint32_t in_range = len;    // keys in [v, v + 2^(shift + 2)) before a round ...
+    uint32_t over_end = 0;      // ... and at or above its end, of those compared
+#pragma unroll 1
+    for (int shift = 30, round = 0; shift >= 0; shift -= 2, ++round) {
+      if (IPT > 1 && !few && in_range <= 1024 && shift < 30) {
+        // the keys that share v's upper bits, one to a thread; those above them are counted off
+        few = true;
+        const uint32_t top = v >> (shift + 2);
+        uint32_t mine = 0, over = 0;
+#pragma unroll
+        for (int i = 0; i < IPT; ++i) {
+          mine += (key[i] >> (shift + 2)) == top && t0 + i < len ? 1u : 0u;
+          over += (key[i] >> (shift + 2)) > top ? 1u : 0u;
+        }
+        uint32_t at = block_prefix(mine, red[4]);
+        want -= static_cast<int>(block_sum(over, red[5]));
+        over_end = 0;
+#pragma unroll
+        for (int i = 0; i < IPT; ++i)
+          if ((key[i] >> (shift + 2)) == top && t0 + i < len) list[at++] = key[i];
+        __syncthreads();
+        one = threadIdx.x < in_range ? list[threadIdx.x] : 0u;
+      }
+      uint32_t n12 = 0, n3 = 0;
+      const uint32_t c1 = v | (1u << shift), c2 = v | (2u << shift), c3 = v | (3u << shift);
+      if (few) {
+        n12 = (one >= c1 ? 1u : 0u) + (one >= c2 ? 0x10000u : 0u);
+        n3 = one >= c3 ? 1u : 0u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < IPT; ++i) {
+          n12 += (key[i] >= c1 ? 1u : 0u) + (key[i] >= c2 ? 0x10000u : 0u);
+          n3 += key[i] >= c3 ? 1u : 0u;
+        }
+      }
+      // a block has at most 32768 keys: two counts to a word
+      const uint32_t w12 = __reduce_add_sync(0xffffffffu, n12);
+      const uint32_t w3 = __reduce_add_sync(0xffffffffu, n3);
+      uint32_t* r = red[2 * (round & 1)];
+      if ((threadIdx.x & 31) == 0) {
+        r[threadIdx.x >> 5] = w12;
+        r[32 + (threadIdx.x >> 5)] = w3;
+      }
+      __syncthreads();
+      const uint32_t s12 = __reduce_add_sync(0xffffffffu, r[threadIdx.x & 31]);
+      const int n1 = static_cast<int>(s12 & 0xFFFFu), n2 = static_cast<int>(s12 >> 16);
+      const int nn3 = static_cast<int>(__reduce_add_sync(0xffffffffu, r[32 + (threadIdx.x & 31)]));
+      // (the keys at or above the bucket's end were counted by the round before: only the counts
+      // inside it matter for in_range)
+      const int above_v = static_cast<int>(over_end);
+      if (nn3 >= want) {
+        v = c3;
+        in_range = nn3 - above_v;
+      } else if (n2 >= want) {
+        v = c2;
+        in_range = n2 - nn3;
+        over_end = nn3;
+      } else if (n1 >= want) {
+        v = c1;
+        in_range = n1 - n2;
+        over_end = n2;
+      } else {
+        in_range = in_range + above_v - n1;
+        over_end = n1;
+      }
+    }
+    uint32_t above = 0, ties = 0;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      above += key[i] > v ? 1u : 0u;
+      ties += key[i] == v && t0 + i < len ? 1u : 0u;
+    }
+    // (the last round left red[2..3] in use: 15 is odd)
+    const uint32_t need = budget - block_sum(above, red[0]);  // ties that stay: the first ones
+    uint32_t rank = block_prefix(ties, red[1]);
+    uint32_t keep = 0, n_hole = 0, n_late = 0;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int t = t0 + i;
+      bool k = key[i] > v;
+      if (key[i] == v && t < len) k = rank++ < need;
+      if (k) keep |= 1u << i;
+      n_hole += t < budget && !k ? 1u : 0u;
+      n_late += t >= budget && k ? 1u : 0u;
+    }
+    const uint32_t before = block_prefix(n_hole | (n_late << 16), red[2]);
+    uint32_t h = before & 0xFFFFu, l = before >> 16;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int t = t0 + i;
+      if (t >= budget) continue;
+      if (keep >> i & 1u) src[t] = t;
+      else hole[h++] = t;
+    }
+    __syncthreads();  // the holes are written before survivors are paired with them
+#pragma unroll
+    for (int i = 0; i < IPT; ++i)
+      if (t0 + i >= budget && (keep >> i & 1u)) src[hole[l++]] = t0 + i;
+  } else {
+    for (int j = threadIdx.x; j < kept_n; j += 1024) src[j] = j;
+  }
+  __syncthreads();
+  if (rows_here)
+    for (int j = (threadIdx.x >> 5) * kMoveRows; j < kept_n; j += 32 * kMoveRows)
+      move_rows(c, dst, b, j, kept_n, src, in_place != 0);
+  if (threadIdx.x == 0) {
+    dst.state[b] = kept_n;
+    dst.state[c.batch + b] = next;
+  }
+}
+
+// The same for any number of slots: the keys are made again for each pass, four of which build
+// histograms of 8 bits, and slots are ranked tile by tile.
+__global__ void __launch_bounds__(1024)
+    evict_plan_long_kernel(Cache c, Cache dst, int budget, int recent,
                       int32_t* __restrict__ src_of, int32_t* __restrict__ holes) {
   __shared__ int hist[256];
   __shared__ int warp_sum[32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
+  ptx::pdl_launch_dependents();
   const int b = blockIdx.x;
   const int len = min(max(c.state[b], 0), c.slots), next = c.state[c.batch + b];
   const float* mass = c.mass + static_cast<int64_t>(b) * c.slots;
@@ -1068,36 +1345,20 @@ __global__ void __launch_bounds__(1024)
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    dst_state[b] = kept_n;
-    dst_state[c.batch + b] = next;
+    dst.state[b] = kept_n;
+    dst.state[c.batch + b] = next;
   }
 }
 
-// Result slot j of sequence b takes row src_of[b, j] (a warp per row; in place, rows that
-// stay are skipped: sources are at or behind the budget and targets before it, so no row
-// is both).
+// The rows of a plan.
 __global__ void __launch_bounds__(256)
     evict_move_kernel(Cache s, Cache d, int budget, const int32_t* __restrict__ src_of,
                       int in_place) {
+  ptx::pdl_wait();
   const int b = blockIdx.y;
-  const int j = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (j >= d.state[b]) return;
-  const int t = src_of[static_cast<int64_t>(b) * budget + j];
-  if (in_place && t == j) return;
-  const int64_t sr = static_cast<int64_t>(b) * s.slots + t;
-  const int64_t dr = static_cast<int64_t>(b) * d.slots + j;
-  if (lane < kRowBytes / 16)
-    reinterpret_cast<uint4*>(d.codes + dr * kRowBytes)[lane] =
-        reinterpret_cast<const uint4*>(s.codes + sr * kRowBytes)[lane];
-  if (lane >= 18 && lane < 23) {
-    const int64_t g = lane - 18;
-    d.scales[(static_cast<int64_t>(b) * kGroups + g) * d.slots + j] =
-        s.scales[(static_cast<int64_t>(b) * kGroups + g) * s.slots + t];
-  }
-  if (lane == 23) d.rstd[dr] = s.rstd[sr];
-  if (lane == 24) d.pos[dr] = s.pos[sr];
-  if (lane == 25) d.mass[dr] = s.mass[sr];
+  const int j = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kMoveRows;
+  const int n = __ldcg(d.state + b);
+  if (j < n) move_rows(s, d, b, j, n, src_of + static_cast<int64_t>(b) * budget, in_place != 0);
 }
 
 Cache cache_of(void* codes, void* scales, float* rstd, int32_t* pos, float* mass, int32_t* state,
@@ -1157,16 +1418,44 @@ int launch_append(const Cache& c, const void* lat, int64_t lat_ld, const void* k
                   const void* cos_t, const void* sin_t, int table_rows, float eps,
                   cudaStream_t s) {
   if (c.batch == 0 || n_new == 0) return DS_OK;
-  const int gx = (n_new + 7) / 8;
-  append_kernel<<<dim3(gx, c.batch), 256, 0, s>>>(
+  const int warps = n_new <= 64 ? 8 : 32;
+  append_kernel<<<dim3((n_new + warps - 1) / warps, c.batch), warps * 32, 0, s>>>(
       c, static_cast<const __nv_bfloat16*>(lat), lat_ld, static_cast<const __nv_bfloat16*>(kpe),
       kpe_ld, src_bstride, n_new, new_lens, static_cast<const __nv_bfloat16*>(cos_t),
-      static_cast<const __nv_bfloat16*>(sin_t), table_rows, eps, gx == 1 ? 1 : 0);
+      static_cast<const __nv_bfloat16*>(sin_t), table_rows, eps);
   DS_LAUNCH_CHECK("append_kernel");
-  if (gx > 1) {
-    advance_kernel<<<(c.batch + 255) / 256, 256, 0, s>>>(c, n_new, new_lens);
-    DS_LAUNCH_CHECK("advance_kernel");
-  }
+  return DS_OK;
+}
+
+int launch_evict(const Cache& s, const Cache& d, int budget, int recent, bool in_place,
+                 int32_t* src_of, int32_t* holes, cudaStream_t st) {
+  // few rows: the planning block moves them (no second launch); many: all SMs do
+  const int here = budget <= 256 ? 1 : 0;
+  if (s.slots <= 1024)
+    evict_plan_kernel<1><<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes, here,
+                                                   in_place);
+  else if (s.slots <= 8192)
+    evict_plan_kernel<8><<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes, here,
+                                                   in_place);
+  else if (s.slots <= 32768)
+    evict_plan_kernel<32><<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes, here,
+                                                    in_place);
+  else
+    evict_plan_long_kernel<<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes);
+  DS_LAUNCH_CHECK("evict_plan_kernel");
+  if (here && s.slots <= 32768) return DS_OK;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((budget + 8 * kMoveRows - 1) / (8 * kMoveRows), s.batch);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  DS_CUDA(cudaLaunchKernelEx(&cfg, evict_move_kernel, s, d, budget,
+                             static_cast<const int32_t*>(src_of), in_place ? 1 : 0));
+  DS_LAUNCH_CHECK("evict_move_kernel");
   return DS_OK;
 }
 
@@ -1256,11 +1545,12 @@ int ds_mla_cache4_get(const void* codes, const void* scales_bf16, const int32_t*
              "mla_cache4_get: null pointer");
   DS_REQUIRE(ds::aligned16(codes) && ds::aligned16(latent_out_bf16) && ds::aligned16(kpe_out_bf16),
              "mla_cache4_get: 16-byte aligned pointers");
-  DS_REQUIRE((rows + 7) / 8 < (1LL << 31), "mla_cache4_get: too many rows");
+  DS_REQUIRE(batch <= 65535, "mla_cache4_get: batch must be at most 65535");
   const ds::c4::Cache c = ds::c4::cache_of(const_cast<void*>(codes), const_cast<void*>(scales_bf16),
                                            nullptr, nullptr, nullptr,
                                            const_cast<int32_t*>(state), batch, slots);
-  ds::c4::get_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0,
+  const int per_block = 8 * ds::c4::kGetSlots;
+  ds::c4::get_kernel<<<dim3((seq_len + per_block - 1) / per_block, batch), 256, 0,
                        static_cast<cudaStream_t>(stream)>>>(
       c, seq_len, static_cast<uint4*>(latent_out_bf16), static_cast<uint4*>(kpe_out_bf16));
   DS_LAUNCH_CHECK("get_kernel");
@@ -1331,13 +1621,8 @@ int ds_mla_cache4_evict(void* codes, void* scales_bf16, float* rstd, int32_t* po
   int32_t* holes = w.take<int32_t>(static_cast<size_t>(batch) * budget);
   if (!w.ok())
     return ds::fail(DS_ERR_WORKSPACE, "mla_cache4_evict: workspace needs %zu bytes", w.used);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  ds::c4::evict_plan_kernel<<<batch, 1024, 0, st>>>(s, dst_state, budget, recent, src_of, holes);
-  DS_LAUNCH_CHECK("evict_plan_kernel");
-  ds::c4::evict_move_kernel<<<dim3((budget + 7) / 8, batch), 256, 0, st>>>(s, d, budget, src_of,
-                                                                           in_place ? 1 : 0);
-  DS_LAUNCH_CHECK("evict_move_kernel");
-  return DS_OK;
+  return ds::c4::launch_evict(s, d, budget, recent, in_place, src_of, holes,
+                              static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

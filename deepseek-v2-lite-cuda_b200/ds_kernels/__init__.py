@@ -16,6 +16,7 @@ raises ImportError, and every op requires CUDA tensors.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import List, Optional, Sequence
 
@@ -164,8 +165,14 @@ def _require(cond: bool, msg: str) -> None:
         raise RuntimeError(msg)
 
 
+# the current stream's handle and the current device, without building Stream / device objects
+# (2 us a call otherwise, as much as a small kernel runs)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.get_device())
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -180,13 +187,14 @@ class _on_device:
     """Make the tensor's device current for the duration of a C-ABI call."""
 
     def __init__(self, t: torch.Tensor):
-        self.ctx = torch.cuda.device(t.device)
+        self.ctx = None if t.get_device() == _current_device() else torch.cuda.device(t.device)
 
     def __enter__(self):
-        self.ctx.__enter__()
+        if self.ctx is not None:
+            self.ctx.__enter__()
 
     def __exit__(self, *exc):
-        return self.ctx.__exit__(*exc)
+        return None if self.ctx is None else self.ctx.__exit__(*exc)
 
 
 # --------------------------------------------------------------------------------------------
@@ -770,33 +778,41 @@ def mla_decode_step(x: torch.Tensor, w_dec: torch.Tensor, w_out: torch.Tensor, c
 
 
 # ---------------------------------------------------------------------- 8-bit integer linear
+# These operators run for a few microseconds, so a good call pays one test of everything it
+# needs; only a call that fails it looks for the first fault and its message.
+_bf16, _i8, _i32, _u8, _f32 = (torch.bfloat16, torch.int8, torch.int32, torch.uint8, torch.float32)
+
+
 def int8_quantize(x: torch.Tensor) -> List[torch.Tensor]:
     """Rows of x to 8-bit integers, one scale per row (additive): x bf16 [..., K] ->
     [q int8 [..., K], scale f32 [...]] with a = max |row|, q = rint(127 x / a) (ties to even),
     scale = a / 127.  A row of zeros gives zeros and scale 0; a row with an infinity or a NaN
     gives zeros and scale NaN.  Weights [N, K] are quantised per output channel the same way.
     K: a multiple of 16."""
-    _require(x.is_cuda, "int8_quantize: x must be a CUDA tensor.")
-    _require(x.dtype == torch.bfloat16, "int8_quantize: x must be bfloat16.")
-    _require(x.dim() >= 1 and x.shape[-1] > 0, "int8_quantize: x must be [..., K].")
+    if not (x.is_cuda and x.dtype is _bf16 and x.dim() >= 1 and x.shape[-1] > 0
+            and x.shape[-1] % 16 == 0):
+        _require(x.is_cuda, "int8_quantize: x must be a CUDA tensor.")
+        _require(x.dtype == _bf16, "int8_quantize: x must be bfloat16.")
+        _require(x.dim() >= 1 and x.shape[-1] > 0, "int8_quantize: x must be [..., K].")
+        _require(False, "int8_quantize: K must be a multiple of 16.")
     K = x.shape[-1]
-    _require(K % 16 == 0, "int8_quantize: K must be a multiple of 16.")
-    x2 = _rows_2d(x)
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    q = torch.empty(x.shape, dtype=_i8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=_f32, device=x.device)
     if x.numel() == 0:
         return [q, scale]
+    x2 = _rows_2d(x)
     with _on_device(x):
-        _check(_lib.ds_int8_quantize(_ptr(x2), x2.stride(0), x2.shape[0], K, _ptr(q), _ptr(scale),
-                                     _stream(x)), "int8_quantize")
+        _check(_lib.ds_int8_quantize(x2.data_ptr(), x2.stride(0), x2.shape[0], K, q.data_ptr(),
+                                     scale.data_ptr(), _stream(x)), "int8_quantize")
     return [q, scale]
 
 
 def _rows_2d(x: torch.Tensor) -> torch.Tensor:
     """x [..., K] as [rows, K] whose rows are contiguous and start on 16-byte boundaries (a
     copy only where the strides do not allow a view)."""
-    x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    ld, inner = x2.stride()
+    if inner != 1 or ld % 8 or ld < x2.shape[1] or x2.data_ptr() % 16:
         x2 = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device).copy_(x2)
     return x2
 
@@ -809,33 +825,46 @@ def int8_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
     (32 bits) and scaled once: bf16(acc * (scale_row * w_scale)).  K: a multiple of 16, at most
     131072; N: a multiple of 8.  `workspace` (uint8, at least int8_linear_workspace_size bytes)
     saves the allocation; calls that overlap need different ones."""
-    _require(x.is_cuda and w_q.is_cuda and w_scale.is_cuda,
-             "int8_linear: x, w_q and w_scale must be CUDA tensors.")
-    _require(x.dtype == torch.bfloat16, "int8_linear: x must be bfloat16.")
-    _require(w_q.dtype == torch.int8 and w_q.dim() == 2 and w_q.is_contiguous(),
-             "int8_linear: w_q must be a contiguous int8 [N, K] tensor.")
-    _require(w_scale.dtype == torch.float32 and tuple(w_scale.shape) == (w_q.shape[0],)
-             and w_scale.is_contiguous(), "int8_linear: w_scale must be a contiguous float32 [N] tensor.")
-    _require(w_q.device == x.device and w_scale.device == x.device,
-             "int8_linear: x, w_q and w_scale must be on one device.")
+    dev = x.device
+    if not (x.is_cuda and x.dtype is _bf16 and w_q.dtype is _i8 and w_scale.dtype is _f32
+            and w_q.dim() == 2 and w_q.is_contiguous() and w_scale.is_contiguous()
+            and w_scale.dim() == 1 and w_scale.shape[0] == w_q.shape[0] and w_q.device == dev
+            and w_scale.device == dev and x.dim() >= 1 and x.shape[-1] == w_q.shape[1]
+            and w_q.shape[1] > 0 and w_q.shape[1] % 16 == 0 and w_q.shape[0] % 8 == 0):
+        _require(x.is_cuda and w_q.is_cuda and w_scale.is_cuda,
+                 "int8_linear: x, w_q and w_scale must be CUDA tensors.")
+        _require(x.dtype == _bf16, "int8_linear: x must be bfloat16.")
+        _require(w_q.dtype == _i8 and w_q.dim() == 2 and w_q.is_contiguous(),
+                 "int8_linear: w_q must be a contiguous int8 [N, K] tensor.")
+        _require(w_scale.dtype == _f32 and tuple(w_scale.shape) == (w_q.shape[0],)
+                 and w_scale.is_contiguous(),
+                 "int8_linear: w_scale must be a contiguous float32 [N] tensor.")
+        _require(w_q.device == dev and w_scale.device == dev,
+                 "int8_linear: x, w_q and w_scale must be on one device.")
+        _require(x.dim() >= 1 and x.shape[-1] == w_q.shape[1],
+                 f"int8_linear: x last dim must match w_q inner dim {w_q.shape[1]}.")
+        _require(w_q.shape[1] > 0 and w_q.shape[1] % 16 == 0,
+                 "int8_linear: K must be a positive multiple of 16.")
+        _require(False, "int8_linear: N must be a multiple of 8.")
     N, K = w_q.shape
-    _require(x.dim() >= 1 and x.shape[-1] == K,
-             f"int8_linear: x last dim must match w_q inner dim {K}.")
-    _require(K > 0 and K % 16 == 0, "int8_linear: K must be a positive multiple of 16.")
-    _require(N % 8 == 0, "int8_linear: N must be a multiple of 8.")
-    out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
+    if x.dim() == 2:
+        out = torch.empty((x.shape[0], N), dtype=_bf16, device=dev)
+    else:
+        out = torch.empty((*x.shape[:-1], N), dtype=_bf16, device=dev)
     if out.numel() == 0:
         return out
     x2 = _rows_2d(x)
-    need = int8_linear_workspace_size(x2.shape[0], N, K)
-    workspace = _scratch(workspace, need, x.device, "int8_linear")
+    rows = x2.shape[0]
+    workspace = _scratch(workspace, int8_linear_workspace_size(rows, N, K), dev, "int8_linear")
     with _on_device(x):
-        _check(_lib.ds_int8_linear(_ptr(x2), x2.stride(0), _ptr(w_q), _ptr(w_scale), _ptr(out),
-                                   x2.shape[0], N, K, _ptr(workspace), workspace.numel(),
-                                   _stream(x)), "int8_linear")
+        _check(_lib.ds_int8_linear(x2.data_ptr(), x2.stride(0), w_q.data_ptr(),
+                                   w_scale.data_ptr(), out.data_ptr(), rows, N, K,
+                                   workspace.data_ptr(), workspace.numel(), _stream(x)),
+               "int8_linear")
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def int8_linear_workspace_size(rows: int, out_features: int, in_features: int) -> int:
     return int(_lib.ds_int8_linear_workspace_size(rows, out_features, in_features))
 
@@ -843,8 +872,8 @@ def int8_linear_workspace_size(rows: int, out_features: int, in_features: int) -
 def _scratch(workspace: Optional[torch.Tensor], need: int, device: torch.device,
              op: str) -> torch.Tensor:
     if workspace is None or workspace.numel() < need:
-        return _workspace(need, device)
-    _require(workspace.dtype == torch.uint8 and workspace.is_contiguous()
+        return torch.empty(max(need, 1), dtype=_u8, device=device)
+    _require(workspace.dtype == _u8 and workspace.is_contiguous()
              and workspace.device == device and workspace.data_ptr() % 16 == 0,
              f"{op}: workspace must be a contiguous, 16-byte aligned uint8 tensor on x's device.")
     return workspace
@@ -855,11 +884,6 @@ def _require_cache4(cache, op: str) -> None:
     _require(cache.codes.is_cuda, f"{op}: the cache must reside on a CUDA device.")
 
 
-def _cache4_ptrs(cache):
-    return (_ptr(cache.codes), _ptr(cache.scales), _ptr(cache.rstd), _ptr(cache.pos),
-            _ptr(cache.mass), _ptr(cache.state))
-
-
 def mla_cache4_append(latent: torch.Tensor, k_pe: torch.Tensor, cache, cos: torch.Tensor,
                       sin: torch.Tensor, eps: float = 1e-6,
                       new_lens: Optional[torch.Tensor] = None) -> None:
@@ -868,48 +892,52 @@ def mla_cache4_append(latent: torch.Tensor, k_pe: torch.Tensor, cache, cos: torc
     (mla_cache.LatentKVCache4), k_pe rotated at its position (cos/sin bf16 [positions, 64]).
     new_lens int32 [bsz] (on the device): only the first new_lens[b] tokens of sequence b (a
     ragged, padded batch)."""
-    _require(latent.is_cuda and k_pe.is_cuda, "mla_cache4_append: inputs must be CUDA tensors.")
-    _require(latent.dtype == torch.bfloat16 and k_pe.dtype == torch.bfloat16,
-             "mla_cache4_append: latent and k_pe must be bfloat16.")
-    _require(latent.dim() == 3 and latent.shape[2] == 512 and latent.shape[0] == cache.bsz
-             and tuple(k_pe.shape) == (*latent.shape[:2], 64),
-             "mla_cache4_append: latent must be [bsz, n, 512] and k_pe [bsz, n, 64].")
-    _require(latent.device == cache.codes.device and k_pe.device == cache.codes.device,
-             "mla_cache4_append: inputs and cache must be on one device.")
-    _check_tables(cos, sin, cache, "mla_cache4_append")
-    B, n, _ = latent.shape
-    if B * n == 0:
-        return
+    dev = cache.device
+    shape = latent.shape
+    if not (latent.is_cuda and latent.dtype is _bf16 and k_pe.dtype is _bf16 and len(shape) == 3
+            and shape[2] == 512 and shape[0] == cache.bsz and k_pe.shape == (shape[0], shape[1], 64)
+            and latent.device == dev and k_pe.device == dev):
+        _require(latent.is_cuda and k_pe.is_cuda, "mla_cache4_append: inputs must be CUDA tensors.")
+        _require(latent.dtype == _bf16 and k_pe.dtype == _bf16,
+                 "mla_cache4_append: latent and k_pe must be bfloat16.")
+        _require(latent.dim() == 3 and shape[2] == 512 and shape[0] == cache.bsz
+                 and tuple(k_pe.shape) == (*shape[:2], 64),
+                 "mla_cache4_append: latent must be [bsz, n, 512] and k_pe [bsz, n, 64].")
+        _require(False, "mla_cache4_append: inputs and cache must be on one device.")
+    _check_tables(cos, sin, dev, "mla_cache4_append")
+    B, n, _ = shape
     if new_lens is not None:
-        _require(new_lens.is_cuda and new_lens.dtype == torch.int32 and new_lens.is_contiguous()
-                 and tuple(new_lens.shape) == (B,) and new_lens.device == cache.codes.device,
+        _require(new_lens.dtype is _i32 and new_lens.dim() == 1 and new_lens.shape[0] == B
+                 and new_lens.is_contiguous() and new_lens.device == dev,
                  "mla_cache4_append: new_lens must be a contiguous int32 [bsz] tensor on the "
                  "cache's device.")
+    if n == 0:
+        return
     cache._check_room(n, cos.shape[0])
-    ok = (latent.stride(2) == 1 and k_pe.stride(2) == 1 and latent.stride(1) % 8 == 0
-          and k_pe.stride(1) % 8 == 0 and latent.data_ptr() % 16 == 0 and k_pe.data_ptr() % 16 == 0
-          and latent.stride(1) > 0 and k_pe.stride(1) > 0)
-    rows = latent.stride(0) // latent.stride(1) if ok else 0
-    if not ok or latent.stride(0) != rows * latent.stride(1) or k_pe.stride(0) != rows * k_pe.stride(1):
-        latent = torch.empty(latent.shape, dtype=latent.dtype, device=latent.device).copy_(latent)
-        k_pe = torch.empty(k_pe.shape, dtype=k_pe.dtype, device=k_pe.device).copy_(k_pe)
-        rows = n
+    lb, lt, l1 = latent.stride()
+    kb, kt, k1 = k_pe.stride()
+    rows = lb // lt if lt > 0 else 0
+    if not (l1 == 1 and k1 == 1 and lt > 0 and kt > 0 and lt % 8 == 0 and kt % 8 == 0
+            and lb == rows * lt and kb == rows * kt and latent.data_ptr() % 16 == 0
+            and k_pe.data_ptr() % 16 == 0):
+        latent = torch.empty(shape, dtype=_bf16, device=dev).copy_(latent)
+        k_pe = torch.empty((B, n, 64), dtype=_bf16, device=dev).copy_(k_pe)
+        lt, kt, rows = 512, 64, n
     with _on_device(latent):
-        _check(_lib.ds_mla_cache4_append(_ptr(latent), latent.stride(1), _ptr(k_pe),
-                                         k_pe.stride(1), rows, n, _ptr(new_lens), _ptr(cos),
-                                         _ptr(sin), cos.shape[0], float(eps),
-                                         *_cache4_ptrs(cache), B, cache.slots, _stream(latent)),
+        _check(_lib.ds_mla_cache4_append(latent.data_ptr(), lt, k_pe.data_ptr(), kt, rows, n,
+                                         None if new_lens is None else new_lens.data_ptr(),
+                                         cos.data_ptr(), sin.data_ptr(), cos.shape[0], float(eps),
+                                         *cache._ptrs, B, cache.slots, _stream(latent)),
                "mla_cache4_append")
     cache._advance(n)
 
 
-def _check_tables(cos: torch.Tensor, sin: torch.Tensor, cache, op: str) -> None:
-    for t in (cos, sin):
-        _require(t.is_cuda and t.dtype == torch.bfloat16 and t.is_contiguous() and t.dim() == 2
-                 and t.shape[1] == 64 and t.shape[0] > 0 and t.shape == cos.shape
-                 and t.device == cache.codes.device,
-                 f"{op}: cos and sin must be contiguous bfloat16 [positions, 64] tensors on the "
-                 "cache's device.")
+def _check_tables(cos: torch.Tensor, sin: torch.Tensor, dev: torch.device, op: str) -> None:
+    if not (cos.dtype is _bf16 and sin.dtype is _bf16 and cos.dim() == 2 and cos.shape[1] == 64
+            and cos.shape[0] > 0 and sin.shape == cos.shape and cos.is_contiguous()
+            and sin.is_contiguous() and cos.device == dev and sin.device == dev):
+        _require(False, f"{op}: cos and sin must be contiguous bfloat16 [positions, 64] tensors on "
+                        "the cache's device.")
 
 
 def mla_cache4_get(cache, seq_len: Optional[int] = None) -> List[torch.Tensor]:
@@ -918,21 +946,27 @@ def mla_cache4_get(cache, seq_len: Optional[int] = None) -> List[torch.Tensor]:
     current_len (its longest sequence's bound)."""
     _require_cache4(cache, "mla_cache4_get")
     n = cache.current_len if seq_len is None else int(seq_len)
-    _require(0 <= n <= cache.slots, f"mla_cache4_get: seq_len={n} outside the cache.")
-    dev = cache.codes.device
-    lat = torch.empty((cache.bsz, n, 512), dtype=torch.bfloat16, device=dev)
-    kpe = torch.empty((cache.bsz, n, 64), dtype=torch.bfloat16, device=dev)
-    if lat.numel() == 0:
+    if not 0 <= n <= cache.slots:
+        _require(False, f"mla_cache4_get: seq_len={n} outside the cache.")
+    lat = torch.empty((cache.bsz, n, 512), dtype=_bf16, device=cache.device)
+    kpe = torch.empty((cache.bsz, n, 64), dtype=_bf16, device=cache.device)
+    if n == 0:
         return [lat, kpe]
     with _on_device(lat):
-        _check(_lib.ds_mla_cache4_get(_ptr(cache.codes), _ptr(cache.scales), _ptr(cache.state),
-                                      cache.bsz, cache.slots, n, _ptr(lat), _ptr(kpe),
+        _check(_lib.ds_mla_cache4_get(cache._ptrs[0], cache._ptrs[1], cache._ptrs[5], cache.bsz,
+                                      cache.slots, n, lat.data_ptr(), kpe.data_ptr(),
                                       _stream(lat)), "mla_cache4_get")
     return [lat, kpe]
 
 
 def mla_decode_attention4_workspace_size(batch: int, heads: int, slots: int, max_len: int,
                                          accumulate: bool = False) -> int:
+    """Bytes of mla_decode_attention4's workspace on the current device."""
+    return _attention4_workspace(batch, heads, slots, max_len, bool(accumulate), _current_device())
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention4_workspace(batch, heads, slots, max_len, accumulate, device) -> int:
     return int(_lib.ds_mla_decode_attention4_workspace_size(batch, heads, slots, max_len,
                                                             1 if accumulate else 0))
 
@@ -947,32 +981,34 @@ def mla_decode_attention4(q: torch.Tensor, cache, softmax_scale: float,
 
     With mass_decay the attention weights are accumulated for a later eviction:
     cache.mass[b, t] = mass_decay * cache.mass[b, t] + sum over heads of p(t)."""
-    _require(q.is_cuda and q.dtype == torch.bfloat16 and q.is_contiguous(),
-             "mla_decode_attention4: q must be a contiguous bfloat16 CUDA tensor.")
-    _require(q.dim() == 3 and q.shape[0] == cache.bsz and q.shape[2] == 576,
-             "mla_decode_attention4: q must be [bsz, heads, 576].")
-    _require(q.device == cache.codes.device,
-             "mla_decode_attention4: q and cache must be on one device.")
-    B, heads, _ = q.shape
-    _require(1 <= heads <= 128, "mla_decode_attention4: heads must be in [1, 128].")
-    _require(mass_decay is None or 0.0 <= mass_decay <= 1.0,
-             "mla_decode_attention4: mass_decay must be in [0, 1].")
-    if out is None:
-        out = torch.empty((B, heads * 512), dtype=torch.bfloat16, device=q.device)
-    else:
-        _check_out(out, B, heads * 512, q.device)
-    if B == 0:
-        return out
+    dev = cache.device
+    if not (q.is_cuda and q.dtype is _bf16 and q.is_contiguous() and q.dim() == 3
+            and q.shape[0] == cache.bsz and q.shape[2] == 576 and q.device == dev
+            and 1 <= q.shape[1] <= 128 and q.data_ptr() % 16 == 0):
+        _require(q.is_cuda and q.dtype == _bf16 and q.is_contiguous(),
+                 "mla_decode_attention4: q must be a contiguous bfloat16 CUDA tensor.")
+        _require(q.dim() == 3 and q.shape[0] == cache.bsz and q.shape[2] == 576,
+                 "mla_decode_attention4: q must be [bsz, heads, 576].")
+        _require(q.device == dev, "mla_decode_attention4: q and cache must be on one device.")
+        _require(1 <= q.shape[1] <= 128, "mla_decode_attention4: heads must be in [1, 128].")
+        q = q.clone()  # a view that starts off a 16-byte boundary
     acc = mass_decay is not None
+    if acc and not 0.0 <= mass_decay <= 1.0:
+        _require(False, "mla_decode_attention4: mass_decay must be in [0, 1].")
+    B, heads, _ = q.shape
+    if out is None:
+        out = torch.empty((B, heads * 512), dtype=_bf16, device=dev)
+    else:
+        _check_out(out, B, heads * 512, dev)
     max_len = cache.bound_for_launch
-    need = mla_decode_attention4_workspace_size(B, heads, cache.slots, max_len, acc)
-    workspace = _scratch(workspace, need, q.device, "mla_decode_attention4")
     with _on_device(q):
+        need = _attention4_workspace(B, heads, cache.slots, max_len, acc, q.get_device())
+        workspace = _scratch(workspace, need, dev, "mla_decode_attention4")
+        codes, scales, rstd, _, mass, state = cache._ptrs
         _check(_lib.ds_mla_decode_attention4(
-            _ptr(q), heads, _ptr(cache.codes), _ptr(cache.scales), _ptr(cache.rstd),
-            _ptr(cache.mass), _ptr(cache.state), B, cache.slots, max_len, float(softmax_scale),
-            1 if acc else 0, float(mass_decay or 0.0), _ptr(out), _ptr(workspace),
-            workspace.numel(), _stream(q)), "mla_decode_attention4")
+            q.data_ptr(), heads, codes, scales, rstd, mass, state, B, cache.slots, max_len,
+            softmax_scale, 1 if acc else 0, mass_decay if acc else 0.0, out.data_ptr(),
+            workspace.data_ptr(), workspace.numel(), _stream(q)), "mla_decode_attention4")
     return out
 
 
@@ -986,19 +1022,26 @@ def mla_cache4_evict(cache, budget: int, recent: int = 0, out=None):
     _require_cache4(cache, "mla_cache4_evict")
     dst = cache if out is None else out
     budget, recent = int(budget), int(recent)
-    _require(dst.bsz == cache.bsz and dst.codes.device == cache.codes.device,
-             "mla_cache4_evict: out must have the cache's batch size and device.")
-    _require(1 <= budget <= dst.max_seq,
-             f"mla_cache4_evict: budget must be in [1, {dst.max_seq}].")
-    _require(0 <= recent <= budget, "mla_cache4_evict: recent must be in [0, budget].")
-    need = int(_lib.ds_mla_cache4_evict_workspace_size(cache.bsz, budget))
-    ws = _workspace(need, cache.codes.device)
-    with _on_device(cache.codes):
-        _check(_lib.ds_mla_cache4_evict(*_cache4_ptrs(cache), cache.bsz, cache.slots, budget,
-                                        recent, *_cache4_ptrs(dst), dst.slots, _ptr(ws), need,
-                                        _stream(cache.codes)), "mla_cache4_evict")
+    if not (dst.bsz == cache.bsz and dst.device == cache.device and 1 <= budget <= dst.max_seq
+            and 0 <= recent <= budget):
+        _require(dst.bsz == cache.bsz and dst.device == cache.device,
+                 "mla_cache4_evict: out must have the cache's batch size and device.")
+        _require(1 <= budget <= dst.max_seq,
+                 f"mla_cache4_evict: budget must be in [1, {dst.max_seq}].")
+        _require(False, "mla_cache4_evict: recent must be in [0, budget].")
+    need = _evict_workspace(cache.bsz, budget)
+    ws = torch.empty(need, dtype=_u8, device=cache.device)
+    with _on_device(ws):
+        _check(_lib.ds_mla_cache4_evict(*cache._ptrs, cache.bsz, cache.slots, budget, recent,
+                                        *dst._ptrs, dst.slots, ws.data_ptr(), need, _stream(ws)),
+               "mla_cache4_evict")
     dst._evicted(cache, budget)
     return dst
+
+
+@functools.lru_cache(maxsize=4096)
+def _evict_workspace(batch: int, budget: int) -> int:
+    return int(_lib.ds_mla_cache4_evict_workspace_size(batch, budget))
 
 
 def device_status() -> int:

@@ -183,14 +183,19 @@ class LatentKVCache4:
             raise ValueError(f"max_seq must be a positive integer, got {max_seq}")
         self.bsz, self.max_seq = bsz, max_seq
         self.slots = -(-max_seq // 64) * 64
-        dev = self.device = torch.device(device)
+        dev = torch.device(device)
         self.codes = torch.zeros((bsz, self.slots, 288), dtype=torch.uint8, device=dev)
+        dev = self.device = self.codes.device  # with its index
         self.scales = torch.zeros((bsz, 5, self.slots), dtype=torch.bfloat16, device=dev)
         self.rstd = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
         self.pos = torch.zeros((bsz, self.slots), dtype=torch.int32, device=dev)
         self.mass = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
-        self.state = torch.zeros((2, bsz), dtype=torch.int32, device=dev)
+        # lengths, next positions, and a row of counters that are zero between calls
+        self.state = torch.zeros((3, bsz), dtype=torch.int32, device=dev)
         self.lens, self.next_pos = self.state[0], self.state[1]
+        # the arrays never move: their addresses as the C entry points take them
+        self._ptrs = tuple(t.data_ptr() for t in (self.codes, self.scales, self.rstd, self.pos,
+                                                  self.mass, self.state))
         self._bound = 0      # no sequence is longer
         self._seen = 0       # no next position is larger
 
@@ -213,9 +218,7 @@ class LatentKVCache4:
     def bound_for_launch(self) -> int:
         """The bound that a launch is sized for: all slots inside a graph capture, because a
         replay sees later lengths."""
-        if self.codes.is_cuda and torch.cuda.is_current_stream_capturing():
-            return self.max_seq
-        return self._bound
+        return self.max_seq if torch.cuda.is_current_stream_capturing() else self._bound
 
     def reset(self) -> None:
         """Clear the cache for new sequences (keeps the memory)."""

@@ -500,8 +500,8 @@ DS_API int ds_int8_linear(const void* x_bf16, int64_t row_stride, const void* w_
  * src/kernels/mla_cache.py:29-219).  Arrays, with slots a multiple of 64: codes u8 [batch,
  * slots, 288] (512 latent then 64 rotated k_pe dimensions, two a byte, low half first, value =
  * (code - 8) * scale), scales bf16 [batch, 5, slots] (four groups of 128 latent dimensions,
- * then k_pe), rstd f32, pos i32 and mass f32 [batch, slots], state i32 [2, batch] (lengths in
- * slots, next positions).
+ * then k_pe), rstd f32, pos i32 and mass f32 [batch, slots], state i32 [3, batch] (lengths in
+ * slots, next positions, counters that are zero between calls).
  *
  * ds_mla_cache4_append: new_tokens tokens of every sequence (token i of sequence b at row
  *   b * src_rows_per_seq + i of latent / kpe; only the first new_lens[b] when given) quantised

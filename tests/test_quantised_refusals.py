@@ -106,7 +106,7 @@ def test_cache_construction_and_host_bounds():
             LatentKVCache4(1, bad, "cpu")
     c = LatentKVCache4(2, 100, "cpu")
     assert c.slots == 128 and c.codes.shape == (2, 128, 288) and c.scales.shape == (2, 5, 128)
-    assert c.memory_bytes == 2 * 128 * 310 + 16
+    assert c.memory_bytes == 2 * 128 * 310 + 24
     assert c.current_len == 0 and c.remaining_capacity == 100
     c._check_room(100, 100)
     with pytest.raises(RuntimeError, match="overflow"):
@@ -125,7 +125,7 @@ def test_cache_construction_and_host_bounds():
 
 def test_load_state_dict_checks_what_it_takes():
     c = LatentKVCache4(2, 64, "cpu")
-    c.state.copy_(torch.tensor([[3, 64], [5, 64]]))
+    c.state[:2].copy_(torch.tensor([[3, 64], [5, 64]]))
     sd = c.state_dict()
     d = LatentKVCache4(2, 200, "cpu")
     d.load_state_dict(sd)
