@@ -150,16 +150,30 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // loads of the first stages go out before the kernel waits for the quantised rows (programmatic
 // dependent launch behind quantize_kernel).
 constexpr int kFewThreads = 128;
+// QUANT: up to four rows of x, rows * K <= kQuantHere: every CTA takes the maxima of whole rows
+// itself and quantises its part of K straight into the operand's shared-memory layout; no first
+// kernel, whose launch costs more than reading x once per CTA (1 x 2048 x 9792: 7.7 us and a
+// launch on the host against one kernel).
+constexpr int kQuantHere = 16384;   // values of x
+constexpr int kQuantRows = 4;
+constexpr int kQuantBlocks = 16;    // k-blocks of a CTA (2 KB of operand each)
 template <int NT>
 struct FewTile {
   static constexpr int stages = NT <= 16 ? 6 : NT <= 32 ? 5 : NT <= 64 ? 4 : 3;  // two CTAs an SM
   static constexpr uint32_t stage = kTileBytes + NT * kBK;
   static constexpr uint32_t tmem_cols = NT < 32 ? 32 : NT;
   static constexpr size_t smem = 1024 + stages * stage + 256;
+  static constexpr int quant_stages = 5;
+  static constexpr size_t smem_quant(int k_blocks) {
+    return 1024 + quant_stages * kTileBytes + static_cast<size_t>(k_blocks) * NT * kBK + 256 + NT * 32;
+  }
   // [splits][ceil(NT / splits)][128] sums, splits <= 8
   static_assert((NT + 7) * 128 * 4 <= stages * stage, "the sums reuse the ring");
 };
 struct FewParams {
+  const uint4* x;  // QUANT: the rows, ld8 vectors apart
+  int64_t ld8;
+  int k8;
   const float* sa;
   const float* sw;
   __nv_bfloat16* out;
@@ -167,17 +181,20 @@ struct FewParams {
   int* status;
 };
 
-template <int NT>
+template <int NT, bool QUANT>
 __global__ void __launch_bounds__(kFewThreads)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                     const FewParams p) {
   using T = FewTile<NT>;
-  constexpr int kFewStages = T::stages;
+  constexpr int kFewStages = QUANT ? T::quant_stages : T::stages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
   const uint32_t s0 = ptx::smem_u32(smem);
-  uint8_t* tail = smem + kFewStages * T::stage;
+  // a stage's weights, then its rows of x; QUANT: all stages' weights, then all rows of x
+  constexpr uint32_t kStage = QUANT ? kTileBytes : T::stage;
+  uint8_t* tail = smem + kFewStages * kStage + (QUANT ? p.kb_per_split * NT * kBK : 0);
+  float* row_scale_s = reinterpret_cast<float*>(tail + 256);  // QUANT
   const uint32_t full0 = ptx::smem_u32(tail), empty0 = full0 + 8 * kFewStages;
   const uint32_t done = empty0 + 8 * kFewStages;
   uint32_t* holder = reinterpret_cast<uint32_t*>(tail + 8 * (2 * kFewStages + 1));
@@ -207,17 +224,68 @@ __global__ void __launch_bounds__(kFewThreads)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *holder;
-  if (warp == 0) {
-    if (lane == 0) {
-      ptx::prefetch_tmap(&tmX);
-      const int pre = min(nkb, kFewStages);
-      for (int i = 0; i < pre; ++i) {
-        ptx::mbar_arrive_expect_tx(full0 + 8 * i, T::stage);
-        ptx::tma_load_2d(s0 + i * T::stage, &tmW, full0 + 8 * i, (kb0 + i) * kBK, n0);
-      }
+  const int pre = min(nkb, kFewStages);
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < pre; ++i) {
+      ptx::mbar_arrive_expect_tx(full0 + 8 * i, kStage);
+      ptx::tma_load_2d(s0 + i * kStage, &tmW, full0 + 8 * i, (kb0 + i) * kBK, n0);
+    }
+    if (!QUANT) {
       ptx::pdl_wait();
       for (int i = 0; i < pre; ++i)
-        ptx::tma_load_2d(s0 + i * T::stage + kTileBytes, &tmX, full0 + 8 * i, (kb0 + i) * kBK, m0);
+        ptx::tma_load_2d(s0 + i * kStage + kTileBytes, &tmX, full0 + 8 * i, (kb0 + i) * kBK, m0);
+    }
+  }
+  __syncwarp();
+  if (QUANT) {
+    // the rows' maxima over all of K, then this CTA's part of them, 16 bytes of operand a thread
+    // and step, in the 128-byte swizzle; rows behind the last, and k behind K, are zeros
+    uint8_t* xs = smem + kFewStages * kStage;
+    uint32_t* part_max = reinterpret_cast<uint32_t*>(tail + 256 + NT * 16);  // [4][NT]
+    RowScale* scales = reinterpret_cast<RowScale*>(tail + 256 + NT * 4);     // [NT]
+    {
+      const int tpr = p.M == 1 ? kFewThreads : p.M == 2 ? 64 : 32;  // threads a row: whole warps
+      const int r = threadIdx.x / tpr;
+      uint32_t m2 = 0;
+      if (r < p.M) {
+        const uint4* src = p.x + static_cast<int64_t>(r) * p.ld8;
+#pragma unroll 8
+        for (int c = threadIdx.x % tpr; c < p.k8; c += tpr) m2 = abs_max8(__ldg(src + c), m2);
+      }
+      const uint32_t m = __reduce_max_sync(0xffffffffu, max(m2 & 0xFFFFu, m2 >> 16));
+      if (lane < kQuantRows) part_max[warp * NT + lane] = lane == r ? m : 0u;
+    }
+    __syncthreads();
+    if (threadIdx.x < p.M) {
+      const int r = threadIdx.x;
+      const uint32_t m = max(max(part_max[r], part_max[NT + r]),
+                             max(part_max[2 * NT + r], part_max[3 * NT + r]));
+      const bool finite = m < 0x7F80u;
+      const float a = __uint_as_float(m << 16);
+      row_scale_s[r] = finite ? a / 127.f : __uint_as_float(0x7FC00000u);
+      scales[r] = row_scale(a, finite);
+    }
+    __syncthreads();
+    const int per_row = nkb * 8;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < NT * per_row; i += kFewThreads) {
+      const int r = i / per_row, c = i - r * per_row;
+      const int k = kb0 * 16 + 2 * c;  // in vectors of 8 values
+      uint2 lo = make_uint2(0u, 0u), hi = lo;
+      if (r < p.M && k < p.k8) {  // (K is a multiple of 16: both vectors or none)
+        const uint4* src = p.x + static_cast<int64_t>(r) * p.ld8 + k;
+        const RowScale rs = scales[r];
+        lo = quant8(__ldg(src), rs);
+        hi = quant8(__ldg(src + 1), rs);
+      }
+      *reinterpret_cast<uint4*>(xs + (c >> 3) * (NT * kBK) + r * kBK + (((c & 7) ^ (r & 7)) << 4)) =
+          make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+    ptx::fence_async_shared();  // written by threads, read by the MMAs
+    __syncthreads();
+  }
+  if (warp == 0) {
+    if (lane == 0) {
       bool ok = true;
       int issued = pre;
       for (int i = pre; ok && i < nkb; ++i) {
@@ -225,9 +293,10 @@ __global__ void __launch_bounds__(kFewThreads)
         ok = ptx::mbar_wait(empty0 + 8 * st, (i / kFewStages - 1) & 1, abort_flag, p.status,
                             kTimeoutCycles, DS_ERR_TIMEOUT);
         if (!ok) break;
-        ptx::mbar_arrive_expect_tx(full0 + 8 * st, T::stage);
-        ptx::tma_load_2d(s0 + st * T::stage, &tmW, full0 + 8 * st, (kb0 + i) * kBK, n0);
-        ptx::tma_load_2d(s0 + st * T::stage + kTileBytes, &tmX, full0 + 8 * st, (kb0 + i) * kBK, m0);
+        ptx::mbar_arrive_expect_tx(full0 + 8 * st, kStage);
+        ptx::tma_load_2d(s0 + st * kStage, &tmW, full0 + 8 * st, (kb0 + i) * kBK, n0);
+        if (!QUANT)
+          ptx::tma_load_2d(s0 + st * kStage + kTileBytes, &tmX, full0 + 8 * st, (kb0 + i) * kBK, m0);
         issued = i + 1;
       }
       // every load has landed before this CTA goes on: the last fill of each stage
@@ -244,7 +313,8 @@ __global__ void __launch_bounds__(kFewThreads)
                             kTimeoutCycles, DS_ERR_TIMEOUT))
           break;
         ptx::tc_fence_after();
-        const uint32_t a = s0 + st * T::stage, b = a + kTileBytes;
+        const uint32_t a = s0 + st * kStage;
+        const uint32_t b = QUANT ? s0 + kFewStages * kStage + i * (NT * kBK) : a + kTileBytes;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           umma_i8(tmem, ptx::sw128_kmajor_desc(a + 32u * k), ptx::sw128_kmajor_desc(b + 32u * k),
@@ -296,7 +366,7 @@ __global__ void __launch_bounds__(kFewThreads)
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, T::tmem_cols);
   }
-  ptx::pdl_wait();  // the rows' scales
+  if (!QUANT) ptx::pdl_wait();  // the rows' scales
   if (!ok) return;
   // 16 threads a row, 8 channels each
   const int r0 = rank * per, rn = min(mrows, r0 + per) - r0;
@@ -306,7 +376,7 @@ __global__ void __launch_bounds__(kFewThreads)
 #pragma unroll
   for (int j = 0; j < 8; ++j) sw[j] = __ldg(p.sw + n + j);
   for (int r = threadIdx.x >> 4; r < rn; r += kFewThreads / 16) {
-    const float sa = __ldg(p.sa + m0 + r0 + r);
+    const float sa = QUANT ? row_scale_s[r0 + r] : __ldg(p.sa + m0 + r0 + r);
     const int4* src = reinterpret_cast<const int4*>(smem) + r * 32 + (threadIdx.x & 15) * 2;
     int4 x = src[0], y = src[1];
     for (int k = 1; k < p.splits; ++k) {
@@ -569,8 +639,13 @@ int g_pairs[64] = {};  // co-resident CTA pairs of the many-rows kernel
 
 template <int NT>
 int few_attr() {
-  DS_CUDA(cudaFuncSetAttribute(few_rows_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  DS_CUDA(cudaFuncSetAttribute(few_rows_kernel<NT, false>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(FewTile<NT>::smem)));
+  if (NT == 16)
+    DS_CUDA(cudaFuncSetAttribute(few_rows_kernel<16, true>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(FewTile<16>::smem_quant(kQuantBlocks))));
   return DS_OK;
 }
 
@@ -601,13 +676,28 @@ int set_attrs(const DeviceInfo& di) {
   return DS_OK;
 }
 
-template <int NT>
-int launch_few(const void* a, const float* sa, const void* w, const float* sw, void* out, int M,
-               int N, int K, const DeviceInfo& di, cudaStream_t s) {
+// K in parts: enough CTAs for the SMs to stream (up to 1.6 a SM; two fit), four k-blocks each at
+// least, clusters of at most 8.  None is empty.
+void few_splits(int tiles, int k_blocks, int num_sms, int* splits, int* per) {
+  int n = 1;
+  while (n < 8 && static_cast<int64_t>(tiles) * n * 10 <= num_sms * 8 && k_blocks >= 4 * n) n *= 2;
+  *per = (k_blocks + n - 1) / n;
+  *splits = (k_blocks + *per - 1) / *per;
+}
+
+// x: the rows to quantise (QUANT) or null; a, sa: the quantised rows.
+template <int NT, bool QUANT>
+int launch_few(const void* x, int64_t ld, const void* a, const float* sa, const void* w,
+               const float* sw, void* out, int M, int N, int K, const DeviceInfo& di,
+               cudaStream_t s) {
   CUtensorMap tmW, tmX;
   DS_TRY(tmap(&tmW, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, N, K, kBK, 128));
-  DS_TRY(tmap(&tmX, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M, K, kBK, NT));
+  if (QUANT) tmX = tmW;
+  else DS_TRY(tmap(&tmX, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M, K, kBK, NT));
   FewParams p{};
+  p.x = static_cast<const uint4*>(x);
+  p.ld8 = ld / 8;
+  p.k8 = K / 8;
   p.sa = sa;
   p.sw = sw;
   p.out = static_cast<__nv_bfloat16*>(out);
@@ -615,28 +705,24 @@ int launch_few(const void* a, const float* sa, const void* w, const float* sw, v
   p.N = N;
   p.k_blocks = (K + kBK - 1) / kBK;
   const int tiles = (N + 127) / 128, mt = (M + NT - 1) / NT;
-  int splits = 1;
-  while (splits < 8 && tiles * mt * splits * 10 <= di.num_sms * 8 && p.k_blocks >= 4 * splits)
-    splits *= 2;
-  p.kb_per_split = (p.k_blocks + splits - 1) / splits;
-  p.splits = (p.k_blocks + p.kb_per_split - 1) / p.kb_per_split;  // none is empty
+  few_splits(tiles * mt, p.k_blocks, di.num_sms, &p.splits, &p.kb_per_split);
   p.status = device_status_ptr();
   if (p.status == nullptr) return fail(DS_ERR_CUDA, "device status word unavailable");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = p.splits;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(tiles * p.splits, mt);
   cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = FewTile<NT>::smem;
+  cfg.dynamicSmemBytes = QUANT ? FewTile<NT>::smem_quant(p.kb_per_split) : FewTile<NT>::smem;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  DS_CUDA(cudaLaunchKernelEx(&cfg, few_rows_kernel<NT>, tmW, tmX, p));
+  cfg.numAttrs = QUANT ? 1 : 2;
+  DS_CUDA(cudaLaunchKernelEx(&cfg, few_rows_kernel<NT, QUANT>, tmW, tmX, p));
   return DS_OK;
 }
 
@@ -713,11 +799,11 @@ int launch_gemm(const void* a, const float* sa, const void* w, const float* sw, 
   DS_TRY(device_info(&di));
   DS_TRY(set_attrs(di));
   int st;
-  if (M <= 16) st = launch_few<16>(a, sa, w, sw, out, M, N, K, di, s);
-  else if (M <= 32) st = launch_few<32>(a, sa, w, sw, out, M, N, K, di, s);
-  else if (M <= 64) st = launch_few<64>(a, sa, w, sw, out, M, N, K, di, s);
+  if (M <= 16) st = launch_few<16, false>(nullptr, 0, a, sa, w, sw, out, M, N, K, di, s);
+  else if (M <= 32) st = launch_few<32, false>(nullptr, 0, a, sa, w, sw, out, M, N, K, di, s);
+  else if (M <= 64) st = launch_few<64, false>(nullptr, 0, a, sa, w, sw, out, M, N, K, di, s);
   else if (M <= 512 || g_pairs[di.device] < 1)
-    st = launch_few<128>(a, sa, w, sw, out, M, N, K, di, s);
+    st = launch_few<128, false>(nullptr, 0, a, sa, w, sw, out, M, N, K, di, s);
   else st = launch_many(a, sa, w, sw, out, M, N, K, di, s);
   DS_TRY(st);
   DS_LAUNCH_CHECK("int8 product");
@@ -734,6 +820,16 @@ int launch_linear(const void* x, int64_t ld, const void* w, const float* sw, voi
   int8_t* q = c.take<int8_t>(static_cast<size_t>(M) * K);
   float* sa = c.take<float>(static_cast<size_t>(M));
   if (!c.ok()) return fail(DS_ERR_WORKSPACE, "int8_linear: workspace needs %zu bytes", c.used);
+  if (M <= kQuantRows && M * K <= kQuantHere && N > 0) {
+    DeviceInfo di;
+    DS_TRY(device_info(&di));
+    DS_TRY(set_attrs(di));
+    int splits, per;
+    few_splits((N + 127) / 128, (K + kBK - 1) / kBK, di.num_sms, &splits, &per);
+    if (per <= kQuantBlocks)
+      return launch_few<16, true>(x, ld, nullptr, nullptr, w, sw, out, static_cast<int>(M), N, K,
+                                  di, s);
+  }
   DS_TRY(launch_quantize(x, ld, M, K, q, sa, s));
   return launch_gemm(q, sa, w, sw, out, M, N, K, s);
 }

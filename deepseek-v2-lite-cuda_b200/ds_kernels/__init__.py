@@ -812,7 +812,7 @@ def _rows_2d(x: torch.Tensor) -> torch.Tensor:
     copy only where the strides do not allow a view)."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     ld, inner = x2.stride()
-    if inner != 1 or ld % 8 or ld < x2.shape[1] or x2.data_ptr() % 16:
+    if inner != 1 or ld & 7 or ld < x2.shape[1] or x2.data_ptr() & 15:
         x2 = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device).copy_(x2)
     return x2
 
@@ -825,42 +825,42 @@ def int8_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
     (32 bits) and scaled once: bf16(acc * (scale_row * w_scale)).  K: a multiple of 16, at most
     131072; N: a multiple of 8.  `workspace` (uint8, at least int8_linear_workspace_size bytes)
     saves the allocation; calls that overlap need different ones."""
-    dev = x.device
-    if not (x.is_cuda and x.dtype is _bf16 and w_q.dtype is _i8 and w_scale.dtype is _f32
-            and w_q.dim() == 2 and w_q.is_contiguous() and w_scale.is_contiguous()
-            and w_scale.dim() == 1 and w_scale.shape[0] == w_q.shape[0] and w_q.device == dev
-            and w_scale.device == dev and x.dim() >= 1 and x.shape[-1] == w_q.shape[1]
-            and w_q.shape[1] > 0 and w_q.shape[1] % 16 == 0 and w_q.shape[0] % 8 == 0):
+    xs, ws, dev = x.shape, w_q.shape, x.get_device()
+    if not (dev >= 0 and x.dtype is _bf16 and w_q.dtype is _i8 and w_scale.dtype is _f32
+            and len(ws) == 2 and w_scale.shape == ws[:1] and w_q.is_contiguous()
+            and w_scale.is_contiguous() and w_q.get_device() == dev
+            and w_scale.get_device() == dev and xs[-1:] == ws[1:] and ws[1] % 16 == 0
+            and ws[1] > 0 and ws[0] % 8 == 0):
         _require(x.is_cuda and w_q.is_cuda and w_scale.is_cuda,
                  "int8_linear: x, w_q and w_scale must be CUDA tensors.")
         _require(x.dtype == _bf16, "int8_linear: x must be bfloat16.")
         _require(w_q.dtype == _i8 and w_q.dim() == 2 and w_q.is_contiguous(),
                  "int8_linear: w_q must be a contiguous int8 [N, K] tensor.")
-        _require(w_scale.dtype == _f32 and tuple(w_scale.shape) == (w_q.shape[0],)
+        _require(w_scale.dtype == _f32 and tuple(w_scale.shape) == (ws[0],)
                  and w_scale.is_contiguous(),
                  "int8_linear: w_scale must be a contiguous float32 [N] tensor.")
-        _require(w_q.device == dev and w_scale.device == dev,
+        _require(w_q.device == x.device and w_scale.device == x.device,
                  "int8_linear: x, w_q and w_scale must be on one device.")
-        _require(x.dim() >= 1 and x.shape[-1] == w_q.shape[1],
-                 f"int8_linear: x last dim must match w_q inner dim {w_q.shape[1]}.")
-        _require(w_q.shape[1] > 0 and w_q.shape[1] % 16 == 0,
+        _require(len(xs) >= 1 and xs[-1] == ws[1],
+                 f"int8_linear: x last dim must match w_q inner dim {ws[1]}.")
+        _require(ws[1] > 0 and ws[1] % 16 == 0,
                  "int8_linear: K must be a positive multiple of 16.")
         _require(False, "int8_linear: N must be a multiple of 8.")
-    N, K = w_q.shape
-    if x.dim() == 2:
-        out = torch.empty((x.shape[0], N), dtype=_bf16, device=dev)
-    else:
-        out = torch.empty((*x.shape[:-1], N), dtype=_bf16, device=dev)
+    N, K = ws
+    out = x.new_empty((*xs[:-1], N))
     if out.numel() == 0:
         return out
     x2 = _rows_2d(x)
     rows = x2.shape[0]
-    workspace = _scratch(workspace, int8_linear_workspace_size(rows, N, K), dev, "int8_linear")
+    need = int8_linear_workspace_size(rows, N, K)
+    if workspace is None or workspace.numel() < need:
+        workspace = w_q.new_empty(need)
+    else:
+        workspace = _scratch(workspace, need, x.device, "int8_linear")
     with _on_device(x):
         _check(_lib.ds_int8_linear(x2.data_ptr(), x2.stride(0), w_q.data_ptr(),
                                    w_scale.data_ptr(), out.data_ptr(), rows, N, K,
-                                   workspace.data_ptr(), workspace.numel(), _stream(x)),
-               "int8_linear")
+                                   workspace.data_ptr(), need, _stream(x)), "int8_linear")
     return out
 
 
@@ -948,8 +948,8 @@ def mla_cache4_get(cache, seq_len: Optional[int] = None) -> List[torch.Tensor]:
     n = cache.current_len if seq_len is None else int(seq_len)
     if not 0 <= n <= cache.slots:
         _require(False, f"mla_cache4_get: seq_len={n} outside the cache.")
-    lat = torch.empty((cache.bsz, n, 512), dtype=_bf16, device=cache.device)
-    kpe = torch.empty((cache.bsz, n, 64), dtype=_bf16, device=cache.device)
+    lat = cache.scales.new_empty((cache.bsz, n, 512))
+    kpe = cache.scales.new_empty((cache.bsz, n, 64))
     if n == 0:
         return [lat, kpe]
     with _on_device(lat):
@@ -997,13 +997,16 @@ def mla_decode_attention4(q: torch.Tensor, cache, softmax_scale: float,
         _require(False, "mla_decode_attention4: mass_decay must be in [0, 1].")
     B, heads, _ = q.shape
     if out is None:
-        out = torch.empty((B, heads * 512), dtype=_bf16, device=dev)
+        out = q.new_empty((B, heads * 512))
     else:
         _check_out(out, B, heads * 512, dev)
     max_len = cache.bound_for_launch
     with _on_device(q):
         need = _attention4_workspace(B, heads, cache.slots, max_len, acc, q.get_device())
-        workspace = _scratch(workspace, need, dev, "mla_decode_attention4")
+        if workspace is None or workspace.numel() < need:
+            workspace = cache.codes.new_empty(need)
+        else:
+            workspace = _scratch(workspace, need, dev, "mla_decode_attention4")
         codes, scales, rstd, _, mass, state = cache._ptrs
         _check(_lib.ds_mla_decode_attention4(
             q.data_ptr(), heads, codes, scales, rstd, mass, state, B, cache.slots, max_len,
@@ -1030,7 +1033,7 @@ def mla_cache4_evict(cache, budget: int, recent: int = 0, out=None):
                  f"mla_cache4_evict: budget must be in [1, {dst.max_seq}].")
         _require(False, "mla_cache4_evict: recent must be in [0, budget].")
     need = _evict_workspace(cache.bsz, budget)
-    ws = torch.empty(need, dtype=_u8, device=cache.device)
+    ws = cache.codes.new_empty(need)
     with _on_device(ws):
         _check(_lib.ds_mla_cache4_evict(*cache._ptrs, cache.bsz, cache.slots, budget, recent,
                                         *dst._ptrs, dst.slots, ws.data_ptr(), need, _stream(ws)),
