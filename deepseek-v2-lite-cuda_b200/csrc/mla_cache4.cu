@@ -262,11 +262,12 @@ __global__ void __launch_bounds__(256)
 // ---- attention ------------------------------------------------------------------------------
 // One query token per sequence over its slots, 16 heads (an MMA's M) at a time.
 //
-// Work is cut into units of (sequence, head tile, chunk of 128 slots), in that order, and CTA i
-// of G takes the units [i U / G, (i + 1) U / G): every CTA does the same number of chunks, whatever
-// the lengths, and none needs them on the host.  A CTA walks its range in segments of one
-// (sequence, head tile).  A segment that holds all its chunks writes the output; one that does not
-// (at most the first and the last of a CTA) leaves a partial, and merge_kernel joins those.
+// Work is cut into segments of one (sequence, head tile): up to `per` consecutive chunks of 128
+// slots, `per` the smallest number for which there are no more segments than CTAs (two an SM), so
+// whatever the lengths the CTAs are about equally long; every block works that out from the
+// lengths on the device.  A segment that is all of its sequence writes the output; the others
+// leave partials, which merge_kernel joins.  (Equal ranges of chunks that cross sequences balance
+// better still, but most CTAs then set up two segments: 64 x 2048 slots took 43 us.)
 //
 // Products run on mma.sync m16n8k16 (f16, f32 accumulators) with the 16 heads as M: tcgen05 would
 // take the heads as N = 16, where an instruction costs the same ~75 cycles as at N = 64 and the
@@ -291,23 +292,24 @@ __global__ void __launch_bounds__(256)
 // The running maximum of a head is raised, and O rescaled, only when it grows by more than 2^4.
 constexpr int kChunk = 128;
 constexpr int kAttnThreads = 128;
-constexpr int kMergeParts = 1024;  // CTAs of the attention kernel, at most
+constexpr int kStages = 2;       // chunks of codes in shared memory
+constexpr int kCtasPerSm = 2;
 constexpr int kPLd = 144;  // floats; 16 modulo 32: conflict-free 16-byte rows
 constexpr uint32_t kStageBytes = kChunk * kRowBytes;                 // 36,864
 constexpr uint32_t kQLd = 2 * kQCols * 2 + 64;  // two heads; 64 modulo 128: conflict-free
 constexpr uint32_t kQBytes = 8 * kQLd;                               // 18,944
 constexpr uint32_t kPBytes = 16 * kPLd * 4;                          // 9,216
 constexpr uint32_t kFacBytes = kGroups * kChunk * 4;                 // 2,560, twice
-constexpr uint32_t kOffQ = 2 * kStageBytes;
+constexpr uint32_t kOffQ = kStages * kStageBytes;
 constexpr uint32_t kOffP = kOffQ + kQBytes;
 constexpr uint32_t kOffFac = kOffP + kPBytes;
 constexpr uint32_t kOffSmall = kOffFac + 2 * kFacBytes;
 struct AttnSmall {  // behind the tiles
-  unsigned long long bar[2];
+  unsigned long long bar[kStages];
   float row[16];            // accumulator -> log2 of a weight
   float wmax[4][16];
   float wsum[4][16];
-  int scan[4];
+  alignas(16) int scan[16];
   int abort_flag;
   int never_flag;
 };
@@ -321,10 +323,12 @@ struct AttnParams {
   int heads, tiles;        // head tiles of 16
   int max_chunks;          // of any sequence, as the host knows it
   float scale_log2;
-  float* part_o;           // [G][2][16][512]
-  float* part_ml;          // [G][2][2][16]: maximum (log2), sum
-  float* lse;              // [batch, tiles * 16]: of the segments that held all their chunks
+  float* part_o;           // [segment][16][512]
+  float* part_ml;          // [segment][2][16]: maximum (log2), sum
+  int2* where;             // [batch, tiles]: a row's first segment, and how many
+  float* lse;              // [batch, tiles * 16]: of whole segments, then of all
   float* scores;           // [batch, tiles, max_chunks, 16, 128] (slots in fragment order) or null
+  int ctas;
   int* status;
 };
 
@@ -332,8 +336,6 @@ __device__ __forceinline__ int chunks_of(const Cache& c, int b, int max_chunks) 
   const int len = min(max(__ldg(c.state + b), 0), c.slots);
   return min((len + kChunk - 1) / kChunk, max_chunks);
 }
-// First unit of CTA i of n.
-__device__ __forceinline__ int64_t unit_start(int64_t units, int i, int n) { return units * i / n; }
 // Position of slot t (0..15) of a 16-slot group in fragment order, and back.
 __device__ __forceinline__ int frag_pos(int t) {
   const int m = (t >> 2) & 3;
@@ -411,18 +413,55 @@ __device__ __forceinline__ float4 lds_f4(uint32_t a) {
                      __uint_as_float(v.w));
 }
 
-// The sum of chunks over all sequences (times head tiles) and, for `unit` >= 0, the (sequence,
-// head tile, chunk) it is.  All threads of the block.
-__device__ __forceinline__ int64_t count_units(const AttnParams& p, int* scan) {
-  int64_t n = 0;
-  for (int b = threadIdx.x; b < p.c.batch; b += kAttnThreads) n += chunks_of(p.c, b, p.max_chunks);
-  int v = static_cast<int>(n);  // at most 65535 sequences of 2^26 / 128 chunks over 128 threads
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+// Sums of u and v over the block (kAttnThreads threads); `red`: 8 words that no earlier call in
+// flight uses (callers alternate between two).
+__device__ __forceinline__ int2 block_add(int u, int v, int* red) {
+  u = __reduce_add_sync(0xffffffffu, u);
+  v = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) {
+    red[threadIdx.x >> 5] = u;
+    red[4 + (threadIdx.x >> 5)] = v;
+  }
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) scan[threadIdx.x >> 5] = v;
-  __syncthreads();
-  return (static_cast<int64_t>(scan[0]) + scan[1] + scan[2] + scan[3]) * p.tiles;
+  const int4 x = *reinterpret_cast<const int4*>(red), y = *reinterpret_cast<const int4*>(red + 4);
+  return make_int2((x.x + x.y) + (x.z + x.w), (y.x + y.y) + (y.z + y.w));
+}
+// The segments' plan, the same in every block: chunks a segment, and the segments in all.
+// Segments are numbered sequence by sequence, head tile by head tile.  (Chunks fit 32 bits: one
+// is 36 KB of cache.)
+struct Plan {
+  int per, segments;
+};
+__device__ __forceinline__ Plan plan_segments(const AttnParams& p, int* red) {
+  // up to 128 sequences stay in registers, one a thread
+  const int mine = static_cast<int>(threadIdx.x) < p.c.batch ? chunks_of(p.c, threadIdx.x, p.max_chunks) : 0;
+  int n = mine, some = mine > 0 ? 1 : 0;
+  for (int b = threadIdx.x + kAttnThreads; b < p.c.batch; b += kAttnThreads) {
+    const int k = chunks_of(p.c, b, p.max_chunks);
+    n += k;
+    some += k > 0 ? 1 : 0;
+  }
+  const int2 sum = block_add(n, some, red);
+  const int total = sum.x * p.tiles, rows = sum.y * p.tiles;  // rows: not empty
+  Plan w;
+  if (rows >= p.ctas) {  // a segment each
+    w.per = p.max_chunks;
+    w.segments = rows;
+    return w;
+  }
+  // a row of n chunks has at most n / per + 1 segments, so total / (ctas - rows) chunks fit
+  int lo = max(1, (total + p.ctas - 1) / p.ctas);
+  int hi = max(lo, min(p.max_chunks, (total + p.ctas - rows - 1) / (p.ctas - rows)));
+  for (int turn = 1;; ++turn) {
+    w.per = (lo + hi) >> 1;
+    n = (mine + w.per - 1) / w.per;
+    for (int b = threadIdx.x + kAttnThreads; b < p.c.batch; b += kAttnThreads)
+      n += (chunks_of(p.c, b, p.max_chunks) + w.per - 1) / w.per;
+    w.segments = block_add(n, 0, red + 8 * (turn & 1)).x * p.tiles;
+    if (lo == hi) return w;
+    if (w.segments <= p.ctas) hi = w.per;
+    else lo = w.per + 1;
+  }
 }
 
 // The scales of slot t0 + threadIdx.x as they multiply the accumulators: scale * rstd for the
@@ -449,7 +488,7 @@ __device__ __forceinline__ void store_factors(float* fac, const Factors& f) {
   fac[4 * kChunk + pos] = __uint_as_float(f.s[4] << 16);
 }
 
-__global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const Cache& c = p.c;
   AttnSmall& sm = *reinterpret_cast<AttnSmall*>(smem + kOffSmall);
@@ -465,45 +504,40 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnPara
     sm.never_flag = 0;
     ptx::fence_barrier_init();
   }
-  const int64_t units = count_units(p, sm.scan);
-  int64_t u = unit_start(units, blockIdx.x, gridDim.x);
-  const int64_t u_end = unit_start(units, blockIdx.x + 1, gridDim.x);
-  if (u >= u_end) return;
-  // the sequence of unit u (a serial walk in blocks of 32 sequences, all warps alike)
-  int b = 0;
-  int64_t before = 0;  // units of the sequences before b
-  for (int base = 0;; base += 32) {
-    int n = base + lane < c.batch ? chunks_of(c, base + lane, p.max_chunks) : 0;
-    int incl = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += y;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + static_cast<int64_t>(incl) * p.tiles > u);
-    if (hit != 0u) {
-      const int l = __ffs(hit) - 1;
-      b = base + l;
-      before += static_cast<int64_t>(__shfl_sync(0xffffffffu, incl - n, l)) * p.tiles;
-      break;
-    }
-    before += static_cast<int64_t>(__shfl_sync(0xffffffffu, incl, 31)) * p.tiles;
-    if (base + 32 >= c.batch) return;  // not reached: u < units
-  }
+  ptx::pdl_launch_dependents();
+  const Plan plan = plan_segments(p, sm.scan);
   const Masks km = masks();
   uint32_t it = 0;  // chunks taken so far: stage it & 1, phase (it >> 1) & 1
-  bool first = true;
-  while (u < u_end) {
-    const int nch = chunks_of(c, b, p.max_chunks);
-    if (before + static_cast<int64_t>(nch) * p.tiles <= u) {  // on to the next sequence
-      before += static_cast<int64_t>(nch) * p.tiles;
-      ++b;
-      continue;
+  for (int index = blockIdx.x; index < plan.segments; index += gridDim.x) {
+    // the sequence of segment `index`: 32 sequences at a time, every warp alike
+    int b = 0, before = 0;
+    for (int base = 0;; base += 32) {
+      const int n = base + lane < c.batch
+                        ? (chunks_of(c, base + lane, p.max_chunks) + plan.per - 1) / plan.per * p.tiles
+                        : 0;
+      int incl = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > index);
+      if (hit != 0u) {
+        const int l = __ffs(hit) - 1;
+        b = base + l;
+        before += __shfl_sync(0xffffffffu, incl - n, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+      if (base + 32 >= c.batch) return;  // not reached: index < segments
     }
-    const int tile = static_cast<int>((u - before) / nch);
-    const int c0 = static_cast<int>((u - before) - static_cast<int64_t>(tile) * nch);
-    const int seg = static_cast<int>(min(static_cast<int64_t>(nch - c0), u_end - u));
-    const bool whole = c0 == 0 && seg == nch;
+    const int nch = chunks_of(c, b, p.max_chunks);
+    const int nseg = (nch + plan.per - 1) / plan.per;
+    const int tile = (index - before) / nseg;
+    const int c0 = (index - before - tile * nseg) * plan.per;
+    const int seg = min(plan.per, nch - c0);
+    const bool whole = nseg == 1;
+    if (c0 == 0 && threadIdx.x == 0) p.where[b * p.tiles + tile] = make_int2(index, nseg);
     const int len = min(__ldg(c.state + b), c.slots);
     const int nh = min(16, p.heads - tile * 16);
     const uint8_t* codes = c.codes + static_cast<int64_t>(b) * c.slots * kRowBytes;
@@ -525,36 +559,41 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnPara
     // Q as f16 fragments: warp w makes the heads r and r + 8 of rows r = 2w, 2w + 1, whose words
     // lie side by side as an MMA takes them.  Lane l holds dimensions 16 l .. (and 2 of q_pe);
     // k-step s of a quad of 64 dimensions takes pairs j = 2 (s & 1), + 1 of word s / 2.
-#pragma unroll 1
+    uint32_t qw[4][9];  // heads 2w, 2w + 8, 2w + 1, 2w + 9: all on their way before the first is used
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = warp * 2 + (i >> 1) + 8 * (i & 1);
+      const __nv_bfloat16* q =
+          p.q + (static_cast<int64_t>(b) * p.heads + tile * 16 + (h < nh ? h : 0)) * kQCols;
+      const uint4 x0 = __ldg(reinterpret_cast<const uint4*>(q) + 2 * lane);
+      const uint4 x1 = __ldg(reinterpret_cast<const uint4*>(q) + 2 * lane + 1);
+      qw[i][0] = x0.x, qw[i][1] = x0.y, qw[i][2] = x0.z, qw[i][3] = x0.w;
+      qw[i][4] = x1.x, qw[i][5] = x1.y, qw[i][6] = x1.z, qw[i][7] = x1.w;
+      qw[i][8] = __ldg(reinterpret_cast<const uint32_t*>(q + kLatent) + lane);
+    }
+#pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = warp * 2 + i;
       uint32_t f[2][8], fr[2][2];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         const int h = r + 8 * hh;
-        const __nv_bfloat16* q =
-            p.q + (static_cast<int64_t>(b) * p.heads + tile * 16 + (h < nh ? h : 0)) * kQCols;
-        const uint4 x0 = __ldg(reinterpret_cast<const uint4*>(q) + 2 * lane);
-        const uint4 x1 = __ldg(reinterpret_cast<const uint4*>(q) + 2 * lane + 1);
-        const uint32_t x2 = __ldg(reinterpret_cast<const uint32_t*>(q + kLatent) + lane);
-        const uint32_t w[9] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w, x2};
-        float v[18];
-        float amax = 0.f;
+        const uint32_t(&w)[9] = qw[2 * i + hh];
+        // the largest magnitude, as a bf16's bits (infinities and NaN order above)
+        uint32_t m2 = 0;
 #pragma unroll
-        for (int j = 0; j < 9; ++j) {
-          v[2 * j] = __uint_as_float(w[j] << 16);
-          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-          amax = fmaxf(amax, fmaxf(fabsf(v[2 * j]), fabsf(v[2 * j + 1])));
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-        // largest magnitude into [2^14, 2^15), by two factors: their product may pass 2^127
-        int e = 0;
-        if (amax > 0.f && amax <= 3.4e38f) e = 14 - ilogbf(amax);
+        for (int j = 0; j < 9; ++j) m2 = __vmaxu2(m2, w[j] & 0x7FFF7FFFu);
+        const uint32_t m = __reduce_max_sync(0xffffffffu, max(m2 & 0xFFFFu, m2 >> 16));
+        // its exponent to 2^14, by two factors: their product may pass 2^127
+        const int e = m == 0 || m >= 0x7F80u ? 0 : 14 + 127 - max(static_cast<int>(m >> 7), 1);
         const float fa = __int_as_float((127 + e / 2) << 23);
         const float fb = h < nh ? __int_as_float((127 + e - e / 2) << 23) : 0.f;
+        float v[18];
 #pragma unroll
-        for (int n = 0; n < 18; ++n) v[n] = v[n] * fa * fb;
+        for (int j = 0; j < 9; ++j) {
+          v[2 * j] = __uint_as_float(w[j] << 16) * fa * fb;
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u) * fa * fb;
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int n = (j & 3) + 8 * (j >> 2);
@@ -563,7 +602,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnPara
         // q_pe dimensions 2 l and 2 l + 1; their partners are two lanes up
         fr[hh][0] = pack_f16(v[16], __shfl_down_sync(0xffffffffu, v[16], 2));
         fr[hh][1] = pack_f16(v[17], __shfl_down_sync(0xffffffffu, v[17], 2));
-        if (lane == 0) sm.row[h] = ldexpf(p.scale_log2, -e);
+        if (lane == 0)
+          sm.row[h] = p.scale_log2 * __int_as_float((127 - e / 2) << 23) *
+                      __int_as_float((127 - (e - e / 2)) << 23);
       }
       uint8_t* row = smem + kOffQ + r * kQLd;
 #pragma unroll
@@ -813,7 +854,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnPara
     l0 = (sm.wsum[0][g] + sm.wsum[1][g]) + (sm.wsum[2][g] + sm.wsum[3][g]);
     l1 = (sm.wsum[0][g + 8] + sm.wsum[1][g + 8]) + (sm.wsum[2][g + 8] + sm.wsum[3][g + 8]);
     const float unit = 1.f / pscale;
-    const int slot = blockIdx.x * 2 + (first ? 0 : 1);
     float f0 = unit, f1 = unit;
     if (whole) {
       f0 = l0 == 0.f ? 0.f : unit / l0;
@@ -827,7 +867,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnPara
           lse[g + 8] = m1 + log2f(l1);
         }
       } else {
-        float* ml = p.part_ml + static_cast<int64_t>(slot) * 32;
+        float* ml = p.part_ml + static_cast<int64_t>(index) * 32;
         ml[g] = m0;
         ml[g + 8] = m1;
         ml[16 + g] = l0;
@@ -858,7 +898,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnPara
             *reinterpret_cast<uint4*>(dst + j) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
-          float* dst = p.part_o + (static_cast<int64_t>(slot) * 16 + h) * kLatent + d;
+          float* dst = p.part_o + (static_cast<int64_t>(index) * 16 + h) * kLatent + d;
 #pragma unroll
           for (int j = 0; j < 16; j += 4)
             *reinterpret_cast<float4*>(dst + j) =
@@ -867,123 +907,69 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attend4_kernel(const AttnPara
         }
       }
     }
-    u += seg;
-    first = false;
   }
 }
 
-// The CTAs that hold the units of (sequence b, head tile): first and last, and the unit range.
-struct Owners {
-  int64_t units, u0, u1;
-  int first, last;
-};
-__device__ __forceinline__ Owners owners_of(const AttnParams& p, int b, int tile, int ctas,
-                                            int* scan) {
-  int64_t mine = 0;
-  int n = 0;
-  for (int x = threadIdx.x; x < p.c.batch; x += kAttnThreads) {
-    const int k = chunks_of(p.c, x, p.max_chunks);
-    mine += k;
-    if (x < b) n += k;
-  }
-  int v = static_cast<int>(mine);
+// Joins the partials of a (sequence, head tile): four blocks each, four heads a block, a warp a
+// head; lse (log2 of the weights' sum) where it is wanted; zeros for a sequence without slots.
+__global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.y, tile = blockIdx.x >> 2, r = (blockIdx.x & 3) * 4 + warp;
+  const int h = tile * 16 + r;
+  if (h >= p.heads) return;
+  const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
+  ptx::pdl_wait();
+  const int2 w = empty ? make_int2(0, 0) : __ldcg(p.where + b * p.tiles + tile);
+  if (w.y == 1) return;  // written by the attention kernel
+  __nv_bfloat16* o = p.out + (static_cast<int64_t>(b) * p.heads + h) * kLatent;
+  const float* ml = p.part_ml + static_cast<int64_t>(w.x) * 32 + r;
+  const float4* po = reinterpret_cast<const float4*>(
+                         p.part_o + (static_cast<int64_t>(w.x) * 16 + r) * kLatent) + lane;
+  float M = -INFINITY, L = 0.f;
+  float a[16];  // dimensions 4 lane + 128 k ..
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    v += __shfl_xor_sync(0xffffffffu, v, d);
-    n += __shfl_xor_sync(0xffffffffu, n, d);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    scan[threadIdx.x >> 5] = v;
-    scan[4 + (threadIdx.x >> 5)] = n;
-  }
-  __syncthreads();
-  Owners w;
-  w.units = (static_cast<int64_t>(scan[0]) + scan[1] + scan[2] + scan[3]) * p.tiles;
-  const int64_t before =
-      (static_cast<int64_t>(scan[4]) + scan[5] + scan[6] + scan[7]) * p.tiles;
-  const int nch = chunks_of(p.c, b, p.max_chunks);
-  w.u0 = before + static_cast<int64_t>(tile) * nch;
-  w.u1 = w.u0 + nch;
-  w.first = w.last = 0;
-  if (nch > 0) {
-    // CTA of unit u: the largest i with floor(units i / ctas) <= u
-    w.first = static_cast<int>(((w.u0 + 1) * ctas - 1) / w.units);
-    w.last = static_cast<int>((w.u1 * ctas - 1) / w.units);
-  }
-  return w;
-}
-// The partial of CTA i that belongs to units [u0, ..): its first segment if it starts inside.
-// -1: a CTA without units (fewer units than CTAs).
-__device__ __forceinline__ int part_slot(const Owners& w, int i, int ctas) {
-  const int64_t u = unit_start(w.units, i, ctas);
-  if (u == unit_start(w.units, i + 1, ctas)) return -1;
-  return 2 * i + (u >= w.u0 ? 0 : 1);
-}
-
-// Joins the partials of one (sequence, head) a block: output, and lse (log2 of the weights' sum)
-// where it is wanted; zeros for a sequence without slots.
-__global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p, int ctas) {
-  __shared__ int scan[8];
-  __shared__ float sw[kMergeParts], sred[8];
-  __shared__ int sslot[kMergeParts];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = static_cast<int>(blockIdx.x) / p.heads;
-  const int h = static_cast<int>(blockIdx.x) - b * p.heads;
-  const int r = h & 15;
-  const Owners w = owners_of(p, b, h >> 4, ctas, scan);
-  __nv_bfloat16* o = p.out + static_cast<int64_t>(blockIdx.x) * kLatent;
-  if (w.u1 == w.u0) {
-    reinterpret_cast<uint2*>(o)[tid] = make_uint2(0u, 0u);
-    return;
-  }
-  if (w.first == w.last) return;  // written by the attention kernel
-  const int n = w.last - w.first + 1;  // at most kMergeParts: the grid's CTAs
-  float M = -INFINITY;
-  for (int i = tid; i < n; i += kAttnThreads) {
-    const int s = part_slot(w, w.first + i, ctas);
-    sslot[i] = s;
-    const float m = s >= 0 ? __ldg(p.part_ml + static_cast<int64_t>(s) * 32 + r) : -INFINITY;
-    sw[i] = m;
-    M = fmaxf(M, m);
-  }
+  for (int k = 0; k < 16; ++k) a[k] = 0.f;
+  for (int i0 = 0; i0 < w.y; i0 += 32) {  // 32 partials at a time: lane i has the i-th's weight
+    const bool in = i0 + lane < w.y;
+    const float m = in ? __ldcg(ml + (i0 + lane) * 32) : -INFINITY;
+    float l = in ? __ldcg(ml + (i0 + lane) * 32 + 16) : 0.f;
+    float mx = fmaxf(m, M);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-  if (lane == 0) sred[warp] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(sred[0], sred[1]), fmaxf(sred[2], sred[3]));
-  const float ref = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  for (int i = tid; i < n; i += kAttnThreads) {
-    const int s = sslot[i];
-    const float f = s >= 0 ? ptx::ex2(sw[i] - ref) : 0.f;
-    sw[i] = f;
-    if (s >= 0) L = fmaf(f, __ldg(p.part_ml + static_cast<int64_t>(s) * 32 + 16 + r), L);
-  }
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    const float keep = ptx::ex2(M - ref);
+    const float f = in ? ptx::ex2(m - ref) : 0.f;
+    l *= f;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
-  if (lane == 0) sred[4 + warp] = L;
-  __syncthreads();
-  L = (sred[4] + sred[5]) + (sred[6] + sred[7]);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    L = fmaf(L, keep, l);
+    M = mx;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) a[k] *= keep;
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const int s = sslot[i];
-    if (s < 0) continue;
-    const float f = sw[i];
-    const float4 v = __ldg(
-        reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(s) * 16 + r) * kLatent) + tid);
-    a.x = fmaf(f, v.x, a.x);
-    a.y = fmaf(f, v.y, a.y);
-    a.z = fmaf(f, v.z, a.z);
-    a.w = fmaf(f, v.w, a.w);
+    for (int i = 0; i < min(32, w.y - i0); ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      const float4* src = po + static_cast<int64_t>(i0 + i) * (16 * kLatent / 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 v = __ldcg(src + 32 * k);
+        a[4 * k] = fmaf(fi, v.x, a[4 * k]);
+        a[4 * k + 1] = fmaf(fi, v.y, a[4 * k + 1]);
+        a[4 * k + 2] = fmaf(fi, v.z, a[4 * k + 2]);
+        a[4 * k + 3] = fmaf(fi, v.w, a[4 * k + 3]);
+      }
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv);
-  const __nv_bfloat162 y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
-  reinterpret_cast<uint2*>(o)[tid] = make_uint2(*reinterpret_cast<const uint32_t*>(&x),
-                                                *reinterpret_cast<const uint32_t*>(&y));
-  if (p.lse != nullptr && tid == 0)
-    p.lse[(static_cast<int64_t>(b) * p.tiles + (h >> 4)) * 16 + r] = M + log2f(L);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a[4 * k] * inv, a[4 * k + 1] * inv);
+    const __nv_bfloat162 y = __floats2bfloat162_rn(a[4 * k + 2] * inv, a[4 * k + 3] * inv);
+    reinterpret_cast<uint2*>(o)[lane + 32 * k] =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  }
+  if (p.lse != nullptr && lane == 0)
+    p.lse[(static_cast<int64_t>(b) * p.tiles + tile) * 16 + r] = M + log2f(L);
 }
 
 // mass[t] = decay mass[t] + sum_h 2^(s_h(t) - lse_h); one chunk of one sequence a block.
@@ -1386,23 +1372,27 @@ int check_cache(const Cache& c, const char* op) {
 }
 
 struct AttnBuffers {
+  int2* where;
   float* part_o;
   float* part_ml;
   float* scores;
   float* lse;
 };
 
-// CTAs of the attention kernel: two per SM, no more than there can be chunks.
+// CTAs of the attention kernel: as many as run at once, no more than there can be chunks.
 int attn_ctas(int batch, int tiles, int max_chunks, int num_sms) {
   const int64_t units = static_cast<int64_t>(batch) * tiles * max_chunks;
-  const int most = std::min(2 * num_sms, kMergeParts);
+  const int most = kCtasPerSm * num_sms;
   return static_cast<int>(units < most ? (units < 1 ? 1 : units) : most);
 }
 
 void carve_attn(Carve& w, AttnBuffers* b, int batch, int heads, int max_len, int num_sms,
                 bool mass) {
   const int tiles = (heads + 15) / 16, chunks = (max_len + kChunk - 1) / kChunk;
-  const size_t parts = 2 * static_cast<size_t>(attn_ctas(batch, tiles, chunks, num_sms));
+  // a partial segment shares its (sequence, head tile) with another one, so there are no more
+  // than CTAs; with more sequences than CTAs every segment is whole, and numbered further
+  const size_t parts = std::max<size_t>(attn_ctas(batch, tiles, chunks, num_sms), 1);
+  b->where = w.take<int2>(static_cast<size_t>(batch) * tiles);
   b->part_o = w.take<float>(parts * 16 * kLatent);
   b->part_ml = w.take<float>(parts * 32);
   b->lse = mass ? w.take<float>(static_cast<size_t>(batch) * tiles * 16) : nullptr;
@@ -1478,6 +1468,7 @@ int launch_attention(const Cache& c, const void* q, int heads, int max_len, floa
   carve_attn(w, &b, c.batch, heads, max_len, di.num_sms, accumulate != 0);
   if (!w.ok())
     return fail(DS_ERR_WORKSPACE, "mla_decode_attention4: workspace needs %zu bytes", w.used);
+  p.where = b.where;
   p.part_o = b.part_o;
   p.part_ml = b.part_ml;
   p.scores = b.scores;
@@ -1492,12 +1483,21 @@ int launch_attention(const Cache& c, const void* q, int heads, int max_len, floa
       g_attr_set[di.device] = true;
     }
   }
-  const int ctas = attn_ctas(c.batch, p.tiles, p.max_chunks, di.num_sms);
+  p.ctas = attn_ctas(c.batch, p.tiles, p.max_chunks, di.num_sms);
   if (max_len > 0) {
-    attend4_kernel<<<ctas, kAttnThreads, kAttnSmem, s>>>(p);
+    attend4_kernel<<<p.ctas, kAttnThreads, kAttnSmem, s>>>(p);
     DS_LAUNCH_CHECK("attend4_kernel");
   }
-  merge_kernel<<<c.batch * heads, kAttnThreads, 0, s>>>(p, ctas);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(p.tiles * 4, c.batch);
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = max_len > 0 ? 1 : 0;
+  DS_CUDA(cudaLaunchKernelEx(&cfg, merge_kernel, p));
   DS_LAUNCH_CHECK("merge_kernel");
   if (accumulate && max_len > 0) {
     mass_kernel<<<dim3(p.max_chunks, c.batch), kChunk, 0, s>>>(p, decay);
