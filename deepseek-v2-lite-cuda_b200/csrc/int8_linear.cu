@@ -810,16 +810,18 @@ int launch_gemm(const void* a, const float* sa, const void* w, const float* sw, 
   return DS_OK;
 }
 
+// Rows that the product's kernel quantises itself, whatever the number of splits.
+bool quantized_inside(int64_t M, int K) {
+  return M <= kQuantRows && M * K <= kQuantHere && K <= kQuantBlocks * kBK;
+}
+
 size_t linear_workspace(int64_t M, int K) {
+  if (quantized_inside(M, K)) return 0;
   return align_up(static_cast<size_t>(M) * K, 256) + align_up(static_cast<size_t>(M) * 4, 256);
 }
 
 int launch_linear(const void* x, int64_t ld, const void* w, const float* sw, void* out, int64_t M,
                   int N, int K, void* workspace, size_t ws_bytes, cudaStream_t s) {
-  Carve c(workspace, ws_bytes);
-  int8_t* q = c.take<int8_t>(static_cast<size_t>(M) * K);
-  float* sa = c.take<float>(static_cast<size_t>(M));
-  if (!c.ok()) return fail(DS_ERR_WORKSPACE, "int8_linear: workspace needs %zu bytes", c.used);
   if (M <= kQuantRows && M * K <= kQuantHere && N > 0) {
     DeviceInfo di;
     DS_TRY(device_info(&di));
@@ -830,6 +832,10 @@ int launch_linear(const void* x, int64_t ld, const void* w, const float* sw, voi
       return launch_few<16, true>(x, ld, nullptr, nullptr, w, sw, out, static_cast<int>(M), N, K,
                                   di, s);
   }
+  Carve c(workspace, ws_bytes);
+  int8_t* q = c.take<int8_t>(static_cast<size_t>(M) * K);
+  float* sa = c.take<float>(static_cast<size_t>(M));
+  if (!c.ok()) return fail(DS_ERR_WORKSPACE, "int8_linear: workspace needs %zu bytes", c.used);
   DS_TRY(launch_quantize(x, ld, M, K, q, sa, s));
   return launch_gemm(q, sa, w, sw, out, M, N, K, s);
 }
@@ -862,7 +868,9 @@ int ds_int8_linear(const void* x_bf16, int64_t row_stride, const void* w_int8,
                    int in_features, void* workspace, size_t workspace_bytes, void* stream) {
   DS_TRY(ds::i8::check_shape(rows, out_features, in_features));
   if (rows == 0 || out_features == 0) return DS_OK;
-  DS_REQUIRE(x_bf16 && w_int8 && w_scale && out_bf16 && workspace, "int8_linear: null pointer");
+  DS_REQUIRE(x_bf16 && w_int8 && w_scale && out_bf16 &&
+                 (workspace || ds::i8::linear_workspace(rows, in_features) == 0),
+             "int8_linear: null pointer");
   DS_REQUIRE(row_stride >= in_features && row_stride % 8 == 0 && ds::aligned16(x_bf16) &&
                  ds::aligned16(w_int8) && ds::aligned16(out_bf16) && ds::aligned16(workspace),
              "int8_linear: x rows, w, out and workspace must be 16-byte aligned");

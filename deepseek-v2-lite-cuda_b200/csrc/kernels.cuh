@@ -60,6 +60,16 @@ int launch_combine_gather(const void* eo, const int32_t* slot_of, const float* w
 
 int launch_swiglu(const void* in, void* out, int64_t rows, int I, cudaStream_t s);
 
+namespace i8 {
+
+// out bf16 [M, N] = rows of x (bf16, `ld` elements apart) quantised per row, times int8 w [N, K]^T,
+// scaled by row and channel; workspace of linear_workspace(M, K) bytes.
+size_t linear_workspace(int64_t M, int K);
+int launch_linear(const void* x, int64_t ld, const void* w, const float* sw, void* out, int64_t M,
+                  int N, int K, void* workspace, size_t ws_bytes, cudaStream_t s);
+
+}  // namespace i8
+
 namespace gemm {
 
 // kPartial is internal: a split-K launch of a kPlain / kSwiGLU problem writes raw f32 partial

@@ -209,6 +209,47 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+// What a decode step does between its projection and the attention, a block a sequence: warp 0
+// appends the new token (latent and k_pe of the projection's row) and moves the length on, the
+// others copy the heads' absorbed queries and rotate their q_pe at the token's position.
+__global__ void __launch_bounds__(288)
+    decode4_prepare_kernel(Cache c, const __nv_bfloat16* __restrict__ proj, int ld, int heads,
+                           const __nv_bfloat16* __restrict__ cos_t,
+                           const __nv_bfloat16* __restrict__ sin_t, int table_rows, float eps,
+                           __nv_bfloat16* __restrict__ q) {
+  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const __nv_bfloat16* row = proj + static_cast<int64_t>(b) * ld;
+  const int len = c.state[b], next = c.state[c.batch + b];
+  if (warp == 0) {
+    const __nv_bfloat16* lat = row + heads * kQCols;
+    const Token tok = load_token(lat, lat + kLatent);
+    if (len >= 0 && len < c.slots)
+      put_token(c, b, len, next, tok, cos_t, sin_t, table_rows, eps);
+  } else {
+    const int prow = min(next, table_rows - 1);
+    const __nv_bfloat16* cr = cos_t + static_cast<int64_t>(prow) * kRope;
+    const __nv_bfloat16* sr = sin_t + static_cast<int64_t>(prow) * kRope;
+    for (int h = warp - 1; h < heads; h += 8) {
+      __nv_bfloat16* dst = q + (static_cast<int64_t>(b) * heads + h) * kQCols;
+      const uint4* s4 = reinterpret_cast<const uint4*>(row + h * kLatent) + 2 * lane;
+      reinterpret_cast<uint4*>(dst)[2 * lane] = s4[0];
+      reinterpret_cast<uint4*>(dst)[2 * lane + 1] = s4[1];
+      const __nv_bfloat162 x =
+          reinterpret_cast<const __nv_bfloat162*>(row + heads * kLatent + h * kRope)[lane];
+      const float xa = __low2float(x), xb = __high2float(x);
+      dst[kLatent + lane] = __float2bfloat16_rn(xa * __bfloat162float(cr[lane]) -
+                                                xb * __bfloat162float(sr[lane]));
+      dst[kLatent + 32 + lane] = __float2bfloat16_rn(xb * __bfloat162float(cr[32 + lane]) +
+                                                     xa * __bfloat162float(sr[32 + lane]));
+    }
+  }
+  __syncthreads();  // every warp has read the position
+  if (threadIdx.x == 0 && len < c.slots) {
+    c.state[b] = len + 1;
+    c.state[c.batch + b] = next + 1;
+  }
+}
+
 // Eight codes of one word -> eight bf16 values (code - 8) * scale, rounded once: 128 + code is a
 // bf16 pair under a mask, 136 off it is exact, and the product rounds.
 __device__ __forceinline__ uint4 values8(uint32_t w, uint32_t scale2) {
@@ -916,8 +957,9 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.y, tile = blockIdx.x >> 2, r = (blockIdx.x & 3) * 4 + warp;
   const int h = tile * 16 + r;
-  if (h >= p.heads) return;
+  if (h >= p.heads) return;  // (a block has a head: its first warp's)
   const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
+  ptx::pdl_launch_dependents();
   ptx::pdl_wait();
   const int2 w = empty ? make_int2(0, 0) : __ldcg(p.where + b * p.tiles + tile);
   if (w.y == 1) return;  // written by the attention kernel
@@ -978,7 +1020,8 @@ __global__ void __launch_bounds__(kChunk) mass_kernel(const AttnParams p, float 
   const int tid = threadIdx.x, b = blockIdx.y, chunk = blockIdx.x;
   const int len = min(__ldg(p.c.state + b), p.c.slots);
   if (chunk * kChunk >= len) return;
-  if (tid < p.heads) slse[tid] = p.lse[static_cast<int64_t>(b) * p.tiles * 16 + tid];
+  ptx::pdl_wait();
+  if (tid < p.heads) slse[tid] = __ldcg(p.lse + static_cast<int64_t>(b) * p.tiles * 16 + tid);
   __syncthreads();
   const int t = chunk * kChunk + frag_slot(tid);
   float a = 0.f;
@@ -988,12 +1031,12 @@ __global__ void __launch_bounds__(kChunk) mass_kernel(const AttnParams p, float 
     if (p.heads >= 16 * tile + 16) {
       float v[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = __ldg(s + r * kChunk);
+      for (int r = 0; r < 16; ++r) v[r] = __ldcg(s + r * kChunk);
 #pragma unroll
       for (int r = 0; r < 16; ++r) a += ptx::ex2(v[r] - slse[tile * 16 + r]);
     } else {
       for (int r = 0; r < p.heads - 16 * tile; ++r)
-        a += ptx::ex2(__ldg(s + r * kChunk) - slse[tile * 16 + r]);
+        a += ptx::ex2(__ldcg(s + r * kChunk) - slse[tile * 16 + r]);
     }
   }
   if (t >= len) return;
@@ -1500,10 +1543,37 @@ int launch_attention(const Cache& c, const void* q, int heads, int max_len, floa
   DS_CUDA(cudaLaunchKernelEx(&cfg, merge_kernel, p));
   DS_LAUNCH_CHECK("merge_kernel");
   if (accumulate && max_len > 0) {
-    mass_kernel<<<dim3(p.max_chunks, c.batch), kChunk, 0, s>>>(p, decay);
+    cfg.gridDim = dim3(p.max_chunks, c.batch);
+    cfg.blockDim = dim3(kChunk);
+    DS_CUDA(cudaLaunchKernelEx(&cfg, mass_kernel, p, decay));
     DS_LAUNCH_CHECK("mass_kernel");
   }
   return DS_OK;
+}
+
+// A decode step's buffers in its workspace.
+struct StepBuffers {
+  __nv_bfloat16* proj;  // [batch, heads * 576 + 576]
+  __nv_bfloat16* q;     // [batch, heads, 576]
+  __nv_bfloat16* olat;  // [batch, heads * 512]
+  uint8_t* linear;
+  size_t linear_bytes;
+  uint8_t* attn;
+  size_t attn_bytes;
+};
+void carve_step(Carve& w, StepBuffers* s, int batch, int heads, int hidden, int max_len,
+                int num_sms, bool mass) {
+  Carve a(nullptr, 0);
+  AttnBuffers ab{};
+  carve_attn(a, &ab, batch, heads, max_len, num_sms, mass);
+  s->attn_bytes = align_up(a.used, 256);
+  s->linear_bytes = std::max(i8::linear_workspace(batch, hidden),
+                             i8::linear_workspace(batch, heads * kLatent));
+  s->proj = w.take<__nv_bfloat16>(static_cast<size_t>(batch) * (heads + 1) * kQCols);
+  s->q = w.take<__nv_bfloat16>(static_cast<size_t>(batch) * heads * kQCols);
+  s->olat = w.take<__nv_bfloat16>(static_cast<size_t>(batch) * heads * kLatent);
+  s->linear = w.take<uint8_t>(s->linear_bytes);
+  s->attn = w.take<uint8_t>(s->attn_bytes);
 }
 
 }  // namespace
@@ -1512,6 +1582,15 @@ int launch_attention(const Cache& c, const void* q, int heads, int max_len, floa
 
 // ---- C ABI ------------------------------------------------------------------------------------
 extern "C" {
+
+int ds_mla_cache4_reset(int32_t* state, int batch, void* stream) {
+  DS_REQUIRE(batch >= 0 && batch <= 65535, "mla_cache4_reset: batch must be at most 65535");
+  if (batch == 0) return DS_OK;
+  DS_REQUIRE(state != nullptr, "mla_cache4_reset: null pointer");
+  DS_CUDA(cudaMemsetAsync(state, 0, static_cast<size_t>(batch) * 3 * sizeof(int32_t),
+                          static_cast<cudaStream_t>(stream)));
+  return DS_OK;
+}
 
 int ds_mla_cache4_append(const void* latent_bf16, int64_t latent_ld, const void* kpe_bf16,
                          int64_t kpe_ld, int64_t src_rows_per_seq, int new_tokens,
@@ -1589,6 +1668,61 @@ int ds_mla_decode_attention4(const void* q_bf16, int heads, const void* codes,
   return ds::c4::launch_attention(c, q_bf16, heads, max_len, softmax_scale, accumulate, mass_decay,
                                   out_bf16, workspace, workspace_bytes,
                                   static_cast<cudaStream_t>(stream));
+}
+
+size_t ds_mla_decode4_workspace_size(int batch, int heads, int hidden, int max_len,
+                                     int accumulate) {
+  if (batch <= 0 || heads <= 0 || hidden <= 0 || max_len < 0) return 0;
+  ds::DeviceInfo di;
+  if (ds::device_info(&di) != DS_OK) return 0;
+  ds::Carve w(nullptr, 0);
+  ds::c4::StepBuffers s{};
+  ds::c4::carve_step(w, &s, batch, heads, hidden, max_len, di.num_sms, accumulate != 0);
+  return ds::align_up(w.used, 256);
+}
+
+int ds_mla_decode4_step(const void* x_bf16, const void* w_dec_int8, const float* w_dec_scale,
+                        const void* w_out_int8, const float* w_out_scale, const void* cos_bf16,
+                        const void* sin_bf16, int table_rows, int hidden, int heads, float eps,
+                        float softmax_scale, int accumulate, float mass_decay, void* codes,
+                        void* scales_bf16, float* rstd, int32_t* pos, float* mass, int32_t* state,
+                        int batch, int slots, int max_len, void* out_bf16, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  using namespace ds::c4;
+  const Cache c = cache_of(codes, scales_bf16, rstd, pos, mass, state, batch, slots);
+  DS_REQUIRE(heads >= 1 && heads <= kMaxHeads, "mla_decode4_step: heads=%d outside [1, %d]", heads,
+             kMaxHeads);
+  DS_REQUIRE(hidden > 0 && hidden % 16 == 0, "mla_decode4_step: hidden=%d must be a multiple of 16",
+             hidden);
+  DS_TRY(check_cache(c, "mla_decode4_step"));
+  DS_REQUIRE(max_len >= 1 && max_len <= slots, "mla_decode4_step: max_len outside the cache");
+  DS_REQUIRE(table_rows > 0, "mla_decode4_step: empty RoPE tables");
+  if (batch == 0) return DS_OK;
+  DS_REQUIRE(x_bf16 && w_dec_int8 && w_dec_scale && w_out_int8 && w_out_scale && cos_bf16 &&
+                 sin_bf16 && out_bf16 && workspace,
+             "mla_decode4_step: null pointer");
+  DS_REQUIRE(ds::aligned16(x_bf16) && ds::aligned16(w_dec_int8) && ds::aligned16(w_out_int8) &&
+                 ds::aligned16(out_bf16) && ds::aligned16(workspace),
+             "mla_decode4_step: x, weights, out and workspace must be 16-byte aligned");
+  ds::DeviceInfo di;
+  DS_TRY(ds::device_info(&di));
+  ds::Carve w(workspace, workspace_bytes);
+  StepBuffers b{};
+  carve_step(w, &b, batch, heads, hidden, max_len, di.num_sms, accumulate != 0);
+  if (!w.ok())
+    return ds::fail(DS_ERR_WORKSPACE, "mla_decode4_step: workspace needs %zu bytes", w.used);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int cols = (heads + 1) * kQCols;
+  DS_TRY(ds::i8::launch_linear(x_bf16, hidden, w_dec_int8, w_dec_scale, b.proj, batch, cols, hidden,
+                               b.linear, b.linear_bytes, s));
+  decode4_prepare_kernel<<<batch, 288, 0, s>>>(
+      c, b.proj, cols, heads, static_cast<const __nv_bfloat16*>(cos_bf16),
+      static_cast<const __nv_bfloat16*>(sin_bf16), table_rows, eps, b.q);
+  DS_LAUNCH_CHECK("decode4_prepare_kernel");
+  DS_TRY(launch_attention(c, b.q, heads, max_len, softmax_scale, accumulate, mass_decay, b.olat,
+                          b.attn, b.attn_bytes, s));
+  return ds::i8::launch_linear(b.olat, heads * kLatent, w_out_int8, w_out_scale, out_bf16, batch,
+                               hidden, heads * kLatent, b.linear, b.linear_bytes, s);
 }
 
 size_t ds_mla_cache4_evict_workspace_size(int batch, int budget) {

@@ -19,7 +19,7 @@ import torch
 
 import ds_kernels
 from mla import FusedMLA
-from mla_cache import LatentKVCache
+from mla_cache import LatentKVCache, LatentKVCache4
 
 
 class DenseFFN:
@@ -54,9 +54,20 @@ class FusedDecoderStack:
     def __init__(self, layers: Sequence[FusedDecoderLayer]):
         self.layers = list(layers)
 
-    def new_caches(self, bsz: int, max_seq: int, device=None) -> List[LatentKVCache]:
+    def new_caches(self, bsz: int, max_seq: int, device=None, bits: int = 16) -> list:
+        """One cache a layer: LatentKVCache (bits=16) or LatentKVCache4 (bits=4: a fourth of the
+        memory, 8-bit projections in the decode step, eviction)."""
         dev = device if device is not None else self.layers[0].w_in.device
-        return [LatentKVCache(bsz, max_seq, device=dev) for _ in self.layers]
+        if bits not in (4, 16):
+            raise ValueError(f"new_caches: bits must be 16 or 4, got {bits}")
+        kind = LatentKVCache4 if bits == 4 else LatentKVCache
+        return [kind(bsz, max_seq, device=dev) for _ in self.layers]
+
+    @staticmethod
+    def evict(caches: Sequence[LatentKVCache4], budget: int, recent: int = 0) -> None:
+        """Every layer's cache down to `budget` slots a sequence, by its own accumulated weights."""
+        for c in caches:
+            c.evict(budget, recent)
 
     def _run(self, x2: torch.Tensor, attn_fn, ffn_rows) -> torch.Tensor:
         L = self.layers
@@ -72,31 +83,38 @@ class FusedDecoderStack:
             normed, hidden = ds_kernels.rms_norm_residual(f, hidden, w_next, eps)
         return hidden
 
-    def decode_step(self, x: torch.Tensor, caches: Sequence[LatentKVCache]) -> torch.Tensor:
-        """x bf16 [bsz, hidden] (one new token per sequence) -> [bsz, hidden]."""
-        return self._run(x.contiguous(), lambda layer, h, i: layer.attn.decode(h, caches[i]),
+    def decode_step(self, x: torch.Tensor, caches: Sequence[LatentKVCache],
+                    mass_decay: Optional[float] = None) -> torch.Tensor:
+        """x bf16 [bsz, hidden] (one new token per sequence) -> [bsz, hidden].  mass_decay (4-bit
+        caches): accumulate every layer's attention weights for evict()."""
+        return self._run(x.contiguous(),
+                         lambda layer, h, i: layer.attn.decode(h, caches[i], mass_decay=mass_decay),
                          lambda h: h)
 
-    def capture_decode(self, x: torch.Tensor, caches: Sequence[LatentKVCache]) -> torch.Tensor:
+    def capture_decode(self, x: torch.Tensor, caches: Sequence[LatentKVCache],
+                       mass_decay: Optional[float] = None) -> torch.Tensor:
         """Run one decode step eagerly (it allocates the workspaces and brings the caches' side
         arrays up to date, and advances the caches by one position), then record the step as a
         CUDA graph: the ~15 launches of each of the layers become one graph launch.  The
         kernels read the position from each cache's device-side length and advance it, so
         replay_decode() steps through successive positions.  Returns the eager step's output."""
         self._graph_x = x.contiguous().clone()
-        first = self.decode_step(self._graph_x, caches)
+        first = self.decode_step(self._graph_x, caches, mass_decay)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         stream = torch.cuda.Stream()
         stream.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(stream):
             with torch.cuda.graph(graph, stream=stream):
-                self._graph_out = self.decode_step(self._graph_x, caches)
+                self._graph_out = self.decode_step(self._graph_x, caches, mass_decay)
         torch.cuda.current_stream().wait_stream(stream)
         # recording ran the host-side bookkeeping of one step without executing it on the GPU
         for c in caches:
-            c._len -= 1
-            c._side_len -= 1
+            if isinstance(c, LatentKVCache4):
+                c.note_replay(-1)
+            else:
+                c._len -= 1
+                c._side_len -= 1
         self._graph = graph
         self._graph_caches = list(caches)
         return first
@@ -110,8 +128,11 @@ class FusedDecoderStack:
         self._graph_x.copy_(x, non_blocking=True)
         self._graph.replay()
         for c in self._graph_caches:
-            c._len += 1
-            c._side_len += 1
+            if isinstance(c, LatentKVCache4):
+                c.note_replay()
+            else:
+                c._len += 1
+                c._side_len += 1
         return self._graph_out
 
     def prefill(self, x: torch.Tensor, caches: Sequence[LatentKVCache]) -> torch.Tensor:

@@ -117,12 +117,16 @@ SIGNATURES = {
     "ds_int8_quantize": (_i, [_vp, _i64, _i, _i, _vp, _vp, _vp]),
     "ds_int8_linear_workspace_size": (_sz, [_i, _i, _i]),
     "ds_int8_linear": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "ds_mla_cache4_reset": (_i, [_vp, _i, _vp]),
     "ds_mla_cache4_append": (_i, [_vp, _i64, _vp, _i64, _i64, _i, _vp, _vp, _vp, _i, _f, _vp, _vp,
                                   _vp, _vp, _vp, _vp, _i, _i, _vp]),
     "ds_mla_cache4_get": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
     "ds_mla_decode_attention4_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
     "ds_mla_decode_attention4": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _f,
                                       _vp, _vp, _sz, _vp]),
+    "ds_mla_decode4_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "ds_mla_decode4_step": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _f, _i, _f,
+                                 _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "ds_mla_cache4_evict_workspace_size": (_sz, [_i, _i]),
     "ds_mla_cache4_evict": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp,
                                  _vp, _vp, _i, _vp, _sz, _vp]),
@@ -801,10 +805,20 @@ def int8_quantize(x: torch.Tensor) -> List[torch.Tensor]:
     if x.numel() == 0:
         return [q, scale]
     x2 = _rows_2d(x)
-    with _on_device(x):
-        _check(_lib.ds_int8_quantize(x2.data_ptr(), x2.stride(0), x2.shape[0], K, q.data_ptr(),
-                                     scale.data_ptr(), _stream(x)), "int8_quantize")
+    _call("int8_quantize", x.get_device(), _lib.ds_int8_quantize, x2.data_ptr(), x2.stride(0),
+          x2.shape[0], K, q.data_ptr(), scale.data_ptr())
     return [q, scale]
+
+
+def _call(op: str, dev: int, fn, *args) -> None:
+    """fn(*args, current stream of device `dev`) with that device current."""
+    if dev == _current_device():
+        status = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _raw_stream(dev))
+    if status:
+        _check(status, op)
 
 
 def _rows_2d(x: torch.Tensor) -> torch.Tensor:
@@ -853,14 +867,15 @@ def int8_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
     x2 = _rows_2d(x)
     rows = x2.shape[0]
     need = int8_linear_workspace_size(rows, N, K)
-    if workspace is None or workspace.numel() < need:
-        workspace = w_q.new_empty(need)
-    else:
-        workspace = _scratch(workspace, need, x.device, "int8_linear")
-    with _on_device(x):
-        _check(_lib.ds_int8_linear(x2.data_ptr(), x2.stride(0), w_q.data_ptr(),
-                                   w_scale.data_ptr(), out.data_ptr(), rows, N, K,
-                                   workspace.data_ptr(), need, _stream(x)), "int8_linear")
+    space = None
+    if need:
+        if workspace is None or workspace.numel() < need:
+            workspace = w_q.new_empty(need)
+        else:
+            workspace = _scratch(workspace, need, x.device, "int8_linear")
+        space = workspace.data_ptr()
+    _call("int8_linear", dev, _lib.ds_int8_linear, x2.data_ptr(), x2.stride(0), w_q.data_ptr(),
+          w_scale.data_ptr(), out.data_ptr(), rows, N, K, space, need)
     return out
 
 
@@ -892,50 +907,56 @@ def mla_cache4_append(latent: torch.Tensor, k_pe: torch.Tensor, cache, cos: torc
     (mla_cache.LatentKVCache4), k_pe rotated at its position (cos/sin bf16 [positions, 64]).
     new_lens int32 [bsz] (on the device): only the first new_lens[b] tokens of sequence b (a
     ragged, padded batch)."""
-    dev = cache.device
-    shape = latent.shape
-    if not (latent.is_cuda and latent.dtype is _bf16 and k_pe.dtype is _bf16 and len(shape) == 3
-            and shape[2] == 512 and shape[0] == cache.bsz and k_pe.shape == (shape[0], shape[1], 64)
-            and latent.device == dev and k_pe.device == dev):
+    dev, shape, B = cache.index, latent.shape, cache.bsz
+    if not (dev >= 0 and latent.dtype is _bf16 and k_pe.dtype is _bf16 and len(shape) == 3
+            and shape[2] == 512 and shape[0] == B and k_pe.shape == (B, shape[1], 64)
+            and latent.get_device() == dev and k_pe.get_device() == dev):
         _require(latent.is_cuda and k_pe.is_cuda, "mla_cache4_append: inputs must be CUDA tensors.")
         _require(latent.dtype == _bf16 and k_pe.dtype == _bf16,
                  "mla_cache4_append: latent and k_pe must be bfloat16.")
-        _require(latent.dim() == 3 and shape[2] == 512 and shape[0] == cache.bsz
+        _require(latent.dim() == 3 and shape[2] == 512 and shape[0] == B
                  and tuple(k_pe.shape) == (*shape[:2], 64),
                  "mla_cache4_append: latent must be [bsz, n, 512] and k_pe [bsz, n, 64].")
         _require(False, "mla_cache4_append: inputs and cache must be on one device.")
     _check_tables(cos, sin, dev, "mla_cache4_append")
-    B, n, _ = shape
+    n = shape[1]
+    lens = None
     if new_lens is not None:
-        _require(new_lens.dtype is _i32 and new_lens.dim() == 1 and new_lens.shape[0] == B
-                 and new_lens.is_contiguous() and new_lens.device == dev,
-                 "mla_cache4_append: new_lens must be a contiguous int32 [bsz] tensor on the "
-                 "cache's device.")
+        if not (new_lens.dtype is _i32 and new_lens.shape == (B,) and new_lens.is_contiguous()
+                and new_lens.get_device() == dev):
+            _require(False, "mla_cache4_append: new_lens must be a contiguous int32 [bsz] tensor on "
+                            "the cache's device.")
+        lens = new_lens.data_ptr()
     if n == 0:
         return
     cache._check_room(n, cos.shape[0])
     lb, lt, l1 = latent.stride()
     kb, kt, k1 = k_pe.stride()
     rows = lb // lt if lt > 0 else 0
-    if not (l1 == 1 and k1 == 1 and lt > 0 and kt > 0 and lt % 8 == 0 and kt % 8 == 0
-            and lb == rows * lt and kb == rows * kt and latent.data_ptr() % 16 == 0
-            and k_pe.data_ptr() % 16 == 0):
-        latent = torch.empty(shape, dtype=_bf16, device=dev).copy_(latent)
-        k_pe = torch.empty((B, n, 64), dtype=_bf16, device=dev).copy_(k_pe)
+    if not (l1 == 1 and k1 == 1 and lt > 0 and kt > 0 and not (lt | kt) & 7 and lb == rows * lt
+            and kb == rows * kt and not (latent.data_ptr() | k_pe.data_ptr()) & 15):
+        latent = torch.empty(shape, dtype=_bf16, device=cache.device).copy_(latent)
+        k_pe = torch.empty((B, n, 64), dtype=_bf16, device=cache.device).copy_(k_pe)
         lt, kt, rows = 512, 64, n
-    with _on_device(latent):
-        _check(_lib.ds_mla_cache4_append(latent.data_ptr(), lt, k_pe.data_ptr(), kt, rows, n,
-                                         None if new_lens is None else new_lens.data_ptr(),
-                                         cos.data_ptr(), sin.data_ptr(), cos.shape[0], float(eps),
-                                         *cache._ptrs, B, cache.slots, _stream(latent)),
-               "mla_cache4_append")
+    _call("mla_cache4_append", dev, _lib.ds_mla_cache4_append, latent.data_ptr(), lt,
+          k_pe.data_ptr(), kt, rows, n, lens, cos.data_ptr(), sin.data_ptr(), cos.shape[0], eps,
+          *cache._ptrs, B, cache.slots)
     cache._advance(n)
 
 
-def _check_tables(cos: torch.Tensor, sin: torch.Tensor, dev: torch.device, op: str) -> None:
-    if not (cos.dtype is _bf16 and sin.dtype is _bf16 and cos.dim() == 2 and cos.shape[1] == 64
-            and cos.shape[0] > 0 and sin.shape == cos.shape and cos.is_contiguous()
-            and sin.is_contiguous() and cos.device == dev and sin.device == dev):
+def mla_cache4_reset(cache) -> None:
+    """Lengths and positions of every sequence to 0 (LatentKVCache4.reset)."""
+    if cache.index < 0:
+        cache.state.zero_()
+        return
+    _call("mla_cache4_reset", cache.index, _lib.ds_mla_cache4_reset, cache._ptrs[5], cache.bsz)
+
+
+def _check_tables(cos: torch.Tensor, sin: torch.Tensor, dev: int, op: str) -> None:
+    shape = cos.shape
+    if not (cos.dtype is _bf16 and sin.dtype is _bf16 and len(shape) == 2 and shape[1] == 64
+            and shape[0] > 0 and sin.shape == shape and cos.is_contiguous() and sin.is_contiguous()
+            and cos.get_device() == dev and sin.get_device() == dev):
         _require(False, f"{op}: cos and sin must be contiguous bfloat16 [positions, 64] tensors on "
                         "the cache's device.")
 
@@ -944,7 +965,8 @@ def mla_cache4_get(cache, seq_len: Optional[int] = None) -> List[torch.Tensor]:
     """The cache read back as bf16 values: [raw latent [bsz, seq_len, 512], rotated k_pe
     [bsz, seq_len, 64]], zeros from a sequence's length on; seq_len defaults to the cache's
     current_len (its longest sequence's bound)."""
-    _require_cache4(cache, "mla_cache4_get")
+    if cache.index < 0:
+        _require_cache4(cache, "mla_cache4_get")
     n = cache.current_len if seq_len is None else int(seq_len)
     if not 0 <= n <= cache.slots:
         _require(False, f"mla_cache4_get: seq_len={n} outside the cache.")
@@ -952,10 +974,9 @@ def mla_cache4_get(cache, seq_len: Optional[int] = None) -> List[torch.Tensor]:
     kpe = cache.scales.new_empty((cache.bsz, n, 64))
     if n == 0:
         return [lat, kpe]
-    with _on_device(lat):
-        _check(_lib.ds_mla_cache4_get(cache._ptrs[0], cache._ptrs[1], cache._ptrs[5], cache.bsz,
-                                      cache.slots, n, lat.data_ptr(), kpe.data_ptr(),
-                                      _stream(lat)), "mla_cache4_get")
+    codes, scales, _, _, _, state = cache._ptrs
+    _call("mla_cache4_get", cache.index, _lib.ds_mla_cache4_get, codes, scales, state, cache.bsz,
+          cache.slots, n, lat.data_ptr(), kpe.data_ptr())
     return [lat, kpe]
 
 
@@ -967,8 +988,9 @@ def mla_decode_attention4_workspace_size(batch: int, heads: int, slots: int, max
 
 @functools.lru_cache(maxsize=4096)
 def _attention4_workspace(batch, heads, slots, max_len, accumulate, device) -> int:
-    return int(_lib.ds_mla_decode_attention4_workspace_size(batch, heads, slots, max_len,
-                                                            1 if accumulate else 0))
+    with torch.cuda.device(device):
+        return int(_lib.ds_mla_decode_attention4_workspace_size(batch, heads, slots, max_len,
+                                                                1 if accumulate else 0))
 
 
 def mla_decode_attention4(q: torch.Tensor, cache, softmax_scale: float,
@@ -981,37 +1003,97 @@ def mla_decode_attention4(q: torch.Tensor, cache, softmax_scale: float,
 
     With mass_decay the attention weights are accumulated for a later eviction:
     cache.mass[b, t] = mass_decay * cache.mass[b, t] + sum over heads of p(t)."""
-    dev = cache.device
-    if not (q.is_cuda and q.dtype is _bf16 and q.is_contiguous() and q.dim() == 3
-            and q.shape[0] == cache.bsz and q.shape[2] == 576 and q.device == dev
-            and 1 <= q.shape[1] <= 128 and q.data_ptr() % 16 == 0):
+    dev, B = cache.index, cache.bsz
+    shape = q.shape
+    if not (dev >= 0 and q.dtype is _bf16 and len(shape) == 3 and shape[0] == B
+            and shape[2] == 576 and 1 <= shape[1] <= 128 and q.is_contiguous()
+            and q.get_device() == dev and not q.data_ptr() & 15):
         _require(q.is_cuda and q.dtype == _bf16 and q.is_contiguous(),
                  "mla_decode_attention4: q must be a contiguous bfloat16 CUDA tensor.")
-        _require(q.dim() == 3 and q.shape[0] == cache.bsz and q.shape[2] == 576,
+        _require(q.dim() == 3 and shape[0] == B and shape[2] == 576,
                  "mla_decode_attention4: q must be [bsz, heads, 576].")
-        _require(q.device == dev, "mla_decode_attention4: q and cache must be on one device.")
-        _require(1 <= q.shape[1] <= 128, "mla_decode_attention4: heads must be in [1, 128].")
+        _require(q.device == cache.device,
+                 "mla_decode_attention4: q and cache must be on one device.")
+        _require(1 <= shape[1] <= 128, "mla_decode_attention4: heads must be in [1, 128].")
         q = q.clone()  # a view that starts off a 16-byte boundary
     acc = mass_decay is not None
     if acc and not 0.0 <= mass_decay <= 1.0:
         _require(False, "mla_decode_attention4: mass_decay must be in [0, 1].")
-    B, heads, _ = q.shape
+    heads = shape[1]
     if out is None:
         out = q.new_empty((B, heads * 512))
     else:
-        _check_out(out, B, heads * 512, dev)
+        _check_out(out, B, heads * 512, cache.device)
     max_len = cache.bound_for_launch
-    with _on_device(q):
-        need = _attention4_workspace(B, heads, cache.slots, max_len, acc, q.get_device())
-        if workspace is None or workspace.numel() < need:
-            workspace = cache.codes.new_empty(need)
-        else:
-            workspace = _scratch(workspace, need, dev, "mla_decode_attention4")
-        codes, scales, rstd, _, mass, state = cache._ptrs
-        _check(_lib.ds_mla_decode_attention4(
-            q.data_ptr(), heads, codes, scales, rstd, mass, state, B, cache.slots, max_len,
-            softmax_scale, 1 if acc else 0, mass_decay if acc else 0.0, out.data_ptr(),
-            workspace.data_ptr(), workspace.numel(), _stream(q)), "mla_decode_attention4")
+    need = _attention4_workspace(B, heads, cache.slots, max_len, acc, dev)
+    if workspace is None or workspace.numel() < need:
+        workspace = cache.codes.new_empty(need)
+    else:
+        workspace = _scratch(workspace, need, cache.device, "mla_decode_attention4")
+    codes, scales, rstd, _, mass, state = cache._ptrs
+    _call("mla_decode_attention4", dev, _lib.ds_mla_decode_attention4, q.data_ptr(), heads, codes,
+          scales, rstd, mass, state, B, cache.slots, max_len, softmax_scale, 1 if acc else 0,
+          mass_decay if acc else 0.0, out.data_ptr(), workspace.data_ptr(), need)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _decode4_workspace(batch, heads, hidden, max_len, accumulate, device) -> int:
+    with torch.cuda.device(device):
+        return int(_lib.ds_mla_decode4_workspace_size(batch, heads, hidden, max_len,
+                                                      1 if accumulate else 0))
+
+
+def mla_decode4_step(x: torch.Tensor, w_dec: torch.Tensor, w_dec_scale: torch.Tensor,
+                     w_out: torch.Tensor, w_out_scale: torch.Tensor, cos: torch.Tensor,
+                     sin: torch.Tensor, cache, softmax_scale: float, heads: int = 16,
+                     eps: float = 1e-6, mass_decay: Optional[float] = None,
+                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One decode step over a 4-bit cache with 8-bit weights (mla_decode_step's counterpart): x
+    bf16 [bsz, hidden] (one new token per sequence) -> [bsz, hidden].  w_dec int8 [heads*576 + 576,
+    hidden] and w_out int8 [hidden, heads*512] with their scales per row (int8_quantize of
+    FusedMLA.decode_weights()).  Appends the token to every sequence of `cache`
+    (mla_cache.LatentKVCache4) and attends over all it then holds; mass_decay as in
+    mla_decode_attention4."""
+    op = "mla_decode4_step"
+    dev, B = cache.index, cache.bsz
+    hidden = x.shape[-1]
+    if not (dev >= 0 and x.dtype is _bf16 and x.shape == (B, hidden) and x.is_contiguous()
+            and x.get_device() == dev and not x.data_ptr() & 15
+            and w_dec.shape == ((heads + 1) * 576, hidden) and w_out.shape == (hidden, heads * 512)
+            and w_dec_scale.shape == w_dec.shape[:1] and w_out_scale.shape == w_out.shape[:1]
+            and all(w.dtype is _i8 and w.is_contiguous() and w.get_device() == dev
+                    for w in (w_dec, w_out))
+            and all(w.dtype is _f32 and w.is_contiguous() and w.get_device() == dev
+                    for w in (w_dec_scale, w_out_scale))):
+        _require(x.is_cuda and x.dtype == _bf16 and x.is_contiguous() and not x.data_ptr() & 15,
+                 f"{op}: x must be a contiguous, 16-byte aligned bfloat16 CUDA tensor.")
+        _require(tuple(x.shape) == (B, hidden), f"{op}: x must be [bsz, hidden].")
+        _require(tuple(w_dec.shape) == ((heads + 1) * 576, hidden)
+                 and tuple(w_out.shape) == (hidden, heads * 512)
+                 and w_dec_scale.shape == w_dec.shape[:1] and w_out_scale.shape == w_out.shape[:1],
+                 f"{op}: w_dec must be [heads*576 + 576, hidden], w_out [hidden, heads*512], each "
+                 "with a scale per row.")
+        _require(False, f"{op}: weights must be contiguous int8 and their scales float32, on the "
+                        "cache's device.")
+    _check_tables(cos, sin, dev, op)
+    cache._check_room(1, cos.shape[0])
+    acc = mass_decay is not None
+    if acc and not 0.0 <= mass_decay <= 1.0:
+        _require(False, f"{op}: mass_decay must be in [0, 1].")
+    out = x.new_empty((B, hidden))
+    max_len = min(cache.bound_for_launch + 1, cache.max_seq)
+    need = _decode4_workspace(B, heads, hidden, max_len, acc, dev)
+    if workspace is None or workspace.numel() < need:
+        workspace = cache.codes.new_empty(need)
+    else:
+        workspace = _scratch(workspace, need, cache.device, op)
+    _call(op, dev, _lib.ds_mla_decode4_step, x.data_ptr(), w_dec.data_ptr(),
+          w_dec_scale.data_ptr(), w_out.data_ptr(), w_out_scale.data_ptr(), cos.data_ptr(),
+          sin.data_ptr(), cos.shape[0], hidden, heads, eps, softmax_scale, 1 if acc else 0,
+          mass_decay if acc else 0.0, *cache._ptrs, B, cache.slots, max_len, out.data_ptr(),
+          workspace.data_ptr(), need)
+    cache._advance(1)
     return out
 
 
@@ -1022,10 +1104,11 @@ def mla_cache4_evict(cache, budget: int, recent: int = 0, out=None):
     (another LatentKVCache4 of the same batch with at least `budget` slots, whose contents it
     replaces).  Survivors behind the budget fill the freed slots before it, both in ascending
     order; the others stay.  Returns the cache that holds the result."""
-    _require_cache4(cache, "mla_cache4_evict")
+    if cache.index < 0:
+        _require_cache4(cache, "mla_cache4_evict")
     dst = cache if out is None else out
     budget, recent = int(budget), int(recent)
-    if not (dst.bsz == cache.bsz and dst.device == cache.device and 1 <= budget <= dst.max_seq
+    if not (dst.bsz == cache.bsz and dst.index == cache.index and 1 <= budget <= dst.max_seq
             and 0 <= recent <= budget):
         _require(dst.bsz == cache.bsz and dst.device == cache.device,
                  "mla_cache4_evict: out must have the cache's batch size and device.")
@@ -1034,10 +1117,8 @@ def mla_cache4_evict(cache, budget: int, recent: int = 0, out=None):
         _require(False, "mla_cache4_evict: recent must be in [0, budget].")
     need = _evict_workspace(cache.bsz, budget)
     ws = cache.codes.new_empty(need)
-    with _on_device(ws):
-        _check(_lib.ds_mla_cache4_evict(*cache._ptrs, cache.bsz, cache.slots, budget, recent,
-                                        *dst._ptrs, dst.slots, ws.data_ptr(), need, _stream(ws)),
-               "mla_cache4_evict")
+    _call("mla_cache4_evict", cache.index, _lib.ds_mla_cache4_evict, *cache._ptrs, cache.bsz,
+          cache.slots, budget, recent, *dst._ptrs, dst.slots, ws.data_ptr(), need)
     dst._evicted(cache, budget)
     return dst
 

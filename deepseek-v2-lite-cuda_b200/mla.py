@@ -19,6 +19,11 @@ through ds_mla_decode_step.  The decode weights absorb the kv_b projection (fold
 f32, rounded to bf16): the query weights become diag(g) W_uk_h^T W_q_nope_h per head (g the
 latent norm weight) and the output weights W_o_h W_uv_h diag(g), so the attention scores and
 values are taken against the 512-wide cached latent directly.
+
+Both take a 4-bit cache (mla_cache.LatentKVCache4) too: prefill quantises the prompt's latents
+into it, and decode runs ds_mla_decode4_step, with the absorbed weights quantised to 8 bits per
+output channel (quantized_decode_weights) and, if asked for, the attention weights accumulated in
+the cache for its eviction.
 """
 from __future__ import annotations
 
@@ -28,6 +33,7 @@ import torch
 import torch.nn as nn
 
 import ds_kernels
+from mla_cache import LatentKVCache, LatentKVCache4
 
 
 class FusedMLA(nn.Module):
@@ -55,6 +61,7 @@ class FusedMLA(nn.Module):
         self.softmax_scale = float(m.softmax_scale)
         self._ws: Optional[torch.Tensor] = None
         self._dec_w = None
+        self._dec_q = None
         self._dec_ws: Optional[torch.Tensor] = None
 
     @classmethod
@@ -79,6 +86,7 @@ class FusedMLA(nn.Module):
         self.softmax_scale = float(softmax_scale)
         self._ws = None
         self._dec_w = None
+        self._dec_q = None
         self._dec_ws = None
         return self
 
@@ -101,10 +109,33 @@ class FusedMLA(nn.Module):
                            w_out.to(torch.bfloat16).contiguous())
         return self._dec_w
 
-    def prefill(self, hidden_states: torch.Tensor, cache) -> torch.Tensor:
-        """forward() over a prompt at positions 0 .. seq-1 that also fills the (empty) cache."""
+    def quantized_decode_weights(self):
+        """(w_dec int8, its scales f32, w_out int8, its scales f32): decode_weights() in 8 bits with
+        a scale per output channel, built once."""
+        if self._dec_q is None:
+            w_dec, w_out = self.decode_weights()
+            self._dec_q = (*ds_kernels.int8_quantize(w_dec), *ds_kernels.int8_quantize(w_out))
+        return self._dec_q
+
+    def prefill(self, hidden_states: torch.Tensor, cache,
+                prompt_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """forward() over a prompt at positions 0 .. seq-1 that also fills the (empty) cache.
+        A 4-bit cache takes prompt_lens (int32 [bsz], on the device) for padded prompts: only the
+        first prompt_lens[b] tokens of sequence b enter it."""
         x = hidden_states.to(torch.bfloat16)
         B, S, _ = x.shape
+        if isinstance(cache, LatentKVCache4):
+            if cache.current_len != 0 or cache.bsz != B:
+                raise RuntimeError("FusedMLA.prefill: the cache must be empty and of x's batch size")
+            if S == 0:
+                return torch.empty_like(x)
+            exact = LatentKVCache(B, S, device=x.device)
+            out = self.prefill(x, exact)
+            ds_kernels.mla_cache4_append(exact.kv_latent, exact.k_pe_cache, cache, self.cos,
+                                         self.sin, self.eps, new_lens=prompt_lens)
+            return out
+        if prompt_lens is not None:
+            raise NotImplementedError("FusedMLA.prefill: prompt_lens needs a 4-bit cache")
         need = ds_kernels.mla_forward_workspace_size(B, S, self.hidden, self.heads)
         if self._ws is None or self._ws.numel() < need or self._ws.device != x.device:
             self._ws = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
@@ -112,11 +143,23 @@ class FusedMLA(nn.Module):
                                       self.w_o, self.cos, self.sin, self.softmax_scale,
                                       self.heads, cache, eps=self.eps, workspace=self._ws)
 
-    def decode(self, hidden_states: torch.Tensor, cache, events=None) -> torch.Tensor:
+    def decode(self, hidden_states: torch.Tensor, cache, events=None,
+               mass_decay: Optional[float] = None) -> torch.Tensor:
         """One new token per sequence: hidden_states [bsz, hidden] or [bsz, 1, hidden] ->
-        same shape; the token is appended to `cache` at its current length."""
+        same shape; the token is appended to `cache` at its current length.  With a 4-bit cache,
+        mass_decay accumulates the attention weights in it (mla_decode_attention4)."""
         x = hidden_states.to(torch.bfloat16)
         x2 = x.reshape(x.shape[0], self.hidden).contiguous()
+        if isinstance(cache, LatentKVCache4):
+            if events is not None:
+                raise NotImplementedError("FusedMLA.decode: events need a bf16 cache")
+            out = ds_kernels.mla_decode4_step(x2, *self.quantized_decode_weights(), self.cos,
+                                              self.sin, cache, self.softmax_scale,
+                                              heads=self.heads, eps=self.eps,
+                                              mass_decay=mass_decay)
+            return out.view(x.shape)
+        if mass_decay is not None:
+            raise NotImplementedError("FusedMLA.decode: mass_decay needs a 4-bit cache")
         if cache.current_len >= self.cos.shape[0]:
             raise RuntimeError("FusedMLA.decode: position beyond the RoPE tables")
         w_dec, w_out = self.decode_weights()

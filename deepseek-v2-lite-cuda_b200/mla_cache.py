@@ -20,6 +20,8 @@ from typing import Optional, Tuple
 
 import torch
 
+_capturing = torch.cuda.is_current_stream_capturing
+
 
 class LatentKVCache:
     def __init__(self, bsz: int, max_seq: int, kv_lora_rank: int = 512, rope_head_dim: int = 64,
@@ -185,7 +187,8 @@ class LatentKVCache4:
         self.slots = -(-max_seq // 64) * 64
         dev = torch.device(device)
         self.codes = torch.zeros((bsz, self.slots, 288), dtype=torch.uint8, device=dev)
-        dev = self.device = self.codes.device  # with its index
+        dev = self.device = self.codes.device
+        self.index = self.codes.get_device()    # the CUDA device's ordinal, -1 off CUDA
         self.scales = torch.zeros((bsz, 5, self.slots), dtype=torch.bfloat16, device=dev)
         self.rstd = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
         self.pos = torch.zeros((bsz, self.slots), dtype=torch.int32, device=dev)
@@ -218,11 +221,12 @@ class LatentKVCache4:
     def bound_for_launch(self) -> int:
         """The bound that a launch is sized for: all slots inside a graph capture, because a
         replay sees later lengths."""
-        return self.max_seq if torch.cuda.is_current_stream_capturing() else self._bound
+        return self.max_seq if _capturing() else self._bound
 
     def reset(self) -> None:
         """Clear the cache for new sequences (keeps the memory)."""
-        self.state.zero_()
+        import ds_kernels
+        ds_kernels.mla_cache4_reset(self)
         self._bound = self._seen = 0
 
     def get(self, seq_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:

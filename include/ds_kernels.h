@@ -503,6 +503,7 @@ DS_API int ds_int8_linear(const void* x_bf16, int64_t row_stride, const void* w_
  * then k_pe), rstd f32, pos i32 and mass f32 [batch, slots], state i32 [3, batch] (lengths in
  * slots, next positions, counters that are zero between calls).
  *
+ * ds_mla_cache4_reset: lengths and positions to 0.
  * ds_mla_cache4_append: new_tokens tokens of every sequence (token i of sequence b at row
  *   b * src_rows_per_seq + i of latent / kpe; only the first new_lens[b] when given) quantised
  *   behind its last slot, k_pe rotated at its position (table rows cos/sin [table_rows, 64];
@@ -522,6 +523,7 @@ DS_API int ds_int8_linear(const void* x_bf16, int64_t row_stride, const void* w_
  *   dst arrays (all the same as the source's: in place; or all others, [batch, dst_slots,
  *   ...]); slots behind the result's length are left as they were.
  * The calls read lengths on the device, so they can be captured into a graph and replayed. */
+DS_API int ds_mla_cache4_reset(int32_t* state, int batch, void* stream);
 DS_API int ds_mla_cache4_append(const void* latent_bf16, int64_t latent_ld, const void* kpe_bf16,
                                 int64_t kpe_ld, int64_t src_rows_per_seq, int new_tokens,
                                 const int32_t* new_lens, const void* cos_bf16,
@@ -539,6 +541,23 @@ DS_API int ds_mla_decode_attention4(const void* q_bf16, int heads, const void* c
                                     float softmax_scale, int accumulate, float mass_decay,
                                     void* out_bf16, void* workspace, size_t workspace_bytes,
                                     void* stream);
+/* One decode step of one layer over a 4-bit cache with 8-bit weights (the counterpart of
+ * ds_mla_decode_step): x bf16 [batch, hidden] -> out bf16 [batch, hidden].  w_dec int8 [heads*576 +
+ * 576, hidden] (absorbed queries, q_pe, latent, k_pe) and w_out int8 [hidden, heads*512], each
+ * with a scale per row: ds_int8_linear, append of the new token, query assembly at its position,
+ * ds_mla_decode_attention4 (max_len: a bound on the lengths after the append), ds_int8_linear.
+ * A full sequence takes no further token and attends over what it holds. */
+DS_API size_t ds_mla_decode4_workspace_size(int batch, int heads, int hidden, int max_len,
+                                            int accumulate);
+DS_API int ds_mla_decode4_step(const void* x_bf16, const void* w_dec_int8,
+                               const float* w_dec_scale, const void* w_out_int8,
+                               const float* w_out_scale, const void* cos_bf16,
+                               const void* sin_bf16, int table_rows, int hidden, int heads,
+                               float eps, float softmax_scale, int accumulate, float mass_decay,
+                               void* codes, void* scales_bf16, float* rstd, int32_t* pos,
+                               float* mass, int32_t* state, int batch, int slots, int max_len,
+                               void* out_bf16, void* workspace, size_t workspace_bytes,
+                               void* stream);
 DS_API size_t ds_mla_cache4_evict_workspace_size(int batch, int budget);
 DS_API int ds_mla_cache4_evict(void* codes, void* scales_bf16, float* rstd, int32_t* pos,
                                float* mass, int32_t* state, int batch, int slots, int budget,

@@ -45,10 +45,10 @@ C = [P(256 * i) for i in range(1, 16)]
     (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], 2, 12, 16, C[4], 1 << 20, None), 1),
     (lambda L: L.ds_int8_linear(C[0], 131088, C[1], C[2], C[3], 2, 8, 131088, C[4], 1 << 20, None), 1),
     (lambda L: L.ds_int8_linear(C[0], 16, None, C[2], C[3], 2, 8, 16, C[4], 1 << 20, None), 1),
-    (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], 2, 8, 16, None, 0, None), 1),
+    (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], 5, 8, 16, None, 0, None), 1),
     (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], -1, 8, 16, C[4], 1 << 20, None), 1),
     (lambda L: L.ds_int8_linear(C[0], 16, P(520), C[2], C[3], 2, 8, 16, C[4], 1 << 20, None), 1),
-    (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], 2, 8, 16, C[4], 31, None), 5),
+    (lambda L: L.ds_int8_linear(C[0], 16, C[1], C[2], C[3], 5, 8, 16, C[4], 31, None), 5),
     # append: slots a multiple of 64, room, aligned rows
     (lambda L: L.ds_mla_cache4_append(C[0], 512, C[1], 64, 1, 1, None, C[2], C[3], 4, F(1e-6), C[4], C[5], C[6], C[7],
                                       C[8], C[9], 1, 63, None), 1),
@@ -76,6 +76,17 @@ C = [P(256 * i) for i in range(1, 16)]
                                           0, None), 1),
     (lambda L: L.ds_mla_decode_attention4(P(260), 16, C[1], C[2], C[3], C[4], C[5], 1, 64, 4, F(1), 0, F(0), C[6], C[7],
                                           1 << 20, None), 1),
+    # the decode step: heads, hidden, room for the token, pointers
+    (lambda L: L.ds_mla_decode4_step(*C[:7], 4, 256, 0, F(1e-6), F(1), 0, F(0), *C[7:13], 1, 64, 4, C[13], C[14],
+                                     1 << 20, None), 1),
+    (lambda L: L.ds_mla_decode4_step(*C[:7], 4, 264, 16, F(1e-6), F(1), 0, F(0), *C[7:13], 1, 64, 4, C[13], C[14],
+                                     1 << 20, None), 1),
+    (lambda L: L.ds_mla_decode4_step(*C[:7], 4, 256, 16, F(1e-6), F(1), 0, F(0), *C[7:13], 1, 64, 65, C[13], C[14],
+                                     1 << 20, None), 1),
+    (lambda L: L.ds_mla_decode4_step(*C[:7], 4, 256, 16, F(1e-6), F(1), 0, F(0), *C[7:13], 1, 64, 4, C[13], None,
+                                     0, None), 1),
+    (lambda L: L.ds_mla_cache4_reset(None, 1, None), 1),
+    (lambda L: L.ds_mla_cache4_reset(C[0], 65536, None), 1),
     # evict: budget, recent, the result shares all or nothing
     (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 0, 0, *C[:6], 64, C[12], 1 << 20, None), 1),
     (lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 65, 0, *C[:6], 64, C[12], 1 << 20, None), 1),
@@ -95,6 +106,7 @@ def test_zero_size_calls_are_no_ops():
     L = lib()
     assert L.ds_int8_quantize(None, 16, 0, 16, None, None, None) == 0
     assert L.ds_int8_linear(None, 16, None, None, None, 0, 8, 16, None, 0, None) == 0
+    assert L.ds_mla_cache4_reset(None, 0, None) == 0
     assert L.ds_mla_cache4_get(None, None, None, 1, 64, 0, None, None, None) == 0
 
 
