@@ -364,7 +364,7 @@ struct AttnParams {
   int heads, tiles;        // head tiles of 16
   int max_chunks;          // of any sequence, as the host knows it
   float scale_log2;
-  float* part_o;           // [segment][16][512]
+  float* part_o;           // [segment][4 warps][16 (row half, k, j / 4)][32 lanes][4 j]: see its store
   float* part_ml;          // [segment][2][16]: maximum (log2), sum
   int2* where;             // [batch, tiles]: a row's first segment, and how many
   float* lse;              // [batch, tiles * 16]: of whole segments, then of all
@@ -916,17 +916,16 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
       }
     }
     // block j holds dimensions 128 warp + 16 (2 cc) + j and 16 (2 cc + 1) + j
+    if (whole) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int h = g + 8 * r;
-      const float f = r ? f1 : f0;
-      if (whole && h >= nh) continue;
+      for (int r = 0; r < 2; ++r) {
+        const int h = g + 8 * r;
+        const float f = r ? f1 : f0;
+        if (h >= nh) continue;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int d = 128 * warp + 16 * (2 * cc + k);
-        if (whole) {
-          __nv_bfloat16* dst =
-              p.out + (static_cast<int64_t>(b) * p.heads + tile * 16 + h) * kLatent + d;
+        for (int k = 0; k < 2; ++k) {
+          __nv_bfloat16* dst = p.out + (static_cast<int64_t>(b) * p.heads + tile * 16 + h) * kLatent +
+                               128 * warp + 16 * (2 * cc + k);
 #pragma unroll
           for (int j = 0; j < 16; j += 8) {
             uint32_t w[4];
@@ -938,15 +937,24 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
             }
             *reinterpret_cast<uint4*>(dst + j) = make_uint4(w[0], w[1], w[2], w[3]);
           }
-        } else {
-          float* dst = p.part_o + (static_cast<int64_t>(index) * 16 + h) * kLatent + d;
-#pragma unroll
-          for (int j = 0; j < 16; j += 4)
-            *reinterpret_cast<float4*>(dst + j) =
-                make_float4(o[j][2 * r + k] * f, o[j + 1][2 * r + k] * f,
-                            o[j + 2][2 * r + k] * f, o[j + 3][2 * r + k] * f);
         }
       }
+    } else {
+      // in the order of the fragments, a warp's 512 bytes side by side (by rows, every store
+      // would touch 32 lines: 2000 cycles a segment)
+      float4* dst = reinterpret_cast<float4*>(p.part_o) +
+                    (static_cast<int64_t>(index) * 4 + warp) * 16 * 32 + lane;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float f = r ? f1 : f0;
+            dst[(r * 8 + k * 4 + j / 4) * 32] =
+                make_float4(o[j][2 * r + k] * f, o[j + 1][2 * r + k] * f, o[j + 2][2 * r + k] * f,
+                            o[j + 3][2 * r + k] * f);
+          }
     }
   }
 }
@@ -965,10 +973,12 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p)
   if (w.y == 1) return;  // written by the attention kernel
   __nv_bfloat16* o = p.out + (static_cast<int64_t>(b) * p.heads + h) * kLatent;
   const float* ml = p.part_ml + static_cast<int64_t>(w.x) * 32 + r;
-  const float4* po = reinterpret_cast<const float4*>(
-                         p.part_o + (static_cast<int64_t>(w.x) * 16 + r) * kLatent) + lane;
+  // lane = (k, j / 4, cc): dimensions 128 w + 16 (2 cc + k) + j .. of row r, for the four w
+  const int cc = lane & 3, jk = lane >> 2;
+  const float4* po = reinterpret_cast<const float4*>(p.part_o) +
+                     (static_cast<int64_t>(w.x) * 64 + (r >> 3) * 8 + jk) * 32 + (r & 7) * 4 + cc;
   float M = -INFINITY, L = 0.f;
-  float a[16];  // dimensions 4 lane + 128 k ..
+  float a[16];  // four dimensions of each w
 #pragma unroll
   for (int k = 0; k < 16; ++k) a[k] = 0.f;
   for (int i0 = 0; i0 < w.y; i0 += 32) {  // 32 partials at a time: lane i has the i-th's weight
@@ -991,10 +1001,10 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p)
 #pragma unroll 4
     for (int i = 0; i < min(32, w.y - i0); ++i) {
       const float fi = __shfl_sync(0xffffffffu, f, i);
-      const float4* src = po + static_cast<int64_t>(i0 + i) * (16 * kLatent / 4);
+      const float4* src = po + static_cast<int64_t>(i0 + i) * (16 * kLatent / 4);  // (64 rows of 32)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float4 v = __ldcg(src + 32 * k);
+        const float4 v = __ldcg(src + 16 * 32 * k);
         a[4 * k] = fmaf(fi, v.x, a[4 * k]);
         a[4 * k + 1] = fmaf(fi, v.y, a[4 * k + 1]);
         a[4 * k + 2] = fmaf(fi, v.z, a[4 * k + 2]);
@@ -1007,7 +1017,7 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p)
   for (int k = 0; k < 4; ++k) {
     const __nv_bfloat162 x = __floats2bfloat162_rn(a[4 * k] * inv, a[4 * k + 1] * inv);
     const __nv_bfloat162 y = __floats2bfloat162_rn(a[4 * k + 2] * inv, a[4 * k + 3] * inv);
-    reinterpret_cast<uint2*>(o)[lane + 32 * k] =
+    *reinterpret_cast<uint2*>(o + 128 * k + 16 * (2 * cc + (jk >> 2)) + 4 * (jk & 3)) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
   }
   if (p.lse != nullptr && lane == 0)

@@ -840,11 +840,11 @@ def int8_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
     131072; N: a multiple of 8.  `workspace` (uint8, at least int8_linear_workspace_size bytes)
     saves the allocation; calls that overlap need different ones."""
     xs, ws, dev = x.shape, w_q.shape, x.get_device()
+    N, K = ws if len(ws) == 2 else (1, 0)
     if not (dev >= 0 and x.dtype is _bf16 and w_q.dtype is _i8 and w_scale.dtype is _f32
-            and len(ws) == 2 and w_scale.shape == ws[:1] and w_q.is_contiguous()
-            and w_scale.is_contiguous() and w_q.get_device() == dev
-            and w_scale.get_device() == dev and xs[-1:] == ws[1:] and ws[1] % 16 == 0
-            and ws[1] > 0 and ws[0] % 8 == 0):
+            and K > 0 and not K & 15 and not N & 7 and len(xs) >= 1 and xs[-1] == K
+            and w_scale.shape == (N,) and w_q.is_contiguous() and w_scale.is_contiguous()
+            and w_q.get_device() == dev and w_scale.get_device() == dev):
         _require(x.is_cuda and w_q.is_cuda and w_scale.is_cuda,
                  "int8_linear: x, w_q and w_scale must be CUDA tensors.")
         _require(x.dtype == _bf16, "int8_linear: x must be bfloat16.")
@@ -855,13 +855,12 @@ def int8_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
                  "int8_linear: w_scale must be a contiguous float32 [N] tensor.")
         _require(w_q.device == x.device and w_scale.device == x.device,
                  "int8_linear: x, w_q and w_scale must be on one device.")
-        _require(len(xs) >= 1 and xs[-1] == ws[1],
-                 f"int8_linear: x last dim must match w_q inner dim {ws[1]}.")
-        _require(ws[1] > 0 and ws[1] % 16 == 0,
+        _require(len(xs) >= 1 and xs[-1] == K,
+                 f"int8_linear: x last dim must match w_q inner dim {K}.")
+        _require(K > 0 and K % 16 == 0,
                  "int8_linear: K must be a positive multiple of 16.")
         _require(False, "int8_linear: N must be a multiple of 8.")
-    N, K = ws
-    out = x.new_empty((*xs[:-1], N))
+    out = x.new_empty((xs[0], N) if len(xs) == 2 else (*xs[:-1], N))
     if out.numel() == 0:
         return out
     x2 = _rows_2d(x)
