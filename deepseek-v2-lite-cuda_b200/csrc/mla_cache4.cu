@@ -1078,17 +1078,15 @@ __device__ __forceinline__ int block_rank(bool flag, int* warp_sum, int* total) 
   return base + __popc(m & ((1u << lane) - 1u));
 }
 
-// Result slots j0 .. j0 + 3 (below n) of sequence b take the rows src[j0 ..]: a warp's work, all
-// loads before the stores.  Lanes: 18 16-byte pieces of codes a row, and for the small fields one
+// Result slots j0 .. j0 + 3 of sequence b take the rows t of lanes 0 .. 3 (of lanes 4 .. 7 and so
+// on again; -1: none): a warp's work, all loads before the stores.  Lanes: 18 16-byte pieces of codes a row, and for the small fields one
 // (field, row) each.  In place, rows that stay are skipped: sources lie at or behind the budget
 // and targets before it, so no row is both.
 constexpr int kMoveRows = 4;
-__device__ __forceinline__ void move_rows(const Cache& s, const Cache& d, int b, int j0, int n,
-                                          const int32_t* src, bool in_place) {
+__device__ __forceinline__ void move_rows(const Cache& s, const Cache& d, int b, int j0, int t,
+                                          bool in_place) {
   const int lane = threadIdx.x & 31;
   const int mine = lane & 3;
-  int t = -1;
-  if (j0 + mine < n) t = __ldcg(src + j0 + mine);
   if (in_place && t == j0 + mine) t = -1;
   uint4 v[3];
 #pragma unroll
@@ -1126,15 +1124,8 @@ __device__ __forceinline__ void move_rows(const Cache& s, const Cache& d, int b,
   }
 }
 
-// Sum of v over the block (1024 threads); `red`: 32 words, not in use by an earlier call any more
-// (callers alternate between two).
-__device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t* red) {
-  const uint32_t w = __reduce_add_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = w;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, red[threadIdx.x & 31]);
-}
-// Exclusive prefix of v over the block's threads.
+// Exclusive prefix of v over the block's threads (1024); `red`: 32 words that no earlier call in
+// flight uses.
 __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t incl = v;
@@ -1149,123 +1140,151 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* red) {
   return before + incl - v;
 }
 
+// One round of the search: a1, a2, a3 keys are at or above v + 1, 2, 3 << shift; the largest of
+// the four bounds that `want` keys reach becomes v, and the range what lies up to the next.
+__device__ __forceinline__ void narrow(int want, int shift, int a1, int a2, int a3, uint32_t* v,
+                                       int* in_range, int* over_end) {
+  if (a3 >= want) {
+    *v |= 3u << shift;
+    *in_range = a3 - *over_end;
+  } else if (a2 >= want) {
+    *v |= 2u << shift;
+    *in_range = a2 - a3;
+    *over_end = a3;
+  } else if (a1 >= want) {
+    *v |= 1u << shift;
+    *in_range = a1 - a2;
+    *over_end = a2;
+  } else {
+    *in_range += *over_end - a1;
+    *over_end = a1;
+  }
+}
+// The same among n <= kFewKeys keys of a list, by the block's first four warps, four keys a lane;
+// returns the value with v's bits completed.
+constexpr int kFewKeys = 512;
+__device__ __forceinline__ uint32_t find_in_list(const uint32_t* list, int n, int want, int shift,
+                                                 uint32_t v, uint32_t (*part)[4]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t k[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k[i] = threadIdx.x + 128 * i < n ? list[threadIdx.x + 128 * i] : 0u;
+#pragma unroll 1
+  for (int round = 0; shift >= 0; shift -= 2, ++round) {
+    const uint32_t c1 = v | (1u << shift), c2 = v | (2u << shift), c3 = v | (3u << shift);
+    uint32_t x = 0;  // three counts of 10 bits
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x += (k[i] >= c1 ? 1u : 0u) + (k[i] >= c2 ? 1u << 10 : 0u) + (k[i] >= c3 ? 1u << 20 : 0u);
+    x = __reduce_add_sync(0xffffffffu, x);
+    if (lane == 0) part[round & 1][warp] = x;
+    ptx::named_bar_sync(1, 128);
+    const uint4 y = *reinterpret_cast<const uint4*>(part[round & 1]);
+    x = (y.x + y.y) + (y.z + y.w);
+    if (static_cast<int>(x >> 20) >= want) v = c3;
+    else if (static_cast<int>((x >> 10) & 1023u) >= want) v = c2;
+    else if (static_cast<int>(x & 1023u) >= want) v = c1;
+  }
+  return v;
+}
+
 // One block per sequence: which slots stay, and src_of[b, j] = the slot whose row result slot j
 // takes: itself where slot j < budget stays, else the next survivor from behind the budget,
 // both in ascending order.  Up to 1024 * IPT slots, whose keys stay in registers (thread i has
-// slots IPT i ..): the budget-th largest key is found two bits a round, by counting the keys at
-// or above three candidates, so no histogram's atomics collide however alike the weights are
-// (four 8-bit histogram passes: 23 us for 333 slots and 68 us for 8192; this: see evict_plan_long).
-// `rows_here`: the block moves the rows itself.
+// slots IPT i ..).  The budget-th largest key is found two bits a round, by counting the keys at
+// or above three candidates: no histogram, whose atomics collide when weights are alike (four
+// passes of 8 bits took 23 us for 333 slots and 68 us for 8192).  A round of the whole block
+// takes 450 cycles and 100 a key of a thread, so once kFewKeys or fewer keys share the bits found
+// so far, they go to shared memory and four warps find the rest (one warp took 500 a round, and
+// counting the keys before each key, n^2 comparisons, 10800 for 333).
+// `rows_here` (budget <= kRowsHere): the block moves the rows itself.
+constexpr int kRowsHere = 256;
+constexpr int kSharedPlan = 2048;  // budgets whose lists fit shared memory
 template <int IPT>
 __global__ void __launch_bounds__(1024)
     evict_plan_kernel(Cache c, Cache dst, int budget, int recent, int32_t* __restrict__ src_of,
                       int32_t* __restrict__ holes, int rows_here, int in_place) {
   __shared__ uint32_t red[6][32];
-  __shared__ uint32_t list[IPT == 1 ? 1 : 1024];
+  __shared__ uint32_t list[kFewKeys];
+  __shared__ int32_t src_s[kSharedPlan], hole_s[kSharedPlan];
+  __shared__ uint32_t found;
+  __shared__ __align__(16) uint32_t part[2][4];
   ptx::pdl_launch_dependents();
-  const int b = blockIdx.x;
-  const int len = min(max(c.state[b], 0), c.slots), next = c.state[c.batch + b];
-  int32_t* src = src_of + static_cast<int64_t>(b) * budget;
-  int32_t* hole = holes + static_cast<int64_t>(b) * budget;
-  const int kept_n = min(len, budget);
+  const int b = blockIdx.x, lane = threadIdx.x & 31;
   const int t0 = threadIdx.x * IPT;
+  // weights and positions are on their way while the lengths are read
+  const float* mass = c.mass + static_cast<int64_t>(b) * c.slots;
+  const int32_t* pos = c.pos + static_cast<int64_t>(b) * c.slots;
+  float m[IPT];
+  int ps[IPT];
+  if (IPT >= 4) {
+#pragma unroll
+    for (int i = 0; i < IPT; i += 4)
+      if (t0 + i < c.slots) {  // (slots are a multiple of 64)
+        *reinterpret_cast<float4*>(m + i) = *reinterpret_cast<const float4*>(mass + t0 + i);
+        *reinterpret_cast<int4*>(ps + i) = *reinterpret_cast<const int4*>(pos + t0 + i);
+      }
+  } else if (t0 < c.slots) {
+    m[0] = mass[t0];
+    ps[0] = pos[t0];
+  }
+  const int len = min(max(c.state[b], 0), c.slots), next = c.state[c.batch + b];
+  int32_t* const out = src_of + static_cast<int64_t>(b) * budget;
+  const bool shared = budget <= kSharedPlan;
+  int32_t* src = shared ? src_s : out;
+  int32_t* hole = shared ? hole_s : holes + static_cast<int64_t>(b) * budget;
+  const int kept_n = min(len, budget);
   if (len > budget) {
-    const float* mass = c.mass + static_cast<int64_t>(b) * c.slots;
-    const int32_t* pos = c.pos + static_cast<int64_t>(b) * c.slots;
     const int from = next - recent;
     uint32_t key[IPT];
 #pragma unroll
-    for (int i = 0; i < IPT; ++i) key[i] = 0u;
-    if (IPT >= 4) {
-#pragma unroll
-      for (int i = 0; i < IPT; i += 4)
-        if (t0 + i < c.slots) {  // (slots are a multiple of 64)
-          const float4 m = *reinterpret_cast<const float4*>(mass + t0 + i);
-          const int4 p = *reinterpret_cast<const int4*>(pos + t0 + i);
-          key[i] = evict_key(m.x, p.x, from);
-          key[i + (IPT > 1 ? 1 : 0)] = evict_key(m.y, p.y, from);
-          key[i + (IPT > 2 ? 2 : 0)] = evict_key(m.z, p.z, from);
-          key[i + (IPT > 3 ? 3 : 0)] = evict_key(m.w, p.w, from);
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < IPT; ++i)
-        if (t0 + i < len) key[i] = evict_key(mass[t0 + i], pos[t0 + i], from);
-    }
-#pragma unroll
-    for (int i = 0; i < IPT; ++i)
-      if (t0 + i >= len) key[i] = 0u;  // below every candidate
+    for (int i = 0; i < IPT; ++i)  // slots behind the last: 0, below every candidate
+      key[i] = t0 + i < len ? evict_key(m[i], ps[i], from) : 0u;
     // the largest v with at least `budget` keys >= v
     uint32_t v = 0;
-    int want = budget;          // keys still to be found among those that are compared
-    uint32_t one = 0;           // this thread's key once 1024 or fewer can still decide
-    bool few = IPT == 1;
-    if (IPT == 1) one = key[0];
-    uint32_t in_range = len;    // keys in [v, v + 2^(shift + 2)) before a round ...
-    uint32_t over_end = 0;      // ... and at or above its end, of those compared
+    int in_range = len;  // keys in [v, v + 2^(shift + 2)) before a round ...
+    int over_end = 0;    // ... and at or above its end
+    int shift = 30;
 #pragma unroll 1
-    for (int shift = 30, round = 0; shift >= 0; shift -= 2, ++round) {
-      if (IPT > 1 && !few && in_range <= 1024 && shift < 30) {
-        // the keys that share v's upper bits, one to a thread; those above them are counted off
-        few = true;
-        const uint32_t top = v >> (shift + 2);
-        uint32_t mine = 0, over = 0;
-#pragma unroll
-        for (int i = 0; i < IPT; ++i) {
-          mine += (key[i] >> (shift + 2)) == top && t0 + i < len ? 1u : 0u;
-          over += (key[i] >> (shift + 2)) > top ? 1u : 0u;
-        }
-        uint32_t at = block_prefix(mine, red[4]);
-        want -= static_cast<int>(block_sum(over, red[5]));
-        over_end = 0;
-#pragma unroll
-        for (int i = 0; i < IPT; ++i)
-          if ((key[i] >> (shift + 2)) == top && t0 + i < len) list[at++] = key[i];
-        __syncthreads();
-        one = threadIdx.x < in_range ? list[threadIdx.x] : 0u;
-      }
+    for (int round = 0; shift >= 0 && in_range > kFewKeys; shift -= 2, ++round) {
       uint32_t n12 = 0, n3 = 0;
       const uint32_t c1 = v | (1u << shift), c2 = v | (2u << shift), c3 = v | (3u << shift);
-      if (few) {
-        n12 = (one >= c1 ? 1u : 0u) + (one >= c2 ? 0x10000u : 0u);
-        n3 = one >= c3 ? 1u : 0u;
-      } else {
 #pragma unroll
-        for (int i = 0; i < IPT; ++i) {
-          n12 += (key[i] >= c1 ? 1u : 0u) + (key[i] >= c2 ? 0x10000u : 0u);
-          n3 += key[i] >= c3 ? 1u : 0u;
-        }
+      for (int i = 0; i < IPT; ++i) {
+        n12 += (key[i] >= c1 ? 1u : 0u) + (key[i] >= c2 ? 0x10000u : 0u);
+        n3 += key[i] >= c3 ? 1u : 0u;
       }
       // a block has at most 32768 keys: two counts to a word
       const uint32_t w12 = __reduce_add_sync(0xffffffffu, n12);
       const uint32_t w3 = __reduce_add_sync(0xffffffffu, n3);
       uint32_t* r = red[2 * (round & 1)];
-      if ((threadIdx.x & 31) == 0) {
+      if (lane == 0) {
         r[threadIdx.x >> 5] = w12;
         r[32 + (threadIdx.x >> 5)] = w3;
       }
       __syncthreads();
-      const uint32_t s12 = __reduce_add_sync(0xffffffffu, r[threadIdx.x & 31]);
-      const int n1 = static_cast<int>(s12 & 0xFFFFu), n2 = static_cast<int>(s12 >> 16);
-      const int nn3 = static_cast<int>(__reduce_add_sync(0xffffffffu, r[32 + (threadIdx.x & 31)]));
-      // (the keys at or above the bucket's end were counted by the round before: only the counts
-      // inside it matter for in_range)
-      const int above_v = static_cast<int>(over_end);
-      if (nn3 >= want) {
-        v = c3;
-        in_range = nn3 - above_v;
-      } else if (n2 >= want) {
-        v = c2;
-        in_range = n2 - nn3;
-        over_end = nn3;
-      } else if (n1 >= want) {
-        v = c1;
-        in_range = n1 - n2;
-        over_end = n2;
-      } else {
-        in_range = in_range + above_v - n1;
-        over_end = n1;
+      const uint32_t s12 = __reduce_add_sync(0xffffffffu, r[lane]);
+      const int a1 = static_cast<int>(s12 & 0xFFFFu), a2 = static_cast<int>(s12 >> 16);
+      const int a3 = static_cast<int>(__reduce_add_sync(0xffffffffu, r[32 + lane]));
+      narrow(budget, shift, a1, a2, a3, &v, &in_range, &over_end);
+    }
+    if (shift >= 0) {  // the rest by one warp: the keys in range, the others counted
+      uint32_t mine = 0;
+#pragma unroll
+      for (int i = 0; i < IPT; ++i)
+        mine += t0 + i < len && (shift == 30 || (key[i] >> (shift + 2)) == (v >> (shift + 2))) ? 1u : 0u;
+      uint32_t at = block_prefix(mine, red[4]);
+#pragma unroll
+      for (int i = 0; i < IPT; ++i)
+        if (t0 + i < len && (shift == 30 || (key[i] >> (shift + 2)) == (v >> (shift + 2))))
+          list[at++] = key[i];
+      __syncthreads();
+      if (threadIdx.x < 128) {
+        const uint32_t f = find_in_list(list, in_range, budget - over_end, shift, v, part);
+        if (threadIdx.x == 0) found = f;
       }
+      __syncthreads();
+      v = found;
     }
     uint32_t above = 0, ties = 0;
 #pragma unroll
@@ -1273,9 +1292,14 @@ __global__ void __launch_bounds__(1024)
       above += key[i] > v ? 1u : 0u;
       ties += key[i] == v && t0 + i < len ? 1u : 0u;
     }
-    // (the last round left red[2..3] in use: 15 is odd)
-    const uint32_t need = budget - block_sum(above, red[0]);  // ties that stay: the first ones
-    uint32_t rank = block_prefix(ties, red[1]);
+    // ties that stay: the first ones (both counts are at most 32768)
+    const uint32_t packed = above | (ties << 16);
+    const uint32_t before_t = block_prefix(packed, red[5]);
+    uint32_t rank = before_t >> 16;
+    // the last warp's last thread ends the prefix: the block's total of `above`
+    if (threadIdx.x == 1023) list[0] = (before_t + packed) & 0xFFFFu;
+    __syncthreads();
+    const uint32_t need = budget - list[0];
     uint32_t keep = 0, n_hole = 0, n_late = 0;
 #pragma unroll
     for (int i = 0; i < IPT; ++i) {
@@ -1286,7 +1310,7 @@ __global__ void __launch_bounds__(1024)
       n_hole += t < budget && !k ? 1u : 0u;
       n_late += t >= budget && k ? 1u : 0u;
     }
-    const uint32_t before = block_prefix(n_hole | (n_late << 16), red[2]);
+    const uint32_t before = block_prefix(n_hole | (n_late << 16), red[4]);
     uint32_t h = before & 0xFFFFu, l = before >> 16;
 #pragma unroll
     for (int i = 0; i < IPT; ++i) {
@@ -1304,8 +1328,12 @@ __global__ void __launch_bounds__(1024)
   }
   __syncthreads();
   if (rows_here)
-    for (int j = (threadIdx.x >> 5) * kMoveRows; j < kept_n; j += 32 * kMoveRows)
-      move_rows(c, dst, b, j, kept_n, src, in_place != 0);
+    for (int j = (threadIdx.x >> 5) * kMoveRows; j < kept_n; j += 32 * kMoveRows) {
+      const int k = j + (lane & 3);
+      move_rows(c, dst, b, j, k < kept_n ? src_s[k] : -1, in_place != 0);
+    }
+  else if (shared)
+    for (int j = threadIdx.x; j < kept_n; j += 1024) out[j] = src_s[j];
   if (threadIdx.x == 0) {
     dst.state[b] = kept_n;
     dst.state[c.batch + b] = next;
@@ -1397,7 +1425,10 @@ __global__ void __launch_bounds__(256)
   const int b = blockIdx.y;
   const int j = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kMoveRows;
   const int n = __ldcg(d.state + b);
-  if (j < n) move_rows(s, d, b, j, n, src_of + static_cast<int64_t>(b) * budget, in_place != 0);
+  if (j >= n) return;
+  const int k = j + (threadIdx.x & 3);
+  move_rows(s, d, b, j, k < n ? __ldcg(src_of + static_cast<int64_t>(b) * budget + k) : -1,
+            in_place != 0);
 }
 
 Cache cache_of(void* codes, void* scales, float* rstd, int32_t* pos, float* mass, int32_t* state,
@@ -1473,7 +1504,7 @@ int launch_append(const Cache& c, const void* lat, int64_t lat_ld, const void* k
 int launch_evict(const Cache& s, const Cache& d, int budget, int recent, bool in_place,
                  int32_t* src_of, int32_t* holes, cudaStream_t st) {
   // few rows: the planning block moves them (no second launch); many: all SMs do
-  const int here = budget <= 256 ? 1 : 0;
+  const int here = budget <= kRowsHere ? 1 : 0;
   if (s.slots <= 1024)
     evict_plan_kernel<1><<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes, here,
                                                    in_place);
