@@ -389,7 +389,7 @@ __device__ __forceinline__ int frag_slot(int pos) {
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -431,29 +431,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds_u2(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint4 lds_u4(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(a));
-  return v;
-}
-__device__ __forceinline__ float4 lds_f4(uint32_t a) {
-  const uint4 v = lds_u4(a);
-  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z),
-                     __uint_as_float(v.w));
-}
-
 // Sums of u and v over the block (kAttnThreads threads); `red`: 8 words that no earlier call in
 // flight uses (callers alternate between two).
 __device__ __forceinline__ int2 block_add(int u, int v, int* red) {
@@ -534,7 +511,6 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
   const Cache& c = p.c;
   AttnSmall& sm = *reinterpret_cast<AttnSmall*>(smem + kOffSmall);
   const uint32_t s0 = ptx::smem_u32(smem);
-  const uint32_t sQ = s0 + kOffQ, sP = s0 + kOffP;
   const uint32_t bar0 = ptx::smem_u32(sm.bar);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, cc = lane & 3;  // fragment row (or column) and column pair
@@ -672,8 +648,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
       const int t0 = (c0 + i) * kChunk;
       const bool ok = ptx::mbar_wait(bar0 + 8 * (it & 1), (it >> 1) & 1, &sm.abort_flag, p.status,
                                      kTimeoutCycles, DS_ERR_TIMEOUT);
-      const uint32_t st = s0 + (it & 1) * kStageBytes;
-      const uint32_t sFac = s0 + kOffFac + (it & 1) * kFacBytes;
+      const uint8_t* st = smem + (it & 1) * kStageBytes;
+      float* fac = reinterpret_cast<float*>(smem + kOffFac + (it & 1) * kFacBytes);
       const bool more = i + 1 < seg;
       if (more) nf = load_factors(c, b, t0 + kChunk + threadIdx.x, len);
       // ---- S: this warp's 32 slots (four blocks of 8 columns) against 16 heads
@@ -685,9 +661,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
       {
         // column n = g of block k: slot T(g / 2, g & 1 | 2 (k & 1)) of 16-slot group 2 warp + k / 2
         const int te = (((g >> 1) ^ (2 * (g & 1))) + 4 * (g & 1)) + warp * 32;
-        const uint32_t base = st + te * kRowBytes + cc * 8;
-        const uint32_t q0 = sQ + g * kQLd + cc * 16;
-        const uint32_t fac0 = sFac + (warp * 32 + 4 * cc) * 4;
+        const uint8_t* base = st + te * kRowBytes + cc * 8;
+        const uint8_t* q0 = smem + kOffQ + g * kQLd + cc * 16;
+        const float* fac0 = fac + warp * 32 + 4 * cc;
 #pragma unroll 1
         for (int gr = 0; gr < kGroups; ++gr) {
           float acc[4][4];
@@ -702,9 +678,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
             uint4 a[4];
             uint2 x[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = lds_u2(base + (k * 8) * kRowBytes + qd * 32);
+            for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint2*>(base + (k * 8) * kRowBytes + qd * 32);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) a[s] = lds_u4(q0 + qd * 256 + s * 64);
+            for (int s = 0; s < 4; ++s) a[s] = *reinterpret_cast<const uint4*>(q0 + qd * 256 + s * 64);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint32_t v[4], w[4];
@@ -718,7 +694,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // the group is complete: times its slots' factors
-            const float2 f = lds_f2(fac0 + (gr * kChunk + (k >> 1) * 16 + 2 * (k & 1)) * 4);
+            const float2 f = *reinterpret_cast<const float2*>(fac0 + gr * kChunk + (k >> 1) * 16 + 2 * (k & 1));
             sc[k][0] = fmaf(acc[k][0], f.x, sc[k][0]);
             sc[k][1] = fmaf(acc[k][1], f.y, sc[k][1]);
             sc[k][2] = fmaf(acc[k][2], f.x, sc[k][2]);
@@ -827,8 +803,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
       __syncthreads();  // barrier B: P and the next chunk's factors are there
       // ---- O += P V over the 128 dimensions of group `warp`
       {
-        const uint32_t fw = sFac + warp * kChunk * 4;
-        const float4 fl = lds_f4(fw + lane * 16);
+        float* fw = fac + warp * kChunk;
+        const float4 fl = reinterpret_cast<const float4*>(fw)[lane];
         float fm = fmaxf(fmaxf(fl.x, fl.y), fmaxf(fl.z, fl.w));
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) fm = fmaxf(fm, __shfl_xor_sync(0xffffffffu, fm, d));
@@ -846,22 +822,22 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
         }
         // this group's factors, scaled, back in place: no other warp reads them any more
         __syncwarp();
-        *reinterpret_cast<float4*>(smem + (fw - s0) + lane * 16) =
+        reinterpret_cast<float4*>(fw)[lane] =
             make_float4(fl.x * pscale, fl.y * pscale, fl.z * pscale, fl.w * pscale);
         __syncwarp();
         // B: slots T(cc, 0..3) of the 16, dimensions 128 warp + 16 g + 0..15
-        const uint32_t v0 = st + cc * kRowBytes + warp * 64 + g * 8;
-        const uint32_t v1 = st + ((cc ^ 2) + 4) * kRowBytes + warp * 64 + g * 8;
-        const uint32_t pr = sP + (g * kPLd + 4 * cc) * 4;
+        const uint8_t* v0 = st + cc * kRowBytes + warp * 64 + g * 8;
+        const uint8_t* v1 = st + ((cc ^ 2) + 4) * kRowBytes + warp * 64 + g * 8;
+        const float* pr = reinterpret_cast<const float*>(smem + kOffP) + g * kPLd + 4 * cc;
 #pragma unroll 2
         for (int kk = 0; kk < 8; ++kk) {
-          const float4 p0 = lds_f4(pr + kk * 64);
-          const float4 p1 = lds_f4(pr + 8 * kPLd * 4 + kk * 64);
-          const float4 f = lds_f4(fw + (kk * 16 + 4 * cc) * 4);
-          const uint2 x0 = lds_u2(v0 + (kk * 16) * kRowBytes);
-          const uint2 x1 = lds_u2(v1 + (kk * 16) * kRowBytes);
-          const uint2 x2 = lds_u2(v0 + (kk * 16 + 8) * kRowBytes);
-          const uint2 x3 = lds_u2(v1 + (kk * 16 + 8) * kRowBytes);
+          const float4 p0 = *reinterpret_cast<const float4*>(pr + kk * 16);
+          const float4 p1 = *reinterpret_cast<const float4*>(pr + 8 * kPLd + kk * 16);
+          const float4 f = *reinterpret_cast<const float4*>(fw + kk * 16 + 4 * cc);
+          const uint2 x0 = *reinterpret_cast<const uint2*>(v0 + (kk * 16) * kRowBytes);
+          const uint2 x1 = *reinterpret_cast<const uint2*>(v1 + (kk * 16) * kRowBytes);
+          const uint2 x2 = *reinterpret_cast<const uint2*>(v0 + (kk * 16 + 8) * kRowBytes);
+          const uint2 x3 = *reinterpret_cast<const uint2*>(v1 + (kk * 16 + 8) * kRowBytes);
           const uint32_t a0 = pack_f16(p0.x * f.x, p0.y * f.y), a1 = pack_f16(p1.x * f.x, p1.y * f.y);
           const uint32_t a2 = pack_f16(p0.z * f.z, p0.w * f.w), a3 = pack_f16(p1.z * f.z, p1.w * f.w);
 #pragma unroll
