@@ -4,8 +4,9 @@ Same function names, argument names, defaults and return conventions as the refe
 binding (src/kernels/bindings.cu:186-301): `moe_routing`, `moe_scan`, `moe_dispatch`,
 `moe_combine`, `swiglu`, `moe_gemm1`, `moe_gemm2`, `rms_norm`, `kv_upproj`, `rope`,
 `run_hello`; plus the additive ops `moe_gemm1_swiglu`, `moe_layer_fused` /
-`moe_layer_forward` / `moe_layer_forward_from_x`, the layer stages and the expert-parallel
-entry points.
+`moe_layer_forward` / `moe_layer_forward_from_x`, the layer stages, the expert-parallel entry
+points, and the quantised decode path: `int8_quantize`, `int8_linear`, `mla_cache4_append` /
+`_get` / `_evict` / `_reset`, `mla_decode_attention4`, `mla_decode4_step`.
 
 Every op validates its tensors with the reference's messages (raising RuntimeError, as
 TORCH_CHECK does), allocates outputs with torch on the input's device, and calls the
@@ -784,6 +785,7 @@ def mla_decode_step(x: torch.Tensor, w_dec: torch.Tensor, w_out: torch.Tensor, c
 # ---------------------------------------------------------------------- 8-bit integer linear
 # These operators run for a few microseconds, so a good call pays one test of everything it
 # needs; only a call that fails it looks for the first fault and its message.
+_compiling = torch.compiler.is_compiling
 _bf16, _i8, _i32, _u8, _f32 = (torch.bfloat16, torch.int8, torch.int32, torch.uint8, torch.float32)
 
 
@@ -793,6 +795,8 @@ def int8_quantize(x: torch.Tensor) -> List[torch.Tensor]:
     scale = a / 127.  A row of zeros gives zeros and scale 0; a row with an infinity or a NaN
     gives zeros and scale NaN.  Weights [N, K] are quantised per output channel the same way.
     K: a multiple of 16."""
+    if _compiling():
+        return list(torch.ops.ds_kernels.int8_quantize(x))
     if not (x.is_cuda and x.dtype is _bf16 and x.dim() >= 1 and x.shape[-1] > 0
             and x.shape[-1] % 16 == 0):
         _require(x.is_cuda, "int8_quantize: x must be a CUDA tensor.")
@@ -839,6 +843,8 @@ def int8_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
     (32 bits) and scaled once: bf16(acc * (scale_row * w_scale)).  K: a multiple of 16, at most
     131072; N: a multiple of 8.  `workspace` (uint8, at least int8_linear_workspace_size bytes)
     saves the allocation; calls that overlap need different ones."""
+    if _compiling():
+        return torch.ops.ds_kernels.int8_linear(x, w_q, w_scale)
     xs, ws, dev = x.shape, w_q.shape, x.get_device()
     N, K = ws if len(ws) == 2 else (1, 0)
     if not (dev >= 0 and x.dtype is _bf16 and w_q.dtype is _i8 and w_scale.dtype is _f32

@@ -8,7 +8,7 @@ gives the output shapes and dtypes from the input shapes alone:
 
     moe_routing  moe_scan  moe_dispatch  moe_combine  swiglu  moe_gemm1  moe_gemm2
     rms_norm  kv_upproj  rope
-    (additive) moe_gemm1_swiglu  rms_norm_residual  moe_layer_fused
+    (additive) moe_gemm1_swiglu  rms_norm_residual  moe_layer_fused  int8_quantize  int8_linear
 
 The real kernel of each operator is the eager function of the same name in `ds_kernels`
 (the C-ABI call of libds_kernels_sm100.so through ctypes), so the two produce the same
@@ -175,6 +175,27 @@ def _(hidden_states, gate_weight, packed_w1, w2, shared_w1=None, shared_w2=None,
     return torch.empty_like(hidden_states)
 
 
+@torch.library.custom_op(f"{_NS}::int8_quantize", mutates_args=())
+def int8_quantize(x: Tensor) -> Tuple[Tensor, Tensor]:
+    q, scale = _k.int8_quantize(x)
+    return q, scale
+
+
+@int8_quantize.register_fake
+def _(x):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::int8_linear", mutates_args=())
+def int8_linear(x: Tensor, w_q: Tensor, w_scale: Tensor) -> Tensor:
+    return _k.int8_linear(x, w_q, w_scale)
+
+
+@int8_linear.register_fake
+def _(x, w_q, w_scale):
+    return x.new_empty((*x.shape[:-1], w_q.shape[0]))
+
+
 OPS = ("moe_routing", "moe_scan", "moe_dispatch", "moe_combine", "swiglu", "moe_gemm1",
        "moe_gemm2", "rms_norm", "kv_upproj", "rope", "moe_gemm1_swiglu", "rms_norm_residual",
-       "moe_layer_fused")
+       "moe_layer_fused", "int8_quantize", "int8_linear")

@@ -371,6 +371,21 @@ def test_evict(kind, lens, budget, recent, in_place):
         assert cache.lens.tolist() == lens
 
 
+@pytest.mark.parametrize("kind", ["random", "ties", "equal"])
+@pytest.mark.parametrize("lens,budget,recent", [([9000, 20000, 3000], 3000, 64), ([32768, 2049], 2048, 0),
+                                                ([8192, 8191], 8191, 8191), ([1024, 600], 300, 17)])
+def test_evict_sizes_of_every_kernel(kind, lens, budget, recent):
+    b = len(lens)
+    cache, _ = random_cache(b, max(lens), lens, budget)
+    cache.mass.copy_(masses(kind, b, cache.slots, budget))
+    mass, pos, codes = cache.mass.cpu().clone(), cache.pos.cpu().clone(), cache.codes.cpu().clone()
+    ds_kernels.mla_cache4_evict(cache, budget, recent)
+    for i, n in enumerate(lens):
+        src = evict_ref(mass[i], pos[i].tolist(), n, n, budget, recent)
+        assert cache.pos[i, :len(src)].cpu().tolist() == pos[i][src].tolist()
+        assert torch.equal(cache.codes[i, :len(src)].cpu(), codes[i][src])
+
+
 def test_evict_long():
     cache, _ = random_cache(2, 40000, [40000, 39999], 3)
     cache.mass.copy_(masses("random", 2, cache.slots, 1))

@@ -168,3 +168,17 @@ def test_other_stream_own_workspace_and_graph_replay():
         static.copy_(y)
         graph.replay()
         assert torch.equal(out, ds_kernels.int8_linear(y, w, ws))
+
+
+def test_custom_operators():
+    x, (w, ws) = rows(7, 64, 15).cuda(), weights(24, 64, 16)
+    w, ws = w.cuda(), ws.cuda()
+    torch.library.opcheck(torch.ops.ds_kernels.int8_quantize.default, (x,))
+    torch.library.opcheck(torch.ops.ds_kernels.int8_linear.default, (x, w, ws))
+
+    def f(x):
+        q, s = ds_kernels.int8_quantize(x)
+        return ds_kernels.int8_linear(x, w, ws) * 2, q, s
+
+    for got, want in zip(torch.compile(f, fullgraph=True)(x), f(x)):
+        assert torch.equal(got, want)
