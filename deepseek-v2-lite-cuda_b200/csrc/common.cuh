@@ -56,6 +56,31 @@ cudaError_t launch_pdl(void (*kernel)(ExpT...), dim3 grid, dim3 block, size_t sm
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<ActT&&>(args)...);
 }
 
+// Launch `kernel` so that its CTAs may be set up while the stream's last kernel still runs (always
+// with the programmatic-serialization attribute; cluster > 1: in clusters of that many CTAs).  The
+// kernel waits (ptx::pdl_wait) before its first access to global memory, in at least one CTA
+// whatever its work, and only then lets the next one in (ptx::pdl_launch_dependents): so all
+// that lies before it in the stream is complete, whoever launched it.
+template <typename... ExpT, typename... ActT>
+cudaError_t launch_chained(void (*kernel)(ExpT...), dim3 grid, dim3 block, size_t smem,
+                           cudaStream_t s, int cluster, ActT&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<ActT&&>(args)...);
+}
+
 // Device status word (one per device, lives in this library's module).
 int* device_status_ptr();
 

@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(256)
     quantize_kernel(const uint4* __restrict__ x, int64_t ld8, int rows, int k8,
                     uint2* __restrict__ q, float* __restrict__ scale) {
   __shared__ uint32_t red[8];
+  ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const int row = TPR == 32 ? static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5)
                             : static_cast<int>(blockIdx.x);
@@ -225,6 +226,9 @@ __global__ void __launch_bounds__(kFewThreads)
   ptx::tc_fence_after();
   const uint32_t tmem = *holder;
   const int pre = min(nkb, kFewStages);
+  // (not QUANT: quantize_kernel lets this one in once all before it is complete, so the weights
+  // may be read at once, and the quantised rows after the wait)
+  if (QUANT) ptx::pdl_wait();
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < pre; ++i) {
       ptx::mbar_arrive_expect_tx(full0 + 8 * i, kStage);
@@ -367,6 +371,7 @@ __global__ void __launch_bounds__(kFewThreads)
     ptx::tmem_dealloc(tmem, T::tmem_cols);
   }
   if (!QUANT) ptx::pdl_wait();  // the rows' scales
+  ptx::pdl_launch_dependents();
   if (!ok) return;
   // 16 threads a row, 8 channels each
   const int r0 = rank * per, rn = min(mrows, r0 + per) - r0;
@@ -445,6 +450,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     ptx::tmem_relinquish_pair();
   }
   ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
   ptx::tc_fence_before();
   __syncwarp();
   ptx::cluster_sync();  // both CTAs' barriers are set up before either signals the other's
@@ -708,21 +714,9 @@ int launch_few(const void* x, int64_t ld, const void* a, const float* sa, const 
   few_splits(tiles * mt, p.k_blocks, di.num_sms, &p.splits, &p.kb_per_split);
   p.status = device_status_ptr();
   if (p.status == nullptr) return fail(DS_ERR_CUDA, "device status word unavailable");
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(tiles * p.splits, mt);
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = QUANT ? FewTile<NT>::smem_quant(p.kb_per_split) : FewTile<NT>::smem;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = QUANT ? 1 : 2;
-  DS_CUDA(cudaLaunchKernelEx(&cfg, few_rows_kernel<NT, QUANT>, tmW, tmX, p));
+  DS_CUDA(launch_chained(few_rows_kernel<NT, QUANT>, dim3(tiles * p.splits, mt), dim3(kFewThreads),
+                         QUANT ? FewTile<NT>::smem_quant(p.kb_per_split) : FewTile<NT>::smem, s,
+                         p.splits, tmW, tmX, p));
   return DS_OK;
 }
 
@@ -744,21 +738,8 @@ int launch_many(const void* a, const float* sa, const void* w, const float* sw, 
   p.tiles = static_cast<int>(tiles);
   p.status = device_status_ptr();
   if (p.status == nullptr) return fail(DS_ERR_CUDA, "device status word unavailable");
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(2 * std::min(p.tiles, g_pairs[di.device]));
-  cfg.blockDim = dim3(kManyThreads);
-  cfg.dynamicSmemBytes = kManySmem;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  DS_CUDA(cudaLaunchKernelEx(&cfg, many_rows_kernel, tmX, tmW, tmO, p));
+  DS_CUDA(launch_chained(many_rows_kernel, dim3(2 * std::min(p.tiles, g_pairs[di.device])),
+                         dim3(kManyThreads), kManySmem, s, 2, tmX, tmW, tmO, p));
   return DS_OK;
 }
 
@@ -780,12 +761,16 @@ int launch_quantize(const void* x, int64_t ld, int64_t rows, int K, void* q, flo
   const int k8 = K / 8, n = static_cast<int>(rows);
   const unsigned r = static_cast<unsigned>(rows), r8 = static_cast<unsigned>((rows + 7) / 8);
   if (rows >= 1024 && k8 <= 256) {  // a warp a row once there are rows enough to fill the SMs
-    if (k8 <= 128) quantize_kernel<32, 4><<<r8, 256, 0, s>>>(src, ld / 8, n, k8, dst, scale);
-    else quantize_kernel<32, 8><<<r8, 256, 0, s>>>(src, ld / 8, n, k8, dst, scale);
+    if (k8 <= 128) DS_CUDA(launch_chained(quantize_kernel<32, 4>, dim3(r8), dim3(256), 0, s, 1, src, ld / 8, n, k8,
+                           dst, scale));
+    else DS_CUDA(launch_chained(quantize_kernel<32, 8>, dim3(r8), dim3(256), 0, s, 1, src, ld / 8, n, k8,
+                           dst, scale));
   } else if (k8 <= 256) {
-    quantize_kernel<256, 1><<<r, 256, 0, s>>>(src, ld / 8, n, k8, dst, scale);
+    DS_CUDA(launch_chained(quantize_kernel<256, 1>, dim3(r), dim3(256), 0, s, 1, src, ld / 8, n, k8,
+                           dst, scale));
   } else {
-    quantize_kernel<256, 4><<<r, 256, 0, s>>>(src, ld / 8, n, k8, dst, scale);
+    DS_CUDA(launch_chained(quantize_kernel<256, 4>, dim3(r), dim3(256), 0, s, 1, src, ld / 8, n, k8,
+                           dst, scale));
   }
   DS_LAUNCH_CHECK("quantize_kernel");
   return DS_OK;

@@ -189,6 +189,8 @@ __global__ void __launch_bounds__(1024)
                   int table_rows, float eps) {
   const int b = blockIdx.y;
   const int i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
   Token tok{};
   if (i < n_new) {
     const int64_t src = static_cast<int64_t>(b) * src_bstride + i;
@@ -218,6 +220,8 @@ __global__ void __launch_bounds__(288)
                            const __nv_bfloat16* __restrict__ sin_t, int table_rows, float eps,
                            __nv_bfloat16* __restrict__ q) {
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
   const __nv_bfloat16* row = proj + static_cast<int64_t>(b) * ld;
   const int len = c.state[b], next = c.state[c.batch + b];
   if (warp == 0) {
@@ -273,6 +277,8 @@ __global__ void __launch_bounds__(256)
   const int b = blockIdx.y;
   const int t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kGetSlots;
   if (t0 >= n) return;
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
   const int len = __ldg(c.state + b);
   const int64_t row0 = static_cast<int64_t>(b) * c.slots + t0;
   const unsigned short* sc = reinterpret_cast<const unsigned short*>(c.scales) +
@@ -521,6 +527,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
     sm.never_flag = 0;
     ptx::fence_barrier_init();
   }
+  ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const Plan plan = plan_segments(p, sm.scan);
   const Masks km = masks();
@@ -942,9 +949,9 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p)
   const int b = blockIdx.y, tile = blockIdx.x >> 2, r = (blockIdx.x & 3) * 4 + warp;
   const int h = tile * 16 + r;
   if (h >= p.heads) return;  // (a block has a head: its first warp's)
-  const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
-  ptx::pdl_launch_dependents();
   ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
+  const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
   const int2 w = empty ? make_int2(0, 0) : __ldcg(p.where + b * p.tiles + tile);
   if (w.y == 1) return;  // written by the attention kernel
   __nv_bfloat16* o = p.out + (static_cast<int64_t>(b) * p.heads + h) * kLatent;
@@ -1004,9 +1011,10 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p)
 __global__ void __launch_bounds__(kChunk) mass_kernel(const AttnParams p, float decay) {
   __shared__ float slse[kMaxHeads];
   const int tid = threadIdx.x, b = blockIdx.y, chunk = blockIdx.x;
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
   const int len = min(__ldg(p.c.state + b), p.c.slots);
   if (chunk * kChunk >= len) return;
-  ptx::pdl_wait();
   if (tid < p.heads) slse[tid] = __ldcg(p.lse + static_cast<int64_t>(b) * p.tiles * 16 + tid);
   __syncthreads();
   const int t = chunk * kChunk + frag_slot(tid);
@@ -1185,6 +1193,7 @@ __global__ void __launch_bounds__(1024)
   __shared__ int32_t src_s[kSharedPlan], hole_s[kSharedPlan];
   __shared__ uint32_t found;
   __shared__ __align__(16) uint32_t part[2][4];
+  ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const int b = blockIdx.x, lane = threadIdx.x & 31;
   const int t0 = threadIdx.x * IPT;
@@ -1325,6 +1334,7 @@ __global__ void __launch_bounds__(1024)
   __shared__ int warp_sum[32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
+  ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const int b = blockIdx.x;
   const int len = min(max(c.state[b], 0), c.slots), next = c.state[c.batch + b];
@@ -1398,6 +1408,7 @@ __global__ void __launch_bounds__(256)
     evict_move_kernel(Cache s, Cache d, int budget, const int32_t* __restrict__ src_of,
                       int in_place) {
   ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
   const int b = blockIdx.y;
   const int j = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kMoveRows;
   const int n = __ldcg(d.state + b);
@@ -1469,10 +1480,11 @@ int launch_append(const Cache& c, const void* lat, int64_t lat_ld, const void* k
                   cudaStream_t s) {
   if (c.batch == 0 || n_new == 0) return DS_OK;
   const int warps = n_new <= 64 ? 8 : 32;
-  append_kernel<<<dim3((n_new + warps - 1) / warps, c.batch), warps * 32, 0, s>>>(
-      c, static_cast<const __nv_bfloat16*>(lat), lat_ld, static_cast<const __nv_bfloat16*>(kpe),
+  DS_CUDA(launch_chained(
+      append_kernel, dim3((n_new + warps - 1) / warps, c.batch), dim3(warps * 32), 0, s, 1, c,
+      static_cast<const __nv_bfloat16*>(lat), lat_ld, static_cast<const __nv_bfloat16*>(kpe),
       kpe_ld, src_bstride, n_new, new_lens, static_cast<const __nv_bfloat16*>(cos_t),
-      static_cast<const __nv_bfloat16*>(sin_t), table_rows, eps);
+      static_cast<const __nv_bfloat16*>(sin_t), table_rows, eps));
   DS_LAUNCH_CHECK("append_kernel");
   return DS_OK;
 }
@@ -1481,30 +1493,22 @@ int launch_evict(const Cache& s, const Cache& d, int budget, int recent, bool in
                  int32_t* src_of, int32_t* holes, cudaStream_t st) {
   // few rows: the planning block moves them (no second launch); many: all SMs do
   const int here = budget <= kRowsHere ? 1 : 0;
-  if (s.slots <= 1024)
-    evict_plan_kernel<1><<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes, here,
-                                                   in_place);
-  else if (s.slots <= 8192)
-    evict_plan_kernel<8><<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes, here,
-                                                   in_place);
-  else if (s.slots <= 32768)
-    evict_plan_kernel<32><<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes, here,
-                                                    in_place);
+  auto plan = s.slots <= 1024    ? evict_plan_kernel<1>
+              : s.slots <= 8192  ? evict_plan_kernel<8>
+              : s.slots <= 32768 ? evict_plan_kernel<32>
+                                 : nullptr;
+  if (plan != nullptr)
+    DS_CUDA(launch_chained(plan, dim3(s.batch), dim3(1024), 0, st, 1, s, d, budget, recent, src_of,
+                           holes, here, in_place ? 1 : 0));
   else
-    evict_plan_long_kernel<<<s.batch, 1024, 0, st>>>(s, d, budget, recent, src_of, holes);
+    DS_CUDA(launch_chained(evict_plan_long_kernel, dim3(s.batch), dim3(1024), 0, st, 1, s, d,
+                           budget, recent, src_of, holes));
   DS_LAUNCH_CHECK("evict_plan_kernel");
-  if (here && s.slots <= 32768) return DS_OK;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((budget + 8 * kMoveRows - 1) / (8 * kMoveRows), s.batch);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  DS_CUDA(cudaLaunchKernelEx(&cfg, evict_move_kernel, s, d, budget,
-                             static_cast<const int32_t*>(src_of), in_place ? 1 : 0));
+  if (here && plan != nullptr) return DS_OK;
+  DS_CUDA(launch_chained(evict_move_kernel,
+                         dim3((budget + 8 * kMoveRows - 1) / (8 * kMoveRows), s.batch), dim3(256),
+                         0, st, 1, s, d, budget, static_cast<const int32_t*>(src_of),
+                         in_place ? 1 : 0));
   DS_LAUNCH_CHECK("evict_move_kernel");
   return DS_OK;
 }
@@ -1545,24 +1549,13 @@ int launch_attention(const Cache& c, const void* q, int heads, int max_len, floa
   }
   p.ctas = attn_ctas(c.batch, p.tiles, p.max_chunks, di.num_sms);
   if (max_len > 0) {
-    attend4_kernel<<<p.ctas, kAttnThreads, kAttnSmem, s>>>(p);
+    DS_CUDA(launch_chained(attend4_kernel, dim3(p.ctas), dim3(kAttnThreads), kAttnSmem, s, 1, p));
     DS_LAUNCH_CHECK("attend4_kernel");
   }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(p.tiles * 4, c.batch);
-  cfg.blockDim = dim3(kAttnThreads);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = max_len > 0 ? 1 : 0;
-  DS_CUDA(cudaLaunchKernelEx(&cfg, merge_kernel, p));
+  DS_CUDA(launch_chained(merge_kernel, dim3(p.tiles * 4, c.batch), dim3(kAttnThreads), 0, s, 1, p));
   DS_LAUNCH_CHECK("merge_kernel");
   if (accumulate && max_len > 0) {
-    cfg.gridDim = dim3(p.max_chunks, c.batch);
-    cfg.blockDim = dim3(kChunk);
-    DS_CUDA(cudaLaunchKernelEx(&cfg, mass_kernel, p, decay));
+    DS_CUDA(launch_chained(mass_kernel, dim3(p.max_chunks, c.batch), dim3(kChunk), 0, s, 1, p, decay));
     DS_LAUNCH_CHECK("mass_kernel");
   }
   return DS_OK;
@@ -1646,9 +1639,11 @@ int ds_mla_cache4_get(const void* codes, const void* scales_bf16, const int32_t*
                                            nullptr, nullptr, nullptr,
                                            const_cast<int32_t*>(state), batch, slots);
   const int per_block = 8 * ds::c4::kGetSlots;
-  ds::c4::get_kernel<<<dim3((seq_len + per_block - 1) / per_block, batch), 256, 0,
-                       static_cast<cudaStream_t>(stream)>>>(
-      c, seq_len, static_cast<uint4*>(latent_out_bf16), static_cast<uint4*>(kpe_out_bf16));
+  DS_CUDA(ds::launch_chained(ds::c4::get_kernel,
+                             dim3((seq_len + per_block - 1) / per_block, batch), dim3(256), 0,
+                             static_cast<cudaStream_t>(stream), 1, c, seq_len,
+                             static_cast<uint4*>(latent_out_bf16),
+                             static_cast<uint4*>(kpe_out_bf16)));
   DS_LAUNCH_CHECK("get_kernel");
   return DS_OK;
 }
@@ -1732,9 +1727,11 @@ int ds_mla_decode4_step(const void* x_bf16, const void* w_dec_int8, const float*
   const int cols = (heads + 1) * kQCols;
   DS_TRY(ds::i8::launch_linear(x_bf16, hidden, w_dec_int8, w_dec_scale, b.proj, batch, cols, hidden,
                                b.linear, b.linear_bytes, s));
-  decode4_prepare_kernel<<<batch, 288, 0, s>>>(
-      c, b.proj, cols, heads, static_cast<const __nv_bfloat16*>(cos_bf16),
-      static_cast<const __nv_bfloat16*>(sin_bf16), table_rows, eps, b.q);
+  DS_CUDA(ds::launch_chained(
+      decode4_prepare_kernel, dim3(batch), dim3(288), 0, s, 1, c,
+      static_cast<const __nv_bfloat16*>(b.proj), cols, heads,
+      static_cast<const __nv_bfloat16*>(cos_bf16), static_cast<const __nv_bfloat16*>(sin_bf16),
+      table_rows, eps, b.q));
   DS_LAUNCH_CHECK("decode4_prepare_kernel");
   DS_TRY(launch_attention(c, b.q, heads, max_len, softmax_scale, accumulate, mass_decay, b.olat,
                           b.attn, b.attn_bytes, s));
