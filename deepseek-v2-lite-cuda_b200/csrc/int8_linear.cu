@@ -684,11 +684,30 @@ int set_attrs(const DeviceInfo& di) {
 
 // K in parts: enough CTAs for the SMs to stream (up to 1.6 a SM; two fit), four k-blocks each at
 // least, clusters of at most 8.  None is empty.
-void few_splits(int tiles, int k_blocks, int num_sms, int* splits, int* per) {
+void few_splits(int64_t tiles, int k_blocks, int num_sms, int* splits, int* per) {
   int n = 1;
-  while (n < 8 && static_cast<int64_t>(tiles) * n * 10 <= num_sms * 8 && k_blocks >= 4 * n) n *= 2;
+  while (n < 8 && tiles * n * 10 <= num_sms * 8 && k_blocks >= 4 * n) n *= 2;
   *per = (k_blocks + n - 1) / n;
   *splits = (k_blocks + *per - 1) / *per;
+}
+
+// Which kernel takes more than 64 rows: an estimate of both, in hundredths of a microsecond, from
+// their times at 65 to 1024 rows of nine weights (256 x 2048 to 9792 x 8192).  A pair takes 0.36 us
+// for 256 x 256 x 128 products, the tensor cores' rate, and does not split K; a CTA of the other
+// kernel takes 0.27 us for 128 x 128 x 128 beside a second one, splits K over a cluster when
+// there are few tiles, and writes its transposed tile more slowly.  Few / many rows' kernel:
+// 128 x 2048 x 9792 15.0 / 13.2 us, 256 x 1424 x 2840 13.1 / 11.4, 512 x 8192 x 2048 23.2 / 30.7,
+// 192 x 8192 x 9792 37.0 / 30.1, 333 x 8192 x 9792 39.2 / 52.9, 1024 x 2048 x 9792 47.7 / 27.4.
+bool many_rows_faster(int M, int N, int K, int num_sms, int pairs) {
+  if (pairs < 1) return false;
+  const int64_t kb = (K + kBK - 1) / kBK, n128 = (N + 127) / 128, m128 = (M + 127) / 128;
+  if (m128 > 65535) return true;  // the other kernel's grid ends there
+  const int64_t tiles = n128 * m128, pair_tiles = ((N + 255) / 256) * static_cast<int64_t>((M + 255) / 256);
+  int splits = 1, per = static_cast<int>(kb);
+  few_splits(tiles, static_cast<int>(kb), num_sms, &splits, &per);
+  const int64_t few = 600 + 270 * std::min(M, 128) / 128 + (splits > 1 ? 50 : 0) +
+                      27 * ((tiles * splits + num_sms - 1) / num_sms) * per;
+  return 570 + 36 * ((pair_tiles + pairs - 1) / pairs) * kb <= few;
 }
 
 // x: the rows to quantise (QUANT) or null; a, sa: the quantised rows.
@@ -711,7 +730,7 @@ int launch_few(const void* x, int64_t ld, const void* a, const float* sa, const 
   p.N = N;
   p.k_blocks = (K + kBK - 1) / kBK;
   const int tiles = (N + 127) / 128, mt = (M + NT - 1) / NT;
-  few_splits(tiles * mt, p.k_blocks, di.num_sms, &p.splits, &p.kb_per_split);
+  few_splits(static_cast<int64_t>(tiles) * mt, p.k_blocks, di.num_sms, &p.splits, &p.kb_per_split);
   p.status = device_status_ptr();
   if (p.status == nullptr) return fail(DS_ERR_CUDA, "device status word unavailable");
   DS_CUDA(launch_chained(few_rows_kernel<NT, QUANT>, dim3(tiles * p.splits, mt), dim3(kFewThreads),
@@ -787,7 +806,7 @@ int launch_gemm(const void* a, const float* sa, const void* w, const float* sw, 
   if (M <= 16) st = launch_few<16, false>(nullptr, 0, a, sa, w, sw, out, M, N, K, di, s);
   else if (M <= 32) st = launch_few<32, false>(nullptr, 0, a, sa, w, sw, out, M, N, K, di, s);
   else if (M <= 64) st = launch_few<64, false>(nullptr, 0, a, sa, w, sw, out, M, N, K, di, s);
-  else if (M <= 512 || g_pairs[di.device] < 1)
+  else if (!many_rows_faster(M, N, K, di.num_sms, g_pairs[di.device]))
     st = launch_few<128, false>(nullptr, 0, a, sa, w, sw, out, M, N, K, di, s);
   else st = launch_many(a, sa, w, sw, out, M, N, K, di, s);
   DS_TRY(st);
