@@ -61,6 +61,9 @@ cudaError_t launch_pdl(void (*kernel)(ExpT...), dim3 grid, dim3 block, size_t sm
 // kernel waits (ptx::pdl_wait) before its first access to global memory, in at least one CTA
 // whatever its work, and only then lets the next one in (ptx::pdl_launch_dependents): so all
 // that lies before it in the stream is complete, whoever launched it.
+// Its loads are plain or through L2 (__ldcg), never __ldg or through a const __restrict__ pointer: what
+// the last kernel wrote was not constant over this one's life, and such a load may move above the
+// wait.
 template <typename... ExpT, typename... ActT>
 cudaError_t launch_chained(void (*kernel)(ExpT...), dim3 grid, dim3 block, size_t smem,
                            cudaStream_t s, int cluster, ActT&&... args) {

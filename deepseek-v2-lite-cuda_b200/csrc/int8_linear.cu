@@ -72,8 +72,8 @@ __device__ __forceinline__ uint2 quant8(const uint4& v, const RowScale& s) {
 // stays in registers between the maximum and the quotients, a longer one is read twice.
 template <int TPR, int V>
 __global__ void __launch_bounds__(256)
-    quantize_kernel(const uint4* __restrict__ x, int64_t ld8, int rows, int k8,
-                    uint2* __restrict__ q, float* __restrict__ scale) {
+    quantize_kernel(const uint4* x, int64_t ld8, int rows, int k8,
+                    uint2* q, float* scale) {
   __shared__ uint32_t red[8];
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
@@ -86,11 +86,11 @@ __global__ void __launch_bounds__(256)
   uint4 v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    v[i] = t + i * TPR < k8 ? __ldg(src + t + i * TPR) : make_uint4(0, 0, 0, 0);
+    v[i] = t + i * TPR < k8 ? src[t + i * TPR] : make_uint4(0, 0, 0, 0);
   uint32_t m2 = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) m2 = abs_max8(v[i], m2);
-  for (int c = t + V * TPR; c < k8; c += TPR) m2 = abs_max8(__ldg(src + c), m2);
+  for (int c = t + V * TPR; c < k8; c += TPR) m2 = abs_max8(src[c], m2);
   uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
   m = __reduce_max_sync(0xffffffffu, m);
   if (TPR > 32) {
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (t + i * TPR < k8) dst[t + i * TPR] = quant8(v[i], s);
-  for (int c = t + V * TPR; c < k8; c += TPR) dst[c] = quant8(__ldg(src + c), s);
+  for (int c = t + V * TPR; c < k8; c += TPR) dst[c] = quant8(src[c], s);
 }
 
 // ---- the product ----------------------------------------------------------------------------
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kFewThreads)
       if (r < p.M) {
         const uint4* src = p.x + static_cast<int64_t>(r) * p.ld8;
 #pragma unroll 8
-        for (int c = threadIdx.x % tpr; c < p.k8; c += tpr) m2 = abs_max8(__ldg(src + c), m2);
+        for (int c = threadIdx.x % tpr; c < p.k8; c += tpr) m2 = abs_max8(src[c], m2);
       }
       const uint32_t m = __reduce_max_sync(0xffffffffu, max(m2 & 0xFFFFu, m2 >> 16));
       if (lane < kQuantRows) part_max[warp * NT + lane] = lane == r ? m : 0u;
@@ -279,8 +279,8 @@ __global__ void __launch_bounds__(kFewThreads)
       if (r < p.M && k < p.k8) {  // (K is a multiple of 16: both vectors or none)
         const uint4* src = p.x + static_cast<int64_t>(r) * p.ld8 + k;
         const RowScale rs = scales[r];
-        lo = quant8(__ldg(src), rs);
-        hi = quant8(__ldg(src + 1), rs);
+        lo = quant8(src[0], rs);
+        hi = quant8(src[1], rs);
       }
       *reinterpret_cast<uint4*>(xs + (c >> 3) * (NT * kBK) + r * kBK + (((c & 7) ^ (r & 7)) << 4)) =
           make_uint4(lo.x, lo.y, hi.x, hi.y);
@@ -379,9 +379,9 @@ __global__ void __launch_bounds__(kFewThreads)
   if (n >= p.N) return;  // (N is a multiple of 8)
   float sw[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sw[j] = __ldg(p.sw + n + j);
+  for (int j = 0; j < 8; ++j) sw[j] = p.sw[n + j];
   for (int r = threadIdx.x >> 4; r < rn; r += kFewThreads / 16) {
-    const float sa = QUANT ? row_scale_s[r0 + r] : __ldg(p.sa + m0 + r0 + r);
+    const float sa = QUANT ? row_scale_s[r0 + r] : p.sa[m0 + r0 + r];
     const int4* src = reinterpret_cast<const int4*>(smem) + r * 32 + (threadIdx.x & 15) * 2;
     int4 x = src[0], y = src[1];
     for (int k = 1; k < p.splits; ++k) {
@@ -543,9 +543,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int m0 = t / p.n_tiles * 256 + rank * 128, n0 = t % p.n_tiles * 256;
       const int cols = min(256, p.N - n0);
       float* swt = sw + acc * 256;
-      swt[et] = n0 + et < p.N ? __ldg(p.sw + n0 + et) : 0.f;
-      swt[et + 128] = n0 + et + 128 < p.N ? __ldg(p.sw + n0 + et + 128) : 0.f;
-      const float sa = m0 + r < p.M ? __ldg(p.sa + m0 + r) : 0.f;
+      swt[et] = n0 + et < p.N ? p.sw[n0 + et] : 0.f;
+      swt[et + 128] = n0 + et + 128 < p.N ? p.sw[n0 + et + 128] : 0.f;
+      const float sa = m0 + r < p.M ? p.sa[m0 + r] : 0.f;
       ptx::named_bar_sync(1, 128);
       int ok = 1;
       if (lane == 0)
