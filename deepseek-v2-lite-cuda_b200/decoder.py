@@ -122,9 +122,11 @@ class FusedDecoderStack:
     def replay_decode(self, x: torch.Tensor) -> torch.Tensor:
         """One decode step through the captured graph: x bf16 [bsz, hidden] is copied into the
         graph's input; returns the graph's output buffer (overwritten by the next replay)."""
-        for c in self._graph_caches:
+        for layer, c in zip(self.layers, self._graph_caches):
             if c.current_len >= c.max_seq:
                 raise RuntimeError("replay_decode: a cache is full")
+            if isinstance(c, LatentKVCache4):
+                c._check_room(1, layer.attn.cos.shape[0])  # (evictions let positions pass max_seq)
         self._graph_x.copy_(x, non_blocking=True)
         self._graph.replay()
         for c in self._graph_caches:

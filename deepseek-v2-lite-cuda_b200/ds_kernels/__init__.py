@@ -937,6 +937,8 @@ def mla_cache4_append(latent: torch.Tensor, k_pe: torch.Tensor, cache, cos: torc
     cache._check_room(n, cos.shape[0])
     lb, lt, l1 = latent.stride()
     kb, kt, k1 = k_pe.stride()
+    if n == 1:
+        lt, kt = lb, kb
     rows = lb // lt if lt > 0 else 0
     if not (l1 == 1 and k1 == 1 and lt > 0 and kt > 0 and not (lt | kt) & 7 and lb == rows * lt
             and kb == rows * kt and not (latent.data_ptr() | k_pe.data_ptr()) & 15):

@@ -176,7 +176,10 @@ class LatentKVCache4:
     The host knows only a bound on the lengths (`current_len`: exact for batches that are not
     ragged), which it advances with every call; no call synchronises.  A call recorded into a
     CUDA graph takes the whole cache as its bound, so replays may go on to the last slot; replays
-    move the device-side lengths only, and the caller reports them with note_replay()."""
+    move the device-side lengths only, and the caller reports them with note_replay().  A replayed
+    token that finds no slot is dropped, and one whose position lies behind the RoPE tables is
+    rotated as their last row: who replays compares current_len with max_seq, and positions with
+    the tables, as FusedDecoderStack.replay_decode does."""
 
     def __init__(self, bsz: int, max_seq: int, device="cuda"):
         if not isinstance(bsz, int) or bsz < 1:
@@ -201,16 +204,20 @@ class LatentKVCache4:
                                                   self.mass, self.state))
         self._bound = 0      # no sequence is longer
         self._seen = 0       # no next position is larger
+        # the same for what a recorded reset or eviction, not replayed yet, has left in place
+        self._held = self._held_seen = 0
 
     @property
     def current_len(self) -> int:
         """A bound on the sequences' lengths (the length itself when they are equal)."""
+        if self._held > self._bound and not self._recording():
+            return self._held
         return self._bound
 
     @property
     def remaining_capacity(self) -> int:
         """Tokens that surely still fit into every sequence."""
-        return self.max_seq - self._bound
+        return self.max_seq - self.current_len
 
     @property
     def memory_bytes(self) -> int:
@@ -221,12 +228,13 @@ class LatentKVCache4:
     def bound_for_launch(self) -> int:
         """The bound that a launch is sized for: all slots inside a graph capture, because a
         replay sees later lengths."""
-        return self.max_seq if _capturing() else self._bound
+        return self.max_seq if _capturing() else max(self._bound, self._held)
 
     def reset(self) -> None:
         """Clear the cache for new sequences (keeps the memory)."""
         import ds_kernels
         ds_kernels.mla_cache4_reset(self)
+        self._hold()
         self._bound = self._seen = 0
 
     def get(self, seq_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -241,8 +249,13 @@ class LatentKVCache4:
         import ds_kernels
         return ds_kernels.mla_cache4_evict(self, budget, recent, out)
 
-    def note_replay(self, tokens: int = 1) -> None:
-        """A replayed graph appended `tokens` tokens to every sequence."""
+    def note_replay(self, tokens: int = 1, budget: Optional[int] = None) -> None:
+        """A replayed graph appended `tokens` tokens to every sequence, and before (or after) it
+        evicted them down to `budget` slots (0: cleared them)."""
+        if budget is not None:
+            self._bound = min(max(self._bound, self._held), budget)
+            self._seen = max(self._seen, self._held_seen) if budget > 0 else 0
+            self._held = self._held_seen = 0
         self._advance(tokens)
 
     # ---- saving and restoring ------------------------------------------------------------
@@ -286,19 +299,34 @@ class LatentKVCache4:
         self.lens.copy_(lens)
         self.next_pos.copy_(nxt)
         self._bound, self._seen = hi, top
+        self._held = self._held_seen = 0
 
     def __repr__(self) -> str:
         return (f"LatentKVCache4(bsz={self.bsz}, tokens<={self._bound}/{self.max_seq}, "
                 f"memory={self.memory_bytes / 2 ** 20:.2f}MB, device={self.device})")
 
     # ---- bookkeeping of the fused calls --------------------------------------------------
+    def _recording(self) -> bool:
+        return self.index >= 0 and _capturing()
+
+    def _hold(self) -> None:
+        """Before the contents are replaced: recorded into a graph, they stay until a replay, and
+        the calls up to then count on what is there."""
+        if self._recording():
+            self._held, self._held_seen = max(self._held, self._bound), max(self._held_seen, self._seen)
+        else:
+            self._held = self._held_seen = 0
+
     def _check_room(self, n: int, table_rows: int) -> None:
-        if self._bound + n > self.max_seq:
+        bound, seen = self._bound, self._seen
+        if self._held_seen and not self._recording():
+            bound, seen = max(bound, self._held), max(seen, self._held_seen)
+        if bound + n > self.max_seq:
             raise RuntimeError(
-                f"KV cache overflow: current_len={self._bound}, new_tokens={n}, "
+                f"KV cache overflow: current_len={bound}, new_tokens={n}, "
                 f"max_seq={self.max_seq}. Increase max_seq, evict or reset the cache.")
-        if self._seen + n > table_rows:
-            raise RuntimeError(f"LatentKVCache4: position {self._seen + n - 1} is beyond the RoPE "
+        if seen + n > table_rows:
+            raise RuntimeError(f"LatentKVCache4: position {seen + n - 1} is beyond the RoPE "
                                f"tables ({table_rows} positions)")
 
     def _advance(self, n: int) -> None:
@@ -306,4 +334,6 @@ class LatentKVCache4:
         self._seen += n
 
     def _evicted(self, src: "LatentKVCache4", budget: int) -> None:
-        self._bound, self._seen = min(src._bound, budget), src._seen
+        bound, seen = min(src.current_len, budget), max(src._seen, src._held_seen)
+        self._hold()
+        self._bound, self._seen = bound, seen

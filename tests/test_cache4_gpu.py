@@ -495,3 +495,37 @@ def test_state_dict_round_trip_into_a_larger_cache():
     q = torch.randn(2, 16, 576).to(bf16).cuda()
     a, b = (ds_kernels.mla_decode_attention4(q, c, SCALE) for c in (cache, big))
     assert (a.float() - b.float()).norm() <= 2.0 ** -7 * a.float().norm()
+
+
+def test_a_captured_eviction_replays():
+    b = 2
+    cos, sin = (t.cuda() for t in tables(512))
+    lat, kpe = (t.cuda() for t in tokens(b, 150, 60))
+    graphed, eager = LatentKVCache4(b, 200), LatentKVCache4(b, 200)
+    q = torch.randn(b, 16, 576).to(bf16).cuda()
+    for c in (graphed, eager):
+        ds_kernels.mla_cache4_append(lat, kpe, c, cos, sin)
+        ds_kernels.mla_decode_attention4(q, c, SCALE, mass_decay=0.0)
+    sl, sk = (t.cuda() for t in tokens(b, 1, 61))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        graphed.evict(100, 8)
+        ds_kernels.mla_cache4_append(sl, sk, graphed, cos, sin)
+        out = ds_kernels.mla_decode_attention4(q, graphed, SCALE, mass_decay=1.0)
+    graphed.note_replay(-1)                                     # recording appended nothing
+    # nothing has run: an eager call still sees all 150 positions
+    assert graphed.current_len == 150
+    a, w = (ds_kernels.mla_decode_attention4(q, c, SCALE) for c in (graphed, eager))
+    assert torch.equal(a, w)
+    for _ in range(3):
+        graph.replay()
+        graphed.note_replay(1, budget=100)
+        eager.evict(100, 8)
+        ds_kernels.mla_cache4_append(sl, sk, eager, cos, sin)
+        want = ds_kernels.mla_decode_attention4(q, eager, SCALE, mass_decay=1.0)
+        assert graphed.current_len == eager.current_len == 101
+        assert graphed.lens.tolist() == eager.lens.tolist() == [101] * b
+        # the same sums, cut into other segments
+        assert (out.float() - want.float()).norm() <= 2.0 ** -7 * want.float().norm()
+    assert graphed.next_pos.tolist() == [153] * b

@@ -140,3 +140,20 @@ def test_stack_decodes_captures_and_evicts(stack):
     with pytest.raises(RuntimeError, match="full"):
         for s in steps:
             stack.replay_decode(s)
+
+
+def test_replays_stop_at_the_end_of_the_rope_tables(stack):
+    caches = stack.new_caches(1, 32, bits=4)
+    stack.prefill(torch.randn(1, 8, 256, device="cuda").to(bf16), caches)
+    x = torch.randn(1, 256, device="cuda").to(bf16)
+    stack.capture_decode(x, caches)
+    for c in caches:                    # as many evictions later
+        c._seen = 511
+        c.next_pos.fill_(511)
+    stack.replay_decode(x)
+    with pytest.raises(RuntimeError, match="RoPE"):
+        stack.replay_decode(x)
+    caches[0].reset()
+    caches[0]._seen = 3
+    with pytest.raises(RuntimeError, match="empty"):
+        stack.layers[0].attn.prefill(torch.randn(1, 4, 256, device="cuda").to(bf16), caches[0])

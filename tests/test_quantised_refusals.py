@@ -155,3 +155,34 @@ def test_load_state_dict_checks_what_it_takes():
     sd["lens"] = torch.tensor([-1, 3], dtype=torch.int32)
     with pytest.raises(ValueError, match="fit"):
         LatentKVCache4(2, 64, "cpu").load_state_dict(sd)
+
+
+def test_a_recorded_eviction_or_reset_keeps_the_bounds_of_what_the_cache_still_holds(monkeypatch):
+    c, d = LatentKVCache4(2, 100, "cpu"), LatentKVCache4(2, 64, "cpu")
+    c._advance(60)
+    d._advance(20)
+    with monkeypatch.context() as m:
+        m.setattr(LatentKVCache4, "_recording", lambda self: True)
+        d._evicted(c, 10)
+        c._evicted(c, 32)
+        c._check_room(68, 128)                  # behind the recorded eviction
+        with pytest.raises(RuntimeError, match="overflow"):
+            c._check_room(69, 1000)
+    assert c.current_len == 60 and c.remaining_capacity == 40 and d.current_len == 20
+    with pytest.raises(RuntimeError, match="overflow"):
+        c._check_room(41, 1000)
+    c.note_replay(1, budget=32)
+    assert c.current_len == 33 and c._seen == 61
+    c._check_room(67, 128)
+    with monkeypatch.context() as m:
+        m.setattr(LatentKVCache4, "_recording", lambda self: True)
+        c.reset()
+        c._check_room(100, 100)
+        c._advance(5)
+    assert c.current_len == 33
+    with pytest.raises(RuntimeError, match="RoPE"):
+        c._check_room(1, 61)
+    c.note_replay(5, budget=0)
+    assert c.current_len == 5 and c._seen == 5
+    c.reset()
+    assert c.current_len == 0 and c._seen == 0
