@@ -69,7 +69,8 @@ __device__ __forceinline__ uint2 quant8(const uint4& v, const RowScale& s) {
 }
 
 // TPR threads a row (a warp, or the block of 256); a row of at most TPR * V 16-byte vectors
-// stays in registers between the maximum and the quotients, a longer one is read twice.
+// stays in registers between the maximum and the quotients, a longer one is read twice.  Bound by its
+// bytes: 16384 x 2048 takes 17.8 us, 5.7 TB/s.
 template <int TPR, int V>
 __global__ void __launch_bounds__(256)
     quantize_kernel(const uint4* x, int64_t ld8, int rows, int k8,
@@ -153,8 +154,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 constexpr int kFewThreads = 128;
 // QUANT: up to four rows of x, rows * K <= kQuantHere: every CTA takes the maxima of whole rows
 // itself and quantises its part of K straight into the operand's shared-memory layout; no first
-// kernel, whose launch costs more than reading x once per CTA (1 x 2048 x 9792: 7.7 us and a
-// launch on the host against one kernel).
+// kernel, whose launch costs more than reading x once per CTA (1 x 2048 x 9792: 6.8 us against 7.7
+// and a second launch on the host).
 constexpr int kQuantHere = 16384;   // values of x
 constexpr int kQuantRows = 4;
 constexpr int kQuantBlocks = 16;    // k-blocks of a CTA (2 KB of operand each)
@@ -402,6 +403,8 @@ __global__ void __launch_bounds__(kFewThreads)
 // the tiles, as grouped_gemm_kernel's pair mode: each CTA loads its own 128 rows and its half of
 // the channels (32 KB a k-block, 6 stages), two accumulators of 256 columns let the epilogue of
 // a tile run under the products of the next.  A last tile of fewer channels runs narrower MMAs.
+// Bound by the tensor cores: 16384 x 2048 x 3648 takes 88 us, 2.8 Pop/s (twice the bf16 burst rate:
+// 73 us).
 constexpr int kManyStages = 6;
 constexpr int kManyThreads = 192;
 constexpr uint32_t kSlabBytes = 32 * 128;

@@ -180,7 +180,7 @@ __device__ __forceinline__ void put_token(const Cache& c, int b, int slot, int p
 // of a sequence moves its length on: by then every other one has read it (state's third row
 // counts them, and is zero between calls).  Prompts run in blocks of 1024 threads: the blocks
 // meet at that counter, one address a sequence, and with 256 threads a block their arrivals took
-// longer than the tokens (4 x 4096: 22 us).
+// longer than the tokens (4 x 4096: 22 us against 8).
 __global__ void __launch_bounds__(1024)
     append_kernel(Cache c, const __nv_bfloat16* lat, int64_t lat_ld,
                   const __nv_bfloat16* kpe, int64_t kpe_ld, int64_t src_bstride,
@@ -314,12 +314,15 @@ __global__ void __launch_bounds__(256)
 // whatever the lengths the CTAs are about equally long; every block works that out from the
 // lengths on the device.  A segment that is all of its sequence writes the output; the others
 // leave partials, which merge_kernel joins.  (Equal ranges of chunks that cross sequences balance
-// better still, but most CTAs then set up two segments: 64 x 2048 slots took 43 us.)
+// better still, but most CTAs then set up two segments: 64 x 2048 slots took 43 us against 36.8.)
 //
-// Products run on mma.sync m16n8k16 (f16, f32 accumulators) with the 16 heads as M: tcgen05 would
-// take the heads as N = 16, where an instruction costs the same ~75 cycles as at N = 64 and the
-// cache as its M operand from shared memory, 68 of them a chunk, so about 40 cycles a slot and
-// SM against 17 here; and the operand would have to be written back to shared memory as 16 bits.
+// Products run on mma.sync m16n8k16 (f16, f32 accumulators) with the 16 heads as M.  A pair of CTAs
+// takes 8900 cycles for two chunks, 35 a slot and SM: S 3850, P V 3300, maxima, exponentials and
+// barriers 1100, waiting 350; the MMAs alone would take 18 a slot, with the conversion of their
+// operands' codes 29.  tcgen05 with the cache as its 128-row operand would have to write the codes
+// back to shared memory as bytes, and with q and P as four 8-bit digits (N = 64) takes 48 cycles
+// an MMA, all of them shared-memory reads: 12.8 a slot, and 21.5 with the unpacked codes' and P's
+// writes, at best.
 // Here the codes go from shared memory to the fragments:
 //   * a nibble c in bits 0-3 of a half, under the exponent of 1024, is 1024 + c; in bits 4-7, under
 //     that of 64, 64 + c.  One AND-OR and one subtraction (1032, 72) make two operands code - 8,
@@ -1257,7 +1260,7 @@ __global__ void __launch_bounds__(1024)
       const int a3 = static_cast<int>(__reduce_add_sync(0xffffffffu, r[32 + lane]));
       narrow(budget, shift, a1, a2, a3, &v, &in_range, &over_end);
     }
-    if (shift >= 0) {  // the rest by one warp: the keys in range, the others counted
+    if (shift >= 0) {  // the rest by four warps: the keys in range, the others counted
       uint32_t mine = 0;
 #pragma unroll
       for (int i = 0; i < IPT; ++i)
