@@ -211,6 +211,14 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+// Lengths, positions and counters to 0 (a kernel like the others: a memset node would end the
+// overlap of what lies before it with what lies behind).
+__global__ void __launch_bounds__(256) reset_kernel(int32_t* state, int n) {
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
+  for (int i = threadIdx.x; i < n; i += 256) state[i] = 0;
+}
+
 // What a decode step does between its projection and the attention, a block a sequence: warp 0
 // appends the new token (latent and k_pe of the projection's row) and moves the length on, the
 // others copy the heads' absorbed queries and rotate their q_pe at the token's position.
@@ -492,29 +500,33 @@ __device__ __forceinline__ Plan plan_segments(const AttnParams& p, int* red) {
 }
 
 // The scales of slot t0 + threadIdx.x as they multiply the accumulators: scale * rstd for the
-// latent groups; 0 outside the segment, whatever the memory there holds.
-// (Loads that stay where they are written, ahead of S: as plain ones they were moved behind it, and
-// 64 x 2048 slots took 33.2 us against 30.4, 32 x 16384 95.3 against 96.4.)
+// latent groups; 0 outside the segment, whatever the memory there holds.  The loads are without
+// condition (the last slot's behind it), wait for nothing and stay where they are written, ahead of
+// S: as plain ones they were moved behind it, and 64 x 2048 slots took 33.2 us against 30.4, 32 x 16384
+// 95.3 against 96.4.
 struct Factors {
-  uint32_t s[kGroups];
+  unsigned short s[kGroups];
   float rstd;
+  bool in;
 };
 __device__ __forceinline__ Factors load_factors(const Cache& c, int b, int t, int t_end) {
   Factors f;
-  const bool in = t < t_end;
+  f.in = t < t_end;
+  t = min(t, c.slots - 1);
 #pragma unroll
   for (int g = 0; g < kGroups; ++g)
-    f.s[g] = in ? __ldcg(reinterpret_cast<const unsigned short*>(c.scales) +
-                        (static_cast<int64_t>(b) * kGroups + g) * c.slots + t)
-                : 0u;
-  f.rstd = in ? __ldcg(c.rstd + static_cast<int64_t>(b) * c.slots + t) : 0.f;
+    f.s[g] = __ldcg(reinterpret_cast<const unsigned short*>(c.scales) +
+                    (static_cast<int64_t>(b) * kGroups + g) * c.slots + t);
+  f.rstd = __ldcg(c.rstd + static_cast<int64_t>(b) * c.slots + t);
   return f;
 }
 __device__ __forceinline__ void store_factors(float* fac, const Factors& f) {
   const int pos = frag_pos(threadIdx.x);
 #pragma unroll
-  for (int g = 0; g < 4; ++g) fac[g * kChunk + pos] = __uint_as_float(f.s[g] << 16) * f.rstd;
-  fac[4 * kChunk + pos] = __uint_as_float(f.s[4] << 16);
+  for (int g = 0; g < kGroups; ++g) {
+    const float x = __uint_as_float(static_cast<uint32_t>(f.s[g]) << 16);
+    fac[g * kChunk + pos] = f.in ? (g < 4 ? x * f.rstd : x) : 0.f;
+  }
 }
 
 __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const AttnParams p) {
@@ -1604,8 +1616,9 @@ int ds_mla_cache4_reset(int32_t* state, int batch, void* stream) {
   DS_REQUIRE(batch >= 0 && batch <= 65535, "mla_cache4_reset: batch must be at most 65535");
   if (batch == 0) return DS_OK;
   DS_REQUIRE(state != nullptr, "mla_cache4_reset: null pointer");
-  DS_CUDA(cudaMemsetAsync(state, 0, static_cast<size_t>(batch) * 3 * sizeof(int32_t),
-                          static_cast<cudaStream_t>(stream)));
+  DS_CUDA(ds::launch_chained(ds::c4::reset_kernel, dim3(1), dim3(256), 0,
+                             static_cast<cudaStream_t>(stream), 1, state, 3 * batch));
+  DS_LAUNCH_CHECK("reset_kernel");
   return DS_OK;
 }
 
