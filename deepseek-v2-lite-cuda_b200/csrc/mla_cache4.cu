@@ -327,10 +327,10 @@ __global__ void __launch_bounds__(256)
 // Products run on mma.sync m16n8k16 (f16, f32 accumulators) with the 16 heads as M.  A pair of CTAs
 // takes 8900 cycles for two chunks, 35 a slot and SM: S 3850, P V 3300, maxima, exponentials and
 // barriers 1100, waiting 350; the MMAs alone would take 18 a slot, with the conversion of their
-// operands' codes 29.  tcgen05 with the cache as its 128-row operand would have to write the codes
-// back to shared memory as bytes, and with q and P as four 8-bit digits (N = 64) takes 48 cycles
-// an MMA, all of them shared-memory reads: 12.8 a slot, and 21.5 with the unpacked codes' and P's
-// writes, at best.
+// operands' codes 29 (the two add up: eight warps a CTA took 115 us against 96 for 32 x 16384 slots).
+// tcgen05 on codes unpacked to bytes, with q in three and P in four 8-bit digits, takes 12.8 a slot
+// for its MMAs but fills the SM's shared memory, which starves the copies and the softmax beside
+// it: 166 us.
 // Here the codes go from shared memory to the fragments:
 //   * a nibble c in bits 0-3 of a half, under the exponent of 1024, is 1024 + c; in bits 4-7, under
 //     that of 64, 64 + c.  One AND-OR and one subtraction (1032, 72) make two operands code - 8,
