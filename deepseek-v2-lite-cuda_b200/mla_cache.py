@@ -189,23 +189,41 @@ class LatentKVCache4:
         self.bsz, self.max_seq = bsz, max_seq
         self.slots = -(-max_seq // 64) * 64
         dev = torch.device(device)
-        self.codes = torch.zeros((bsz, self.slots, 288), dtype=torch.uint8, device=dev)
-        dev = self.device = self.codes.device
-        self.index = self.codes.get_device()    # the CUDA device's ordinal, -1 off CUDA
-        self.scales = torch.zeros((bsz, 5, self.slots), dtype=torch.bfloat16, device=dev)
-        self.rstd = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
-        self.pos = torch.zeros((bsz, self.slots), dtype=torch.int32, device=dev)
-        self.mass = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
+        self._codes = torch.zeros((bsz, self.slots, 288), dtype=torch.uint8, device=dev)
+        dev = self._codes.device
+        self._scales = torch.zeros((bsz, 5, self.slots), dtype=torch.bfloat16, device=dev)
+        self._rstd = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
+        self._pos = torch.zeros((bsz, self.slots), dtype=torch.int32, device=dev)
+        self._mass = torch.zeros((bsz, self.slots), dtype=torch.float32, device=dev)
         # lengths, next positions, and a row of counters that are zero between calls
-        self.state = torch.zeros((3, bsz), dtype=torch.int32, device=dev)
-        self.lens, self.next_pos = self.state[0], self.state[1]
-        # the arrays never move: their addresses as the C entry points take them
-        self._ptrs = tuple(t.data_ptr() for t in (self.codes, self.scales, self.rstd, self.pos,
-                                                  self.mass, self.state))
+        self._state = torch.zeros((3, bsz), dtype=torch.int32, device=dev)
+        self._bind()
         self._bound = 0      # no sequence is longer
         self._seen = 0       # no next position is larger
         # the same for what a recorded reset or eviction, not replayed yet, has left in place
         self._held = self._held_seen = 0
+
+    # the arrays may be written into, but not replaced: launches take their addresses
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    rstd = property(lambda self: self._rstd)
+    pos = property(lambda self: self._pos)
+    mass = property(lambda self: self._mass)
+    state = property(lambda self: self._state)
+    lens = property(lambda self: self._lens)
+    next_pos = property(lambda self: self._next_pos)
+
+    def _bind(self) -> None:
+        self.device = self._codes.device
+        self.index = self._codes.get_device()    # the CUDA device's ordinal, -1 off CUDA
+        self._lens, self._next_pos = self._state[0], self._state[1]
+        # the addresses as the C entry points take them
+        self._ptrs = tuple(t.data_ptr() for t in (self._codes, self._scales, self._rstd, self._pos,
+                                                  self._mass, self._state))
+
+    def __setstate__(self, state: dict) -> None:  # a deep copy's or a pickle's arrays are others
+        self.__dict__.update(state)
+        self._bind()
 
     @property
     def current_len(self) -> int:

@@ -186,3 +186,20 @@ def test_a_recorded_eviction_or_reset_keeps_the_bounds_of_what_the_cache_still_h
     assert c.current_len == 5 and c._seen == 5
     c.reset()
     assert c.current_len == 0 and c._seen == 0
+
+
+def test_copies_have_arrays_of_their_own_and_arrays_are_not_replaced():
+    import copy
+    import pickle
+    c = LatentKVCache4(2, 64, "cpu")
+    c.state[:2].copy_(torch.tensor([[3, 4], [5, 6]]))
+    c._advance(6)
+    for d in (copy.deepcopy(c), pickle.loads(pickle.dumps(c))):
+        assert not set(d._ptrs) & set(c._ptrs)
+        assert d._ptrs == tuple(t.data_ptr() for t in (d.codes, d.scales, d.rstd, d.pos, d.mass, d.state))
+        assert d.lens.tolist() == [3, 4] and d.next_pos.tolist() == [5, 6] and d.current_len == 6
+        d.lens.zero_()
+        assert d.state[0].tolist() == [0, 0] and c.lens.tolist() == [3, 4]
+    for name in ("codes", "scales", "rstd", "pos", "mass", "state", "lens", "next_pos"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, torch.zeros(2))
