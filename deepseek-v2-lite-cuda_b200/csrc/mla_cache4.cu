@@ -961,9 +961,11 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
   }
 }
 
-// Joins the partials of a (sequence, head tile): four blocks each, four heads a block, a warp a
-// head; lse (log2 of the weights' sum) where it is wanted; zeros for a sequence without slots.
-__global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p) {
+// Joins the partials of a (sequence, head tile), up to `most` of them: four blocks each, four heads
+// a block, a warp a head; lse (log2 of the weights' sum) where it is wanted; zeros for a sequence
+// without slots.  (48 registers and no shared memory: two blocks fit beside two CTAs of the attention and
+// are there when it ends.  With 64 registers, one, 64 x 2048 slots took 31.7 us against 30.2.)
+__global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p, int most) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.y, tile = blockIdx.x >> 2, r = (blockIdx.x & 3) * 4 + warp;
   const int h = tile * 16 + r;
@@ -972,7 +974,7 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p)
   ptx::pdl_launch_dependents();
   const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
   const int2 w = empty ? make_int2(0, 0) : __ldcg(p.where + b * p.tiles + tile);
-  if (w.y == 1) return;  // written by the attention kernel
+  if (w.y == 1 || w.y > most) return;  // written by the attention kernel; merge_wide_kernel's
   __nv_bfloat16* o = p.out + (static_cast<int64_t>(b) * p.heads + h) * kLatent;
   const float* ml = p.part_ml + static_cast<int64_t>(w.x) * 32 + r;
   // lane = (k, j / 4, cc): dimensions 128 w + 16 (2 cc + k) + j .. of row r, for the four w
@@ -1023,6 +1025,96 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p)
         make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
   }
   if (p.lse != nullptr && lane == 0)
+    p.lse[(static_cast<int64_t>(b) * p.tiles + tile) * 16 + r] = M + log2f(L);
+}
+
+// The same for many partials, `least` or more (or none): a block a head, eight warps that take the
+// partials in turn.  A long sequence alone has one of every CTA: 1 x 32768 slots took 90 us with a warp
+// a head, 24 with this kernel.
+constexpr int kWideWarps = 8;
+constexpr int kWideRows = 48, kMergeMost = 32;
+__global__ void __launch_bounds__(32 * kWideWarps) merge_wide_kernel(const AttnParams p, int least) {
+  __shared__ float4 sum[kWideWarps][kLatent / 4];
+  __shared__ float2 ml_of[kWideWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.y, tile = blockIdx.x >> 4, r = blockIdx.x & 15;
+  if (tile * 16 + r >= p.heads) return;  // (head 0 has a block)
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
+  const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
+  const int2 w = empty ? make_int2(0, 0) : __ldcg(p.where + b * p.tiles + tile);
+  if (w.y == 1 || w.y < least) return;
+  const float* ml = p.part_ml + static_cast<int64_t>(w.x) * 32 + r;
+  const int cc = lane & 3, jk = lane >> 2;  // as in merge_kernel
+  const float4* po = reinterpret_cast<const float4*>(p.part_o) +
+                     (static_cast<int64_t>(w.x) * 64 + (r >> 3) * 8 + jk) * 32 + (r & 7) * 4 + cc;
+  const int used = min(w.y, kWideWarps);
+  if (warp < used) {
+    float M = -INFINITY, L = 0.f;
+    float a[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) a[k] = 0.f;
+    const int n = (w.y - warp + kWideWarps - 1) / kWideWarps;  // partials warp, warp + 8, ..
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const bool in = i0 + lane < n;
+      const int64_t at = static_cast<int64_t>(i0 + lane) * kWideWarps + warp;
+      const float m = in ? __ldcg(ml + at * 32) : -INFINITY;
+      float l = in ? __ldcg(ml + at * 32 + 16) : 0.f;
+      float mx = fmaxf(m, M);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      const float keep = ptx::ex2(M - ref);
+      const float f = in ? ptx::ex2(m - ref) : 0.f;
+      l *= f;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      L = fmaf(L, keep, l);
+      M = mx;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) a[k] *= keep;
+#pragma unroll 4
+      for (int i = 0; i < min(32, n - i0); ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        const float4* src = po + (static_cast<int64_t>(i0 + i) * kWideWarps + warp) * (16 * kLatent / 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 v = __ldcg(src + 16 * 32 * k);
+          a[4 * k] = fmaf(fi, v.x, a[4 * k]);
+          a[4 * k + 1] = fmaf(fi, v.y, a[4 * k + 1]);
+          a[4 * k + 2] = fmaf(fi, v.z, a[4 * k + 2]);
+          a[4 * k + 3] = fmaf(fi, v.w, a[4 * k + 3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      sum[warp][32 * k + lane] = make_float4(a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3]);
+    if (lane == 0) ml_of[warp] = make_float2(M, L);
+  }
+  __syncthreads();
+  if (threadIdx.x >= kLatent / 4) return;
+  // warp k: the lane's four dimensions of w = k
+  float M = -INFINITY, L = 0.f;
+  for (int k = 0; k < used; ++k) M = fmaxf(M, ml_of[k].x);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < used; ++k) {
+    const float f = ptx::ex2(ml_of[k].x - ref);
+    const float4 v = sum[k][threadIdx.x];
+    L = fmaf(f, ml_of[k].y, L);
+    o.x = fmaf(f, v.x, o.x);
+    o.y = fmaf(f, v.y, o.y);
+    o.z = fmaf(f, v.z, o.z);
+    o.w = fmaf(f, v.w, o.w);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv);
+  const __nv_bfloat162 y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+  __nv_bfloat16* dst = p.out + (static_cast<int64_t>(b) * p.heads + tile * 16 + r) * kLatent;
+  *reinterpret_cast<uint2*>(dst + 128 * warp + 16 * (2 * cc + (jk >> 2)) + 4 * (jk & 3)) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  if (p.lse != nullptr && threadIdx.x == 0)
     p.lse[(static_cast<int64_t>(b) * p.tiles + tile) * 16 + r] = M + log2f(L);
 }
 
@@ -1571,7 +1663,15 @@ int launch_attention(const Cache& c, const void* q, int heads, int max_len, floa
     DS_CUDA(launch_chained(attend4_kernel, dim3(p.ctas), dim3(kAttnThreads), kAttnSmem, s, 1, p));
     DS_LAUNCH_CHECK("attend4_kernel");
   }
-  DS_CUDA(launch_chained(merge_kernel, dim3(p.tiles * 4, c.batch), dim3(kAttnThreads), 0, s, 1, p));
+  // the kernel for many partials takes all of few rows, and of many rows those that have more than
+  // kMergeMost all the same
+  const int64_t rows = static_cast<int64_t>(c.batch) * p.tiles;
+  const bool few = rows <= kWideRows;
+  if (!few)
+    DS_CUDA(launch_chained(merge_kernel, dim3(p.tiles * 4, c.batch), dim3(kAttnThreads), 0, s, 1, p, kMergeMost));
+  if (few || std::min(p.max_chunks, p.ctas) > kMergeMost)
+    DS_CUDA(launch_chained(merge_wide_kernel, dim3(p.tiles * 16, c.batch), dim3(32 * kWideWarps), 0, s, 1, p,
+                           few ? 0 : kMergeMost + 1));
   DS_LAUNCH_CHECK("merge_kernel");
   if (accumulate && max_len > 0) {
     DS_CUDA(launch_chained(mass_kernel, dim3(p.max_chunks, c.batch), dim3(kChunk), 0, s, 1, p, decay));
