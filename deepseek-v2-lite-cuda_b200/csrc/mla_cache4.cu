@@ -1028,17 +1028,19 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p,
     p.lse[(static_cast<int64_t>(b) * p.tiles + tile) * 16 + r] = M + log2f(L);
 }
 
-// The same for many partials, `least` or more (or none): a block a head, eight warps that take the
-// partials in turn.  A long sequence alone has one of every CTA: 1 x 32768 slots took 90 us with a warp
-// a head, 24 with this kernel.
-constexpr int kWideWarps = 8;
-constexpr int kWideRows = 48, kMergeMost = 32;
-__global__ void __launch_bounds__(32 * kWideWarps) merge_wide_kernel(const AttnParams p, int least) {
-  __shared__ float4 sum[kWideWarps][kLatent / 4];
-  __shared__ float2 ml_of[kWideWarps];
+// The same for many partials, `least` or more (or none): a block a head and D-th of its dimensions, W
+// warps that take the partials in turn.  A long sequence alone has one of every CTA: 1 x 32768 slots
+// took 90 us with a warp a head, 24 with <8, 1>, 18.5 with <16, 4> (16 blocks of <16, 1> read 0.5 MB
+// each, an SM's 4 us: 23).
+constexpr int kWideRows = 48, kWiderRows = 4, kMergeMost = 32;
+template <int W, int D>
+__global__ void __launch_bounds__(32 * W) merge_wide_kernel(const AttnParams p, int least) {
+  constexpr int kW = 4 / D;  // of the four w of merge_kernel
+  __shared__ float4 sum[W][kLatent / 4 / D];
+  __shared__ float2 ml_of[W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.y, tile = blockIdx.x >> 4, r = blockIdx.x & 15;
-  if (tile * 16 + r >= p.heads) return;  // (head 0 has a block)
+  if (tile * 16 + r >= p.heads) return;  // (head 0 has blocks)
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
   const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
@@ -1047,17 +1049,18 @@ __global__ void __launch_bounds__(32 * kWideWarps) merge_wide_kernel(const AttnP
   const float* ml = p.part_ml + static_cast<int64_t>(w.x) * 32 + r;
   const int cc = lane & 3, jk = lane >> 2;  // as in merge_kernel
   const float4* po = reinterpret_cast<const float4*>(p.part_o) +
-                     (static_cast<int64_t>(w.x) * 64 + (r >> 3) * 8 + jk) * 32 + (r & 7) * 4 + cc;
-  const int used = min(w.y, kWideWarps);
+                     (static_cast<int64_t>(w.x) * 64 + (r >> 3) * 8 + jk) * 32 + (r & 7) * 4 + cc +
+                     16 * 32 * kW * static_cast<int>(blockIdx.z);
+  const int used = min(w.y, W);
   if (warp < used) {
     float M = -INFINITY, L = 0.f;
-    float a[16];
+    float a[4 * kW];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) a[k] = 0.f;
-    const int n = (w.y - warp + kWideWarps - 1) / kWideWarps;  // partials warp, warp + 8, ..
+    for (int k = 0; k < 4 * kW; ++k) a[k] = 0.f;
+    const int n = (w.y - warp + W - 1) / W;  // partials warp, warp + 8, ..
     for (int i0 = 0; i0 < n; i0 += 32) {
       const bool in = i0 + lane < n;
-      const int64_t at = static_cast<int64_t>(i0 + lane) * kWideWarps + warp;
+      const int64_t at = static_cast<int64_t>(i0 + lane) * W + warp;
       const float m = in ? __ldcg(ml + at * 32) : -INFINITY;
       float l = in ? __ldcg(ml + at * 32 + 16) : 0.f;
       float mx = fmaxf(m, M);
@@ -1072,13 +1075,13 @@ __global__ void __launch_bounds__(32 * kWideWarps) merge_wide_kernel(const AttnP
       L = fmaf(L, keep, l);
       M = mx;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) a[k] *= keep;
-#pragma unroll 4
+      for (int k = 0; k < 4 * kW; ++k) a[k] *= keep;
+#pragma unroll (4 * D > 8 ? 8 : 4 * D)
       for (int i = 0; i < min(32, n - i0); ++i) {
         const float fi = __shfl_sync(0xffffffffu, f, i);
-        const float4* src = po + (static_cast<int64_t>(i0 + i) * kWideWarps + warp) * (16 * kLatent / 4);
+        const float4* src = po + (static_cast<int64_t>(i0 + i) * W + warp) * (16 * kLatent / 4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kW; ++k) {
           const float4 v = __ldcg(src + 16 * 32 * k);
           a[4 * k] = fmaf(fi, v.x, a[4 * k]);
           a[4 * k + 1] = fmaf(fi, v.y, a[4 * k + 1]);
@@ -1088,13 +1091,13 @@ __global__ void __launch_bounds__(32 * kWideWarps) merge_wide_kernel(const AttnP
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < kW; ++k)
       sum[warp][32 * k + lane] = make_float4(a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3]);
     if (lane == 0) ml_of[warp] = make_float2(M, L);
   }
   __syncthreads();
-  if (threadIdx.x >= kLatent / 4) return;
-  // warp k: the lane's four dimensions of w = k
+  if (warp >= kW) return;
+  // warp k: the lane's four dimensions of the block's k-th w
   float M = -INFINITY, L = 0.f;
   for (int k = 0; k < used; ++k) M = fmaxf(M, ml_of[k].x);
   const float ref = M == -INFINITY ? 0.f : M;
@@ -1112,9 +1115,9 @@ __global__ void __launch_bounds__(32 * kWideWarps) merge_wide_kernel(const AttnP
   const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv);
   const __nv_bfloat162 y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
   __nv_bfloat16* dst = p.out + (static_cast<int64_t>(b) * p.heads + tile * 16 + r) * kLatent;
-  *reinterpret_cast<uint2*>(dst + 128 * warp + 16 * (2 * cc + (jk >> 2)) + 4 * (jk & 3)) =
+  *reinterpret_cast<uint2*>(dst + 128 * (kW * blockIdx.z + warp) + 16 * (2 * cc + (jk >> 2)) + 4 * (jk & 3)) =
       make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-  if (p.lse != nullptr && threadIdx.x == 0)
+  if (p.lse != nullptr && threadIdx.x == 0 && blockIdx.z == 0)
     p.lse[(static_cast<int64_t>(b) * p.tiles + tile) * 16 + r] = M + log2f(L);
 }
 
@@ -1436,6 +1439,177 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+// Sums of three counts over the cluster's blocks, and over those before this one: each block's go to
+// all (`x`: [2][8] entries; calls alternate between the two, and the barrier of the one between them
+// says that everyone has read the last).
+struct ClusterSum {
+  int all[3], before[3];
+};
+__device__ __forceinline__ ClusterSum cluster_sum(int u, int v, int w, int4 (*x)[8], int turn) {
+  const uint32_t rank = ptx::cluster_ctarank();
+  uint32_t size;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+  if (threadIdx.x < size) {
+    const uint32_t to = ptx::mapa_shared(ptx::smem_u32(&x[turn & 1][rank]), threadIdx.x);
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(u), "r"(v), "r"(w), "r"(0)
+                 : "memory");
+  }
+  ptx::cluster_sync();
+  ClusterSum s = {};
+  for (uint32_t k = 0; k < size; ++k) {
+    const int4 y = x[turn & 1][k];
+    const int z[3] = {y.x, y.y, y.z};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      s.all[i] += z[i];
+      if (k < rank) s.before[i] += z[i];
+    }
+  }
+  return s;
+}
+
+// The plan of more slots by a cluster of blocks a sequence, 1024 * IPT slots each: as above, with the
+// counts of every round summed over the cluster, the last keys found by its first block, and the lists in
+// global memory.  (8 x 32768 slots to 4096: 29.5 us against 53 with 32 keys a thread in one block; 2 x
+// 100000 to 4096: 67 against 635 with histograms.)
+template <int IPT>
+__global__ void __launch_bounds__(1024)
+    evict_plan_cluster_kernel(Cache c, Cache dst, int budget, int recent, int32_t* src_of, int32_t* holes) {
+  __shared__ uint32_t red[4][32];
+  __shared__ uint32_t list[kFewKeys];
+  __shared__ uint32_t found;
+  __shared__ __align__(16) uint32_t part[2][4];
+  __shared__ __align__(16) int4 counts[2][8];
+  ptx::pdl_wait();
+  ptx::pdl_launch_dependents();
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  uint32_t blocks;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
+  const int b = blockIdx.x / blocks, lane = threadIdx.x & 31;
+  const int t0 = (rank * 1024 + threadIdx.x) * IPT;
+  const float* mass = c.mass + static_cast<int64_t>(b) * c.slots;
+  const int32_t* pos = c.pos + static_cast<int64_t>(b) * c.slots;
+  float m[IPT];
+  int ps[IPT];
+#pragma unroll
+  for (int i = 0; i < IPT; i += 4)
+    if (t0 + i < c.slots) {  // (slots are a multiple of 64)
+      *reinterpret_cast<float4*>(m + i) = *reinterpret_cast<const float4*>(mass + t0 + i);
+      *reinterpret_cast<int4*>(ps + i) = *reinterpret_cast<const int4*>(pos + t0 + i);
+    }
+  const int len = min(max(c.state[b], 0), c.slots), next = c.state[c.batch + b];
+  ptx::cluster_sync();  // all blocks have started, and have read the length
+  int32_t* const src = src_of + static_cast<int64_t>(b) * budget;
+  int32_t* const hole = holes + static_cast<int64_t>(b) * budget;
+  const int kept_n = min(len, budget);
+  if (len > budget) {  // (the same for all of the cluster)
+    const int from = next - recent;
+    uint32_t key[IPT];
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) key[i] = t0 + i < len ? evict_key(m[i], ps[i], from) : 0u;
+    uint32_t v = 0;
+    int in_range = len, over_end = 0, shift = 30, turn = 0;
+#pragma unroll 1
+    for (; shift >= 0 && in_range > kFewKeys; shift -= 2, ++turn) {
+      uint32_t n12 = 0, n3 = 0;
+      const uint32_t c1 = v | (1u << shift), c2 = v | (2u << shift), c3 = v | (3u << shift);
+#pragma unroll
+      for (int i = 0; i < IPT; ++i) {
+        n12 += (key[i] >= c1 ? 1u : 0u) + (key[i] >= c2 ? 0x10000u : 0u);
+        n3 += key[i] >= c3 ? 1u : 0u;
+      }
+      // (a block has at most 32768 keys: two counts to a word)
+      const uint32_t w12 = __reduce_add_sync(0xffffffffu, n12);
+      const uint32_t w3 = __reduce_add_sync(0xffffffffu, n3);
+      if (lane == 0) {
+        red[0][threadIdx.x >> 5] = w12;
+        red[1][threadIdx.x >> 5] = w3;
+      }
+      __syncthreads();
+      const uint32_t s12 = __reduce_add_sync(0xffffffffu, red[0][lane]);
+      const uint32_t s3 = __reduce_add_sync(0xffffffffu, red[1][lane]);
+      const ClusterSum s = cluster_sum(s12 & 0xFFFFu, s12 >> 16, s3, counts, turn);
+      narrow(budget, shift, s.all[0], s.all[1], s.all[2], &v, &in_range, &over_end);
+    }
+    if (shift >= 0) {  // the rest by four warps of the first block
+      uint32_t mine = 0;
+#pragma unroll
+      for (int i = 0; i < IPT; ++i)
+        mine += t0 + i < len && (shift == 30 || (key[i] >> (shift + 2)) == (v >> (shift + 2))) ? 1u : 0u;
+      uint32_t at = block_prefix(mine, red[2]);
+      if (threadIdx.x == 1023) red[3][0] = at + mine;
+      __syncthreads();
+      at += cluster_sum(red[3][0], 0, 0, counts, turn++).before[0];
+      const uint32_t first = ptx::mapa_shared(ptx::smem_u32(list), 0);
+#pragma unroll
+      for (int i = 0; i < IPT; ++i)
+        if (t0 + i < len && (shift == 30 || (key[i] >> (shift + 2)) == (v >> (shift + 2)))) {
+          asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(first + 4 * at), "r"(key[i]) : "memory");
+          ++at;
+        }
+      ptx::cluster_sync();
+      if (rank == 0 && threadIdx.x < 128) {
+        const uint32_t f = find_in_list(list, in_range, budget - over_end, shift, v, part);
+        if (threadIdx.x < blocks)
+          asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(ptx::mapa_shared(ptx::smem_u32(&found), threadIdx.x)),
+                       "r"(f)
+                       : "memory");
+      }
+      ptx::cluster_sync();
+      v = found;
+    }
+    uint32_t above = 0, ties = 0;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      above += key[i] > v ? 1u : 0u;
+      ties += key[i] == v && t0 + i < len ? 1u : 0u;
+    }
+    __syncthreads();  // (the words of `red` are free)
+    const uint32_t packed = above | (ties << 16);
+    const uint32_t before_t = block_prefix(packed, red[0]);
+    if (threadIdx.x == 1023) red[3][1] = before_t + packed;
+    __syncthreads();
+    const ClusterSum kept = cluster_sum(red[3][1] & 0xFFFFu, red[3][1] >> 16, 0, counts, turn++);
+    // ties that stay: the first ones
+    int rank_t = static_cast<int>(before_t >> 16) + kept.before[1];
+    const int need = budget - kept.all[0];
+    uint32_t keep = 0, n_hole = 0, n_late = 0;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int t = t0 + i;
+      bool k = key[i] > v;
+      if (key[i] == v && t < len) k = rank_t++ < need;
+      if (k) keep |= 1u << i;
+      n_hole += t < budget && !k ? 1u : 0u;
+      n_late += t >= budget && k ? 1u : 0u;
+    }
+    const uint32_t moved = n_hole | (n_late << 16);
+    const uint32_t before = block_prefix(moved, red[1]);
+    if (threadIdx.x == 1023) red[3][2] = before + moved;
+    __syncthreads();
+    const ClusterSum gone = cluster_sum(red[3][2] & 0xFFFFu, red[3][2] >> 16, 0, counts, turn++);
+    int h = static_cast<int>(before & 0xFFFFu) + gone.before[0];
+    int l = static_cast<int>(before >> 16) + gone.before[1];
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int t = t0 + i;
+      if (t >= budget) continue;
+      if (keep >> i & 1u) src[t] = t;
+      else hole[h++] = t;
+    }
+    ptx::cluster_sync();  // the holes are written before survivors are paired with them
+#pragma unroll
+    for (int i = 0; i < IPT; ++i)
+      if (t0 + i >= budget && (keep >> i & 1u)) src[__ldcg(hole + l++)] = t0 + i;
+  } else {
+    for (int j = rank * 1024 + threadIdx.x; j < kept_n; j += 1024 * static_cast<int>(blocks)) src[j] = j;
+  }
+  if (rank == 0 && threadIdx.x == 0) {
+    dst.state[b] = kept_n;
+    dst.state[c.batch + b] = next;
+  }
+}
+
 // The same for any number of slots: the keys are made again for each pass, four of which build
 // histograms of 8 bits, and slots are ranked tile by tile.
 __global__ void __launch_bounds__(1024)
@@ -1603,19 +1777,24 @@ int launch_append(const Cache& c, const void* lat, int64_t lat_ld, const void* k
 int launch_evict(const Cache& s, const Cache& d, int budget, int recent, bool in_place,
                  int32_t* src_of, int32_t* holes, cudaStream_t st) {
   // few rows: the planning block moves them (no second launch); many: all SMs do
-  const int here = budget <= kRowsHere ? 1 : 0;
-  auto plan = s.slots <= 1024    ? evict_plan_kernel<1>
-              : s.slots <= 8192  ? evict_plan_kernel<8>
-              : s.slots <= 32768 ? evict_plan_kernel<32>
-                                 : nullptr;
-  if (plan != nullptr)
-    DS_CUDA(launch_chained(plan, dim3(s.batch), dim3(1024), 0, st, 1, s, d, budget, recent, src_of,
-                           holes, here, in_place ? 1 : 0));
-  else
+  const bool one = s.slots <= 8192, here = one && budget <= kRowsHere;
+  if (one) {
+    DS_CUDA(launch_chained(s.slots <= 1024 ? evict_plan_kernel<1> : evict_plan_kernel<8>, dim3(s.batch),
+                           dim3(1024), 0, st, 1, s, d, budget, recent, src_of, holes, here ? 1 : 0,
+                           in_place ? 1 : 0));
+  } else if (s.slots <= 262144) {
+    const int ipt = s.slots <= 65536 ? 8 : 32;
+    int blocks = 2;
+    while (blocks * ipt * 1024 < s.slots) blocks *= 2;
+    DS_CUDA(launch_chained(ipt == 8 ? evict_plan_cluster_kernel<8> : evict_plan_cluster_kernel<32>,
+                           dim3(s.batch * blocks), dim3(1024), 0, st, blocks, s, d, budget, recent, src_of,
+                           holes));
+  } else {
     DS_CUDA(launch_chained(evict_plan_long_kernel, dim3(s.batch), dim3(1024), 0, st, 1, s, d,
                            budget, recent, src_of, holes));
+  }
   DS_LAUNCH_CHECK("evict_plan_kernel");
-  if (here && plan != nullptr) return DS_OK;
+  if (here) return DS_OK;
   DS_CUDA(launch_chained(evict_move_kernel,
                          dim3((budget + 8 * kMoveRows - 1) / (8 * kMoveRows), s.batch), dim3(256),
                          0, st, 1, s, d, budget, static_cast<const int32_t*>(src_of),
@@ -1669,8 +1848,10 @@ int launch_attention(const Cache& c, const void* q, int heads, int max_len, floa
   const bool few = rows <= kWideRows;
   if (!few)
     DS_CUDA(launch_chained(merge_kernel, dim3(p.tiles * 4, c.batch), dim3(kAttnThreads), 0, s, 1, p, kMergeMost));
-  if (few || std::min(p.max_chunks, p.ctas) > kMergeMost)
-    DS_CUDA(launch_chained(merge_wide_kernel, dim3(p.tiles * 16, c.batch), dim3(32 * kWideWarps), 0, s, 1, p,
+  if (rows <= kWiderRows)
+    DS_CUDA(launch_chained(merge_wide_kernel<16, 4>, dim3(p.tiles * 16, c.batch, 4), dim3(512), 0, s, 1, p, 0));
+  else if (few || std::min(p.max_chunks, p.ctas) > kMergeMost)
+    DS_CUDA(launch_chained(merge_wide_kernel<8, 1>, dim3(p.tiles * 16, c.batch), dim3(256), 0, s, 1, p,
                            few ? 0 : kMergeMost + 1));
   DS_LAUNCH_CHECK("merge_kernel");
   if (accumulate && max_len > 0) {

@@ -396,6 +396,59 @@ def test_evict_long():
         assert out.pos[i].cpu().tolist() == pos[i][src].tolist()
 
 
+def evict_ref_long(mass, pos, n, nxt, budget, recent):
+    """evict_ref by arrays"""
+    if n <= budget:
+        return torch.arange(n)
+    m = mass[:n].double()
+    nan = torch.isnan(m)
+    m = torch.where(nan, -math.inf, m)
+    order = torch.argsort(m, descending=True, stable=True)          # (-0 and 0 are equal)
+    order = order[torch.argsort(nan[order].int(), stable=True)]
+    order = order[torch.argsort((pos[:n] < nxt - recent)[order].int(), stable=True)]
+    kept = torch.zeros(n, dtype=torch.bool)
+    kept[order[:budget]] = True
+    src = torch.arange(budget)
+    src[~kept[:budget]] = budget + kept[budget:].nonzero().flatten()
+    return src
+
+
+@pytest.mark.parametrize("kind", ["random", "ties", "equal", "odd"])
+@pytest.mark.parametrize("lens,budget,recent", [([16000, 5, 8193], 1000, 10), ([65536, 40000, 0], 20000, 300),
+                                                ([100000, 65537, 1], 30000, 0), ([262208], 5000, 5000)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_by_clusters_and_beyond(kind, lens, budget, recent, in_place):
+    b = len(lens)
+    cache, _ = random_cache(b, max(lens), lens, budget)
+    cache.mass.copy_(masses(kind, b, cache.slots, budget))
+    g = torch.Generator().manual_seed(9)
+    for i, n in enumerate(lens):
+        cache.pos[i, :n] = torch.randperm(n, generator=g).int().cuda()
+    mass, pos = cache.mass.cpu().clone(), cache.pos.cpu().clone()
+    rows = {i: cache.codes[i].cpu() for i in range(b)}
+    out = ds_kernels.mla_cache4_evict(cache, budget, recent, None if in_place else LatentKVCache4(b, budget))
+    assert out.lens.tolist() == [min(n, budget) for n in lens] and out.next_pos.tolist() == lens
+    for i, n in enumerate(lens):
+        src = evict_ref_long(mass[i], pos[i], n, n, budget, recent)
+        assert torch.equal(out.pos[i, :len(src)].cpu(), pos[i][src])
+        assert torch.equal(out.codes[i, :len(src)].cpu(), rows[i][src])
+
+
+def test_attention_of_few_long_sequences_among_many():
+    """More partials of a sequence than the joining kernels take by a warp a head, in few and in many
+    rows."""
+    for lens in ([20000], [9000, 0, 300], [30000] + [5] * 70):
+        b = len(lens)
+        cache, st = random_cache(b, max(lens), lens, b)
+        q = torch.randn(b, 16, 576, generator=torch.Generator().manual_seed(b)).to(bf16)
+        few = [i for i in range(b) if lens[i] > 0][:3] + [b - 1]
+        o = ds_kernels.mla_decode_attention4(q.cuda(), cache, SCALE, mass_decay=0.0)
+        part = {k: v[few] for k, v in st.items()}
+        want, tol, mass, mtol = attend64(part, q[few], [lens[i] for i in few])
+        check(o.view(b, -1)[few], want, tol)
+        check(cache.mass[few], mass, mtol)
+
+
 # ---- together ---------------------------------------------------------------------------------
 def test_a_run_of_steps_with_evictions():
     """Append, attend with accumulation and evict, step after step, against the same in 64 bits on
