@@ -175,31 +175,40 @@ __device__ __forceinline__ void put_token(const Cache& c, int b, int slot, int p
   }
 }
 
-// n_new tokens of each sequence (new_lens[b] of them when given) behind its last slot; a warp a
-// token, whose loads are on their way while the lengths are read.  The block that finishes last
-// of a sequence moves its length on: by then every other one has read it (state's third row
-// counts them, and is zero between calls).  Prompts run in blocks of 1024 threads: the blocks
-// meet at that counter, one address a sequence, and with 256 threads a block their arrivals took
-// longer than the tokens (4 x 4096: 22 us against 8).
-__global__ void __launch_bounds__(1024)
+// n_new tokens of each sequence (new_lens[b] of them when given) behind its last slot; a warp takes
+// TPW tokens, the next one's loads under the work on the last.  The block that finishes last of a
+// sequence moves its length on: by then every other one has read it (state's third row counts them,
+// and is zero between calls).  A block has 32 tokens of a prompt: the blocks meet at that counter, one
+// address a sequence, and with 8 tokens a block their arrivals took longer than the tokens (4 x 4096: 22
+// us).  By 32 warps, or, from 8192 tokens on, by 8 warps of four tokens each: 4 x 4096 tokens 12.7 and
+// 10.1 us, 1 x 4096 3.4 and 5.4.
+constexpr int kManyTokens = 8192;
+template <int TPW>
+__global__ void __launch_bounds__(TPW == 1 ? 1024 : 256)
     append_kernel(Cache c, const __nv_bfloat16* lat, int64_t lat_ld,
                   const __nv_bfloat16* kpe, int64_t kpe_ld, int64_t src_bstride,
                   int n_new, const int32_t* new_lens,
                   const __nv_bfloat16* cos_t, const __nv_bfloat16* sin_t,
                   int table_rows, float eps) {
   const int b = blockIdx.y;
-  const int i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int warps = blockDim.x >> 5;
+  const int i0 = blockIdx.x * warps * TPW + (threadIdx.x >> 5);
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
+  const int64_t src0 = static_cast<int64_t>(b) * src_bstride;
   Token tok{};
-  if (i < n_new) {
-    const int64_t src = static_cast<int64_t>(b) * src_bstride + i;
-    tok = load_token(lat + src * lat_ld, kpe + src * kpe_ld);
-  }
+  if (i0 < n_new) tok = load_token(lat + (src0 + i0) * lat_ld, kpe + (src0 + i0) * kpe_ld);
   const int len = c.state[b], next = c.state[c.batch + b];
   const int n = new_lens != nullptr ? min(n_new, new_lens[b]) : n_new;
-  if (i < n && len >= 0 && len + i < c.slots)
-    put_token(c, b, len + i, next + i, tok, cos_t, sin_t, table_rows, eps);
+#pragma unroll 1
+  for (int k = 0; k < TPW; ++k) {
+    const int i = i0 + warps * k;
+    if (i >= n || len < 0 || len + i >= c.slots) break;
+    const Token now = tok;
+    if (k + 1 < TPW && i + warps < n)
+      tok = load_token(lat + (src0 + i + warps) * lat_ld, kpe + (src0 + i + warps) * kpe_ld);
+    put_token(c, b, len + i, next + i, now, cos_t, sin_t, table_rows, eps);
+  }
   __syncthreads();  // every warp has read the length
   if (threadIdx.x == 0 &&
       (gridDim.x == 1 ||
@@ -1764,12 +1773,14 @@ int launch_append(const Cache& c, const void* lat, int64_t lat_ld, const void* k
                   const void* cos_t, const void* sin_t, int table_rows, float eps,
                   cudaStream_t s) {
   if (c.batch == 0 || n_new == 0) return DS_OK;
-  const int warps = n_new <= 64 ? 8 : 32;
+  const int tokens = n_new <= 64 ? 8 : 32;  // of a block
+  const bool many = tokens == 32 && static_cast<int64_t>(c.batch) * n_new >= kManyTokens;
   DS_CUDA(launch_chained(
-      append_kernel, dim3((n_new + warps - 1) / warps, c.batch), dim3(warps * 32), 0, s, 1, c,
-      static_cast<const __nv_bfloat16*>(lat), lat_ld, static_cast<const __nv_bfloat16*>(kpe),
-      kpe_ld, src_bstride, n_new, new_lens, static_cast<const __nv_bfloat16*>(cos_t),
-      static_cast<const __nv_bfloat16*>(sin_t), table_rows, eps));
+      many ? append_kernel<4> : append_kernel<1>, dim3((n_new + tokens - 1) / tokens, c.batch),
+      dim3(many ? 256 : 32 * tokens), 0, s, 1, c, static_cast<const __nv_bfloat16*>(lat), lat_ld,
+      static_cast<const __nv_bfloat16*>(kpe), kpe_ld, src_bstride, n_new, new_lens,
+      static_cast<const __nv_bfloat16*>(cos_t), static_cast<const __nv_bfloat16*>(sin_t), table_rows,
+      eps));
   DS_LAUNCH_CHECK("append_kernel");
   return DS_OK;
 }

@@ -162,6 +162,31 @@ def test_ragged_append_touches_nothing_else(n):
         assert (got[i, m:] == 0).all()
 
 
+def test_append_of_many_tokens():
+    """Enough for the kernel that takes four tokens a warp; ragged, behind what is there, more tokens than
+    one sequence has slots for in its padding."""
+    b, n, had = 3, 3001, 70
+    cos, sin = (t for t in tables(4000))
+    cache = LatentKVCache4(b, n + had)
+    lat0, kpe0 = tokens(b, had, 70)
+    ds_kernels.mla_cache4_append(lat0.cuda(), kpe0.cuda(), cache, cos.cuda(), sin.cuda())
+    for f in ("codes", "rstd", "mass"):
+        getattr(cache, f)[:, had:].fill_(77)
+    lat, kpe = tokens(b, n, 71)
+    lens = [n, 0, 1777]
+    ds_kernels.mla_cache4_append(lat.cuda(), kpe.cuda(), cache, cos.cuda(), sin.cuda(),
+                                 new_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    assert cache.lens.tolist() == [had + m for m in lens] == cache.next_pos.tolist()
+    assert cache.state[2].tolist() == [0] * b
+    at = torch.arange(had, had + n)
+    want = torch.cat([quant64(lat, 128)[0], quant64(rotate(kpe, at.expand(b, -1), cos, sin), 64)[0]], -1)
+    for i, m in enumerate(lens):
+        assert torch.equal(unpack(cache.codes[i, had:had + m].cpu()), want[i, :m])
+        assert torch.equal(cache.pos[i, had:had + m].cpu().long(), at[:m])
+        assert (cache.codes[i, had + m:] == 77).all() and (cache.rstd[i, had + m:] == 77).all()
+        assert (cache.mass[i, had + m:] == 77).all() and (cache.mass[i, :had + m] == 0).all()
+
+
 def test_append_takes_strided_rows_and_odd_views():
     cos, sin = tables(64)
     proj = torch.randn(3, 9792 + 8, dtype=torch.float32).to(bf16).cuda()
