@@ -2070,6 +2070,9 @@ int ds_mla_cache4_evict(void* codes, void* scales_bf16, float* rstd, int32_t* po
   DS_REQUIRE(budget >= 1 && budget <= dst_slots, "mla_cache4_evict: budget outside the cache");
   DS_REQUIRE(recent >= 0 && recent <= budget, "mla_cache4_evict: recent must be in [0, budget]");
   if (batch == 0) return DS_OK;
+  // weights and positions of more than 1024 slots are read four at a time
+  DS_REQUIRE(ds::aligned16(mass) && ds::aligned16(pos),
+             "mla_cache4_evict: the cache's mass and pos must be 16-byte aligned");
   const bool in_place = dst_codes == codes;
   DS_REQUIRE(in_place ? (dst_scales_bf16 == scales_bf16 && dst_rstd == rstd && dst_pos == pos &&
                          dst_mass == mass && dst_state == state && dst_slots == slots)

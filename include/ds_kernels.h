@@ -521,7 +521,10 @@ DS_API int ds_int8_linear(const void* x_bf16, int64_t row_stride, const void* w_
  *   last), ties to the lowest slot.  Kept slots below the budget stay where they are; the
  *   others move, in ascending order, into the evicted ones below it.  The result goes to the
  *   dst arrays (all the same as the source's: in place; or all others, [batch, dst_slots,
- *   ...]); slots behind the result's length are left as they were.
+ *   ...]); slots behind the result's length are left as they were.  The source's mass and pos are
+ *   read four at a time.
+ * codes, scales and rstd are 16-byte aligned, for ds_mla_cache4_evict the source's mass and pos
+ * too; other alignments are DS_ERR_INVALID_ARG.
  * The calls read lengths on the device, so they can be captured into a graph and replayed. */
 DS_API int ds_mla_cache4_reset(int32_t* state, int batch, void* stream);
 DS_API int ds_mla_cache4_append(const void* latent_bf16, int64_t latent_ld, const void* kpe_bf16,

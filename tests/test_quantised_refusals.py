@@ -203,3 +203,16 @@ def test_copies_have_arrays_of_their_own_and_arrays_are_not_replaced():
     for name in ("codes", "scales", "rstd", "pos", "mass", "state", "lens", "next_pos"):
         with pytest.raises(AttributeError):
             setattr(c, name, torch.zeros(2))
+
+
+@pytest.mark.parametrize("slots", [64, 1024, 1088, 16384])
+@pytest.mark.parametrize("which", ["mass", "pos"])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_eviction_refuses_arrays_that_it_could_not_read_four_at_a_time(slots, which, in_place):
+    src = list(C[:6])
+    i = {"pos": 3, "mass": 4}[which]
+    for off in (4, 8):
+        src[i] = P(C[i].value + off)
+        dst = src if in_place else C[6:12]
+        assert lib().ds_mla_cache4_evict(*src, 1, slots, 8, 0, *dst, slots, C[12], 1 << 20, None) == 1
+        assert "aligned" in lib().ds_last_error().decode()
