@@ -1930,6 +1930,8 @@ int ds_mla_cache4_append(const void* latent_bf16, int64_t latent_ld, const void*
   DS_REQUIRE(latent_ld % 8 == 0 && kpe_ld % 8 == 0 && ds::aligned16(latent_bf16) &&
                  ds::aligned16(kpe_bf16),
              "mla_cache4_append: rows must start on 16-byte boundaries");
+  DS_REQUIRE(ds::aligned2(cos_bf16) && ds::aligned2(sin_bf16),
+             "mla_cache4_append: misaligned RoPE tables");
   return ds::c4::launch_append(c, latent_bf16, latent_ld, kpe_bf16, kpe_ld, src_rows_per_seq,
                                new_tokens, new_lens, cos_bf16, sin_bf16, table_rows, eps,
                                static_cast<cudaStream_t>(stream));
@@ -1944,8 +1946,9 @@ int ds_mla_cache4_get(const void* codes, const void* scales_bf16, const int32_t*
   if (rows == 0) return DS_OK;
   DS_REQUIRE(codes && scales_bf16 && state && latent_out_bf16 && kpe_out_bf16,
              "mla_cache4_get: null pointer");
-  DS_REQUIRE(ds::aligned16(codes) && ds::aligned16(latent_out_bf16) && ds::aligned16(kpe_out_bf16),
-             "mla_cache4_get: 16-byte aligned pointers");
+  DS_REQUIRE(ds::aligned16(codes) && ds::aligned16(scales_bf16) &&
+                 ds::aligned16(latent_out_bf16) && ds::aligned16(kpe_out_bf16),
+             "mla_cache4_get: codes, scales and outputs must be 16-byte aligned");
   DS_REQUIRE(batch <= 65535, "mla_cache4_get: batch must be at most 65535");
   const ds::c4::Cache c = ds::c4::cache_of(const_cast<void*>(codes), const_cast<void*>(scales_bf16),
                                            nullptr, nullptr, nullptr,
@@ -2028,6 +2031,8 @@ int ds_mla_decode4_step(const void* x_bf16, const void* w_dec_int8, const float*
   DS_REQUIRE(ds::aligned16(x_bf16) && ds::aligned16(w_dec_int8) && ds::aligned16(w_out_int8) &&
                  ds::aligned16(out_bf16) && ds::aligned16(workspace),
              "mla_decode4_step: x, weights, out and workspace must be 16-byte aligned");
+  DS_REQUIRE(ds::aligned2(cos_bf16) && ds::aligned2(sin_bf16),
+             "mla_decode4_step: misaligned RoPE tables");
   ds::DeviceInfo di;
   DS_TRY(ds::device_info(&di));
   ds::Carve w(workspace, workspace_bytes);
@@ -2079,6 +2084,7 @@ int ds_mla_cache4_evict(void* codes, void* scales_bf16, float* rstd, int32_t* po
                       : (dst_scales_bf16 != scales_bf16 && dst_rstd != rstd && dst_pos != pos &&
                          dst_mass != mass && dst_state != state),
              "mla_cache4_evict: the result must be the cache itself or share nothing with it");
+  DS_REQUIRE(ds::aligned16(workspace), "mla_cache4_evict: workspace must be 16-byte aligned");
   ds::Carve w(workspace, workspace_bytes);
   int32_t* src_of = w.take<int32_t>(static_cast<size_t>(batch) * budget);
   int32_t* holes = w.take<int32_t>(static_cast<size_t>(batch) * budget);

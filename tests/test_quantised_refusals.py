@@ -216,3 +216,20 @@ def test_eviction_refuses_arrays_that_it_could_not_read_four_at_a_time(slots, wh
         dst = src if in_place else C[6:12]
         assert lib().ds_mla_cache4_evict(*src, 1, slots, 8, 0, *dst, slots, C[12], 1 << 20, None) == 1
         assert "aligned" in lib().ds_last_error().decode()
+
+
+@pytest.mark.parametrize("call", [
+    lambda L: L.ds_mla_cache4_evict(*C[:6], 1, 64, 8, 0, *C[:6], 64, P(C[12].value + 2), 1 << 20, None),
+    lambda L: L.ds_mla_cache4_get(C[0], P(C[1].value + 1), C[2], 1, 64, 4, C[3], C[4], None),
+    lambda L: L.ds_mla_cache4_append(C[0], 512, C[1], 64, 1, 1, None, P(C[2].value + 1), C[3], 4, F(1e-6), *C[4:10], 1,
+                                     64, None),
+    lambda L: L.ds_mla_cache4_append(C[0], 512, C[1], 64, 1, 1, None, C[2], P(C[3].value + 1), 4, F(1e-6), *C[4:10], 1,
+                                     64, None),
+    lambda L: L.ds_mla_decode4_step(*C[:5], P(C[5].value + 1), C[6], 4, 256, 16, F(1e-6), F(1), 0, F(0), *C[7:13], 1,
+                                    64, 4, C[13], C[14], 1 << 20, None),
+    lambda L: L.ds_mla_decode4_step(*C[:6], P(C[6].value + 1), 4, 256, 16, F(1e-6), F(1), 0, F(0), *C[7:13], 1, 64, 4,
+                                    C[13], C[14], 1 << 20, None),
+])
+def test_untyped_pointers_off_their_type_s_boundary_are_refused(call):
+    assert call(lib()) == 1
+    assert "aligned" in lib().ds_last_error().decode()
