@@ -21,6 +21,7 @@
 #include <mutex>
 
 #include "kernels.cuh"
+#include "partials.h"
 #include "ptx.cuh"
 
 namespace ds {
@@ -970,6 +971,15 @@ __global__ void __launch_bounds__(kAttnThreads, kCtasPerSm) attend4_kernel(const
   }
 }
 
+// A row's first partial and how many it has (1: none, the attention wrote the output); none for a sequence
+// without slots, nor where the attention gave up (the status word says so) before it wrote the entry.
+__device__ __forceinline__ int2 partials_of(const AttnParams& p, int b, int tile) {
+  if (chunks_of(p.c, b, p.max_chunks) == 0) return make_int2(0, 0);
+  const int2 w = __ldcg(p.where + b * p.tiles + tile);
+  if (w.y == 1 || partials_exist(w.x, w.y, p.ctas)) return w;
+  return make_int2(0, 0);
+}
+
 // Joins the partials of a (sequence, head tile), up to `most` of them: four blocks each, four heads
 // a block, a warp a head; lse (log2 of the weights' sum) where it is wanted; zeros for a sequence
 // without slots.  (48 registers and no shared memory: two blocks fit beside two CTAs of the attention and
@@ -981,8 +991,7 @@ __global__ void __launch_bounds__(kAttnThreads) merge_kernel(const AttnParams p,
   if (h >= p.heads) return;  // (a block has a head: its first warp's)
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
-  const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
-  const int2 w = empty ? make_int2(0, 0) : __ldcg(p.where + b * p.tiles + tile);
+  const int2 w = partials_of(p, b, tile);
   if (w.y == 1 || w.y > most) return;  // written by the attention kernel; merge_wide_kernel's
   __nv_bfloat16* o = p.out + (static_cast<int64_t>(b) * p.heads + h) * kLatent;
   const float* ml = p.part_ml + static_cast<int64_t>(w.x) * 32 + r;
@@ -1052,8 +1061,7 @@ __global__ void __launch_bounds__(32 * W) merge_wide_kernel(const AttnParams p, 
   if (tile * 16 + r >= p.heads) return;  // (head 0 has blocks)
   ptx::pdl_wait();
   ptx::pdl_launch_dependents();
-  const bool empty = chunks_of(p.c, b, p.max_chunks) == 0;
-  const int2 w = empty ? make_int2(0, 0) : __ldcg(p.where + b * p.tiles + tile);
+  const int2 w = partials_of(p, b, tile);
   if (w.y == 1 || w.y < least) return;
   const float* ml = p.part_ml + static_cast<int64_t>(w.x) * 32 + r;
   const int cc = lane & 3, jk = lane >> 2;  // as in merge_kernel
