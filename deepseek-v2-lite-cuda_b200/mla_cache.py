@@ -350,6 +350,11 @@ class LatentKVCache4:
     def _advance(self, n: int) -> None:
         self._bound = min(self._bound + n, self.max_seq)
         self._seen += n
+        # what runs before a recorded reset or eviction does adds to what they will find; what a
+        # recording has counted too many (n < 0) was never there
+        if self._held_seen and n > 0 and not self._recording():
+            self._held = min(self._held + n, self.max_seq)
+            self._held_seen += n
 
     def _evicted(self, src: "LatentKVCache4", budget: int) -> None:
         bound, seen = min(src.current_len, budget), max(src._seen, src._held_seen)

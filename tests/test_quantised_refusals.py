@@ -233,3 +233,41 @@ def test_eviction_refuses_arrays_that_it_could_not_read_four_at_a_time(slots, wh
 def test_untyped_pointers_off_their_type_s_boundary_are_refused(call):
     assert call(lib()) == 1
     assert "aligned" in lib().ds_last_error().decode()
+
+
+def recording(m):
+    m.setattr(LatentKVCache4, "_recording", lambda self: True)
+
+
+def test_eager_calls_behind_a_recorded_eviction_move_the_bounds_of_what_is_held(monkeypatch):
+    monkeypatch.setattr("mla_cache._capturing", lambda: False)
+    c = LatentKVCache4(2, 400, "cpu")
+    c._advance(200)
+    with monkeypatch.context() as m:
+        recording(m)
+        c._evicted(c, 100)
+        c._advance(1)                            # the recorded step's token
+    c.note_replay(-1)                            # recording appended nothing
+    assert c.current_len == 200 and c.bound_for_launch == 200
+    for i in range(150):                         # eager tokens: the eviction has not run
+        c._check_room(1, 1000)
+        c._advance(1)
+        assert c.current_len == c.bound_for_launch == 201 + i
+    c._advance(50)
+    with pytest.raises(RuntimeError, match="overflow"):
+        c._check_room(1, 1000)                   # the device holds 400 of 400
+    with pytest.raises(RuntimeError, match="RoPE"):
+        LatentKVCache4._check_room(c, 0, 399)
+    c.note_replay(1, budget=100)
+    assert c.current_len == 101 and c._seen == 401
+    # the same behind a recorded reset, and behind replays of a graph that does not evict
+    d = LatentKVCache4(2, 400, "cpu")
+    d._advance(300)
+    with monkeypatch.context() as m:
+        recording(m)
+        d.reset()
+    d._advance(3)
+    d.note_replay(2)
+    assert d.current_len == 305
+    d.note_replay(4, budget=0)
+    assert d.current_len == 4 and d._seen == 4
