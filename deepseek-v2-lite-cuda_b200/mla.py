@@ -125,7 +125,7 @@ class FusedMLA(nn.Module):
         x = hidden_states.to(torch.bfloat16)
         B, S, _ = x.shape
         if isinstance(cache, LatentKVCache4):
-            if cache.current_len != 0 or max(cache._seen, cache._held_seen) != 0 or cache.bsz != B:
+            if cache._now() != (0, 0) or cache.bsz != B:
                 raise RuntimeError("FusedMLA.prefill: the cache must be empty and of x's batch size")
             if S == 0:
                 return torch.empty_like(x)

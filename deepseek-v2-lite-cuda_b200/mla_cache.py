@@ -16,6 +16,7 @@ reference does; `side_bytes` the side arrays.
 """
 from __future__ import annotations
 
+import weakref
 from typing import Optional, Tuple
 
 import torch
@@ -200,8 +201,9 @@ class LatentKVCache4:
         self._bind()
         self._bound = 0      # no sequence is longer
         self._seen = 0       # no next position is larger
-        # the same for what a recorded reset or eviction, not replayed yet, has left in place
-        self._held = self._held_seen = 0
+        # (the two are those behind a recorded reset or eviction; until it is replayed the cache
+        # holds what it held, and this pair bounds that)
+        self._held: Optional[Tuple[int, int]] = None
 
     # the arrays may be written into, but not replaced: launches take their addresses
     codes = property(lambda self: self._codes)
@@ -221,6 +223,11 @@ class LatentKVCache4:
         self._ptrs = tuple(t.data_ptr() for t in (self._codes, self._scales, self._rstd, self._pos,
                                                   self._mass, self._state))
 
+    _source = None  # the cache that a recorded eviction into this one reads, as a weak reference
+
+    def __getstate__(self) -> dict:  # no graph evicts into a copy
+        return {**self.__dict__, "_source": None}
+
     def __setstate__(self, state: dict) -> None:  # a deep copy's or a pickle's arrays are others
         self.__dict__.update(state)
         self._bind()
@@ -228,9 +235,7 @@ class LatentKVCache4:
     @property
     def current_len(self) -> int:
         """A bound on the sequences' lengths (the length itself when they are equal)."""
-        if self._held > self._bound and not self._recording():
-            return self._held
-        return self._bound
+        return self._now()[0]
 
     @property
     def remaining_capacity(self) -> int:
@@ -246,7 +251,7 @@ class LatentKVCache4:
     def bound_for_launch(self) -> int:
         """The bound that a launch is sized for: all slots inside a graph capture, because a
         replay sees later lengths."""
-        return self.max_seq if _capturing() else max(self._bound, self._held)
+        return self.max_seq if _capturing() else self.current_len
 
     def reset(self) -> None:
         """Clear the cache for new sequences (keeps the memory)."""
@@ -267,13 +272,23 @@ class LatentKVCache4:
         import ds_kernels
         return ds_kernels.mla_cache4_evict(self, budget, recent, out)
 
-    def note_replay(self, tokens: int = 1, budget: Optional[int] = None) -> None:
+    def note_replay(self, tokens: int = 1, budget: Optional[int] = None,
+                    src: "Optional[LatentKVCache4]" = None) -> None:
         """A replayed graph appended `tokens` tokens to every sequence, and before (or after) it
-        evicted them down to `budget` slots (0: cleared them)."""
+        evicted them down to `budget` slots (0: cleared them).  If the eviction read another cache,
+        the bound is the whole budget, whatever that one holds; with the other cache named as `src`
+        it is what `src` is bounded by now.  Notes on several caches go in the order of the
+        graph's work."""
         if budget is not None:
-            self._bound = min(max(self._bound, self._held), budget)
-            self._seen = max(self._seen, self._held_seen) if budget > 0 else 0
-            self._held = self._held_seen = 0
+            bound, seen = self._now()
+            if budget <= 0:
+                bound = seen = 0
+            elif src is not None:
+                bound, seen = src._now()
+            elif self._source is not None:
+                other = self._source()
+                bound, seen = budget, max(seen, other._now()[1] if other is not None else 0)
+            self._bound, self._seen, self._held = min(bound, budget), seen, None
         self._advance(tokens)
 
     # ---- saving and restoring ------------------------------------------------------------
@@ -316,29 +331,32 @@ class LatentKVCache4:
             self.mass.zero_()
         self.lens.copy_(lens)
         self.next_pos.copy_(nxt)
-        self._bound, self._seen = hi, top
-        self._held = self._held_seen = 0
+        self._bound, self._seen, self._held = hi, top, None
 
     def __repr__(self) -> str:
-        return (f"LatentKVCache4(bsz={self.bsz}, tokens<={self._bound}/{self.max_seq}, "
+        return (f"LatentKVCache4(bsz={self.bsz}, tokens<={self.current_len}/{self.max_seq}, "
                 f"memory={self.memory_bytes / 2 ** 20:.2f}MB, device={self.device})")
 
     # ---- bookkeeping of the fused calls --------------------------------------------------
     def _recording(self) -> bool:
         return self.index >= 0 and _capturing()
 
+    def _now(self) -> Tuple[int, int]:
+        """Bounds on the lengths and next positions that the next call meets."""
+        if self._held is not None and not self._recording():
+            return self._held
+        return self._bound, self._seen
+
     def _hold(self) -> None:
         """Before the contents are replaced: recorded into a graph, they stay until a replay, and
         the calls up to then count on what is there."""
-        if self._recording():
-            self._held, self._held_seen = max(self._held, self._bound), max(self._held_seen, self._seen)
-        else:
-            self._held = self._held_seen = 0
+        if not self._recording():
+            self._held = None
+        elif self._held is None:
+            self._held = self._bound, self._seen
 
     def _check_room(self, n: int, table_rows: int) -> None:
-        bound, seen = self._bound, self._seen
-        if self._held_seen and not self._recording():
-            bound, seen = max(bound, self._held), max(seen, self._held_seen)
+        bound, seen = self._now()
         if bound + n > self.max_seq:
             raise RuntimeError(
                 f"KV cache overflow: current_len={bound}, new_tokens={n}, "
@@ -348,15 +366,18 @@ class LatentKVCache4:
                                f"tables ({table_rows} positions)")
 
     def _advance(self, n: int) -> None:
+        if self._held is not None and n > 0 and not self._recording():
+            self._held = min(self._held[0] + n, self.max_seq), self._held[1] + n
+            return
+        # (n < 0: what a recording has counted too many)
         self._bound = min(self._bound + n, self.max_seq)
         self._seen += n
-        # what runs before a recorded reset or eviction does adds to what they will find; what a
-        # recording has counted too many (n < 0) was never there
-        if self._held_seen and n > 0 and not self._recording():
-            self._held = min(self._held + n, self.max_seq)
-            self._held_seen += n
 
     def _evicted(self, src: "LatentKVCache4", budget: int) -> None:
-        bound, seen = min(src.current_len, budget), max(src._seen, src._held_seen)
+        bound, seen = src._now()
+        bound = min(bound, budget)
         self._hold()
+        if src is not self and self._recording():  # a replay takes what src holds by then
+            self._source = weakref.ref(src)
+            bound = budget
         self._bound, self._seen = bound, seen

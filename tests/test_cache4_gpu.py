@@ -607,3 +607,60 @@ def test_a_captured_eviction_replays():
         # the same sums, cut into other segments
         assert (out.float() - want.float()).norm() <= 2.0 ** -7 * want.float().norm()
     assert graphed.next_pos.tolist() == [153] * b
+
+
+def test_a_captured_eviction_into_another_cache_replays_over_a_grown_source():
+    b, heads = 2, 16
+    cos, sin = (t.cuda() for t in tables(2048))
+    lat, kpe = (t.cuda() for t in tokens(b, 1000, 80))
+    src, dst = LatentKVCache4(b, 1500), LatentKVCache4(b, 1000)
+    q = torch.randn(b, heads, 576).to(bf16).cuda()
+    ds_kernels.mla_cache4_append(lat[:, :200], kpe[:, :200], src, cos, sin)
+    ds_kernels.mla_cache4_append(lat[:, :40], kpe[:, :40], dst, cos, sin)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        src.evict(800, 8, out=dst)
+    # nothing has run yet: dst holds its 40 tokens, and takes more
+    assert dst.current_len == 40
+    ds_kernels.mla_cache4_append(lat[:, 40:60], kpe[:, 40:60], dst, cos, sin)
+    assert dst.current_len == 60 and dst.lens.tolist() == [60] * b
+    ds_kernels.mla_cache4_append(lat[:, 200:], kpe[:, 200:], src, cos, sin)
+    ds_kernels.mla_decode_attention4(q, src, SCALE, mass_decay=0.0)
+    want = src.evict(800, 8, out=LatentKVCache4(b, 1000))
+    graph.replay()
+    dst.note_replay(0, budget=800)
+    assert dst.lens.tolist() == [800] * b and dst.current_len == 800 and dst.next_pos.tolist() == [1000] * b
+    dst.mass.zero_()
+    want.mass.zero_()
+    got, ref = (ds_kernels.mla_decode_attention4(q, c, SCALE, mass_decay=0.0) for c in (dst, want))
+    assert torch.equal(got, ref)                         # all 800 slots, with and without the graph
+    assert torch.equal(dst.mass[:, :800], want.mass[:, :800])
+    assert ((dst.mass[:, :800].sum(1) - heads).abs() <= heads * 2.0 ** -14).all()
+    with pytest.raises(RuntimeError, match="overflow"):
+        ds_kernels.mla_cache4_append(lat[:, :201], kpe[:, :201], dst, cos, sin)
+    with pytest.raises(RuntimeError, match="RoPE"):
+        ds_kernels.mla_cache4_append(lat[:, :5], kpe[:, :5], dst, cos[:1004], sin[:1004])
+
+
+def test_eager_steps_behind_a_recorded_eviction_see_every_token():
+    b, n, more = 2, 200, 150
+    cos, sin = (t.cuda() for t in tables(512))
+    lat, kpe = (t.cuda() for t in tokens(b, n + more, 81))
+    c, eager = LatentKVCache4(b, 400), LatentKVCache4(b, 400)
+    q = torch.randn(b, 16, 576).to(bf16).cuda()
+    for x in (c, eager):
+        ds_kernels.mla_cache4_append(lat[:, :n], kpe[:, :n], x, cos, sin)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.evict(100, 8)
+    for x in (c, eager):
+        ds_kernels.mla_cache4_append(lat[:, n:], kpe[:, n:], x, cos, sin)
+    assert c.current_len == eager.current_len == n + more == c.lens[0].item()
+    got, want = (ds_kernels.mla_decode_attention4(q, x, SCALE, mass_decay=0.0) for x in (c, eager))
+    assert torch.equal(got, want) and torch.equal(c.mass, eager.mass)
+    graph.replay()
+    c.note_replay(0, budget=100)
+    eager.evict(100, 8)
+    assert c.current_len == 100 and torch.equal(c.pos[:, :100], eager.pos[:, :100])

@@ -271,3 +271,44 @@ def test_eager_calls_behind_a_recorded_eviction_move_the_bounds_of_what_is_held(
     assert d.current_len == 305
     d.note_replay(4, budget=0)
     assert d.current_len == 4 and d._seen == 4
+
+
+def test_a_recorded_eviction_into_another_cache_bounds_whatever_its_source_holds_by_then(monkeypatch):
+    import copy
+    import pickle
+    monkeypatch.setattr("mla_cache._capturing", lambda: False)
+    src, dst = LatentKVCache4(2, 2000, "cpu"), LatentKVCache4(2, 1000, "cpu")
+    src._advance(200)
+    with monkeypatch.context() as m:
+        recording(m)
+        dst._evicted(src, 800)
+        with pytest.raises(RuntimeError, match="overflow"):
+            dst._check_room(201, 5000)           # a replay may leave 800
+    assert src.current_len == 200 and dst.current_len >= 0
+    src._advance(800)                            # 1000 by the replay: min(1000, 800) slots arrive
+    dst.note_replay(0, 800)
+    assert dst.current_len == dst.bound_for_launch == 800 and dst._seen == 1000
+    with pytest.raises(RuntimeError, match="overflow"):
+        dst._check_room(201, 5000)
+    with pytest.raises(RuntimeError, match="RoPE"):
+        dst._check_room(1, 1000)
+    dst.reset()                                  # and again behind a reset of the result
+    assert dst.current_len == 0
+    src._advance(300)
+    dst.note_replay(0, budget=800)
+    assert dst.current_len == 800 and dst._seen == 1300
+    dst.reset()
+    dst.note_replay(2, 800, src=src)             # with the source named, its own bounds count
+    assert dst.current_len == 802 and dst._seen == 1302
+    short = LatentKVCache4(2, 2000, "cpu")
+    short._advance(5)
+    dst.reset()
+    dst.note_replay(0, 800, src=short)
+    assert dst.current_len == 5 and dst._seen == 5
+    for d in (copy.deepcopy(dst), pickle.loads(pickle.dumps(dst))):  # no graph writes into a copy
+        d.reset()
+        d.note_replay(0, 800)
+        assert d.current_len == 0 and d._seen == 0
+    del src                                      # the graph's memory is gone, the bounds stay usable
+    dst.note_replay(0, 800)
+    assert dst.current_len == 800
