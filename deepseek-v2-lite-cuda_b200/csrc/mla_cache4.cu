@@ -97,6 +97,11 @@ __device__ __forceinline__ float usable(__nv_bfloat16 sc) {
   return s > 0.f ? s : 0.f;  // false for NaN
 }
 
+// The RoPE tables' row of a position, which stands in an array that the caller may write.
+__device__ __forceinline__ int table_row(int position, int rows) {
+  return min(max(position, 0), rows - 1);
+}
+
 // One warp quantises one token into (b, slot): lane l holds latent dimensions 16 l .. 16 l +
 // 15 (a group of 128 = 8 lanes) and the rotation pair l of k_pe.
 struct Token {
@@ -141,7 +146,7 @@ __device__ __forceinline__ void put_token(const Cache& c, int b, int slot, int p
   else
     packed = make_uint2(codes8<false>(v, qs), codes8<false>(v + 8, qs));
   // k_pe at its position: the interleave -> half RoPE of src/reference/mla.py:176-206
-  const int prow = min(position, table_rows - 1);
+  const int prow = table_row(position, table_rows);
   const __nv_bfloat16* cr = cos_t + static_cast<int64_t>(prow) * kRope;
   const __nv_bfloat16* sr = sin_t + static_cast<int64_t>(prow) * kRope;
   const float xa = __low2float(kp), xb = __high2float(kp);
@@ -248,7 +253,7 @@ __global__ void __launch_bounds__(288)
     if (len >= 0 && len < c.slots)
       put_token(c, b, len, next, tok, cos_t, sin_t, table_rows, eps);
   } else {
-    const int prow = min(next, table_rows - 1);
+    const int prow = table_row(next, table_rows);
     const __nv_bfloat16* cr = cos_t + static_cast<int64_t>(prow) * kRope;
     const __nv_bfloat16* sr = sin_t + static_cast<int64_t>(prow) * kRope;
     for (int h = warp - 1; h < heads; h += 8) {

@@ -314,9 +314,13 @@ class LatentKVCache4:
                 raise ValueError(f"load_state_dict: unexpected {k} of shape {tuple(t.shape)}")
         lens = state["lens"].to(self.device, torch.int32)
         nxt = state["next_pos"].to(self.device, torch.int32) if "next_pos" in state else lens
-        lo, hi, top = (int(v) for v in torch.stack([lens.min(), lens.max(), nxt.max()]).tolist())
+        early = (nxt < lens).any().to(torch.int32)
+        lo, hi, top, early = (int(v) for v in
+                              torch.stack([lens.min(), lens.max(), nxt.max(), early]).tolist())
         if n > self.slots or lo < 0 or hi > min(n, self.max_seq):
             raise ValueError("load_state_dict: the saved sequences do not fit the cache")
+        if early:
+            raise ValueError("load_state_dict: next_pos must be at least the number of tokens")
         for k in ("codes", "scales", "rstd"):
             dst = getattr(self, k)
             (dst[:, :, :n] if k == "scales" else dst[:, :n]).copy_(state[k])

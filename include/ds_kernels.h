@@ -507,8 +507,8 @@ DS_API int ds_int8_linear(const void* x_bf16, int64_t row_stride, const void* w_
  * ds_mla_cache4_append: new_tokens tokens of every sequence (token i of sequence b at row
  *   b * src_rows_per_seq + i of latent / kpe; only the first new_lens[b] when given) quantised
  *   behind its last slot, k_pe rotated at its position (table rows cos/sin [table_rows, 64];
- *   positions past the table take its last row); mass 0.  Lengths and positions move on.
- *   Tokens past the last slot are dropped.
+ *   positions past the table take its last row, negative ones its first); mass 0.  Lengths and
+ *   positions move on.  Tokens past the last slot are dropped.
  * ds_mla_cache4_get: slots 0 .. seq_len-1 as bf16 values (raw latent [batch, seq_len, 512],
  *   rotated k_pe [batch, seq_len, 64]); zeros from a sequence's length on.
  * ds_mla_decode_attention4: one query token per sequence: q bf16 [batch, heads, 576] (absorbed

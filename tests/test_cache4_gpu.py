@@ -664,3 +664,19 @@ def test_eager_steps_behind_a_recorded_eviction_see_every_token():
     c.note_replay(0, budget=100)
     eager.evict(100, 8)
     assert c.current_len == 100 and torch.equal(c.pos[:, :100], eager.pos[:, :100])
+
+
+@pytest.mark.parametrize("start", [-5, -2 ** 31, 62, 2 ** 31 - 2])
+def test_positions_outside_the_tables_take_their_first_or_last_row(start):
+    """next_pos is an array that the caller may write (the host's bound does not see it)."""
+    b, n, rows = 2, 7, 64
+    cos, sin = tables(rows)
+    lat, kpe = tokens(b, n, 82)
+    cache = LatentKVCache4(b, 64)
+    cache.next_pos.fill_(start)
+    ds_kernels.mla_cache4_append(lat.cuda(), kpe.cuda(), cache, cos.cuda(), sin.cuda())
+    at = torch.arange(start, start + n)
+    at = (at + 2 ** 31) % 2 ** 32 - 2 ** 31                # as int32 counts
+    want = quant64(rotate(kpe, at.clamp(0, rows - 1).expand(b, -1), cos, sin), 64)[0]
+    assert torch.equal(unpack(cache.codes[:, :n].cpu())[..., 512:], want)
+    assert torch.equal(cache.pos[:, :n].cpu().long(), at.expand(b, -1))

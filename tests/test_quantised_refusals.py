@@ -312,3 +312,15 @@ def test_a_recorded_eviction_into_another_cache_bounds_whatever_its_source_holds
     del src                                      # the graph's memory is gone, the bounds stay usable
     dst.note_replay(0, 800)
     assert dst.current_len == 800
+
+
+@pytest.mark.parametrize("next_pos", [[-1, 5], [2, 5], [3, -2 ** 31]])
+def test_load_state_dict_refuses_positions_before_the_tokens_that_are_there(next_pos):
+    c = LatentKVCache4(2, 64, "cpu")
+    c.state[:2].copy_(torch.tensor([[3, 4], [3, 4]]))
+    sd = c.state_dict()
+    sd["next_pos"] = torch.tensor(next_pos, dtype=torch.int32)
+    d = LatentKVCache4(2, 64, "cpu")
+    with pytest.raises(ValueError, match="next_pos"):
+        d.load_state_dict(sd)
+    assert d.lens.tolist() == [0, 0] and d.current_len == 0
