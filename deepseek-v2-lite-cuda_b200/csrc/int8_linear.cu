@@ -549,6 +549,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       swt[et] = n0 + et < p.N ? p.sw[n0 + et] : 0.f;
       swt[et + 128] = n0 + et + 128 < p.N ? p.sw[n0 + et + 128] : 0.f;
       const float sa = m0 + r < p.M ? p.sa[m0 + r] : 0.f;
+      __syncwarp();
       ptx::named_bar_sync(1, 128);
       int ok = 1;
       if (lane == 0)

@@ -1298,6 +1298,7 @@ __device__ __forceinline__ uint32_t find_in_list(const uint32_t* list, int n, in
       x += (k[i] >= c1 ? 1u : 0u) + (k[i] >= c2 ? 1u << 10 : 0u) + (k[i] >= c3 ? 1u << 20 : 0u);
     x = __reduce_add_sync(0xffffffffu, x);
     if (lane == 0) part[round & 1][warp] = x;
+    __syncwarp();
     ptx::named_bar_sync(1, 128);
     const uint4 y = *reinterpret_cast<const uint4*>(part[round & 1]);
     x = (y.x + y.y) + (y.z + y.w);
@@ -1476,6 +1477,7 @@ __device__ __forceinline__ ClusterSum cluster_sum(int u, int v, int w, int4 (*x)
     asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(u), "r"(v), "r"(w), "r"(0)
                  : "memory");
   }
+  __syncwarp();  // the barrier is `.aligned`: a warp's lanes have to reach it together
   ptx::cluster_sync();
   ClusterSum s = {};
   for (uint32_t k = 0; k < size; ++k) {
@@ -1520,6 +1522,7 @@ __global__ void __launch_bounds__(1024)
       *reinterpret_cast<int4*>(ps + i) = *reinterpret_cast<const int4*>(pos + t0 + i);
     }
   const int len = min(max(c.state[b], 0), c.slots), next = c.state[c.batch + b];
+  __syncwarp();  // (some lanes may have had slots to load)
   ptx::cluster_sync();  // all blocks have started, and have read the length
   int32_t* const src = src_of + static_cast<int64_t>(b) * budget;
   int32_t* const hole = holes + static_cast<int64_t>(b) * budget;
@@ -1569,6 +1572,7 @@ __global__ void __launch_bounds__(1024)
           asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(first + 4 * at), "r"(key[i]) : "memory");
           ++at;
         }
+      __syncwarp();
       ptx::cluster_sync();
       if (rank == 0 && threadIdx.x < 128) {
         const uint32_t f = find_in_list(list, in_range, budget - over_end, shift, v, part);
@@ -1577,6 +1581,7 @@ __global__ void __launch_bounds__(1024)
                        "r"(f)
                        : "memory");
       }
+      __syncwarp();
       ptx::cluster_sync();
       v = found;
     }
@@ -1619,6 +1624,7 @@ __global__ void __launch_bounds__(1024)
       if (keep >> i & 1u) src[t] = t;
       else hole[h++] = t;
     }
+    __syncwarp();
     ptx::cluster_sync();  // the holes are written before survivors are paired with them
 #pragma unroll
     for (int i = 0; i < IPT; ++i)
