@@ -87,8 +87,10 @@ class FusedDecoderStack:
                     mass_decay: Optional[float] = None) -> torch.Tensor:
         """x bf16 [bsz, hidden] (one new token per sequence) -> [bsz, hidden].  mass_decay (4-bit
         caches): accumulate every layer's attention weights for evict()."""
+        # (only where asked for: attention objects of bf16 caches alone need not know it)
+        kw = {} if mass_decay is None else {"mass_decay": mass_decay}
         return self._run(x.contiguous(),
-                         lambda layer, h, i: layer.attn.decode(h, caches[i], mass_decay=mass_decay),
+                         lambda layer, h, i: layer.attn.decode(h, caches[i], **kw),
                          lambda h: h)
 
     def capture_decode(self, x: torch.Tensor, caches: Sequence[LatentKVCache],
