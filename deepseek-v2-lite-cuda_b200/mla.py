@@ -111,9 +111,12 @@ class FusedMLA(nn.Module):
 
     def quantized_decode_weights(self):
         """(w_dec int8, its scales f32, w_out int8, its scales f32): decode_weights() in 8 bits with
-        a scale per output channel, built once."""
+        a scale per output channel, built once.  The bf16 ones (twice the memory) stay only if a
+        bf16 step has built them before."""
         if self._dec_q is None:
+            kept = self._dec_w
             w_dec, w_out = self.decode_weights()
+            self._dec_w = kept
             self._dec_q = (*ds_kernels.int8_quantize(w_dec), *ds_kernels.int8_quantize(w_out))
         return self._dec_q
 
