@@ -680,3 +680,63 @@ def test_positions_outside_the_tables_take_their_first_or_last_row(start):
     want = quant64(rotate(kpe, at.clamp(0, rows - 1).expand(b, -1), cos, sin), 64)[0]
     assert torch.equal(unpack(cache.codes[:, :n].cpu())[..., 512:], want)
     assert torch.equal(cache.pos[:, :n].cpu().long(), at.expand(b, -1))
+
+
+@pytest.mark.parametrize("heads", [1, 5, 15, 17, 24, 40, 48, 128])
+@pytest.mark.parametrize("lens", [[1, 0, 700], [129, 64, 1000, 5]])
+def test_weights_of_any_number_of_heads(heads, lens):
+    b = len(lens)
+    cache, st = random_cache(b, 1000, lens, heads)
+    q = torch.randn(b, heads, 576, generator=torch.Generator().manual_seed(heads)).to(bf16)
+    ref, tol, mass, mtol = attend64(st, q, lens)
+    cache.mass.fill_(3.0)
+    check(ds_kernels.mla_decode_attention4(q.cuda(), cache, SCALE, mass_decay=0.25), ref, tol)
+    for i, n in enumerate(lens):
+        check(cache.mass[i, :n], 0.75 + mass[i, :n], mtol[i, :n] + 2.0 ** -22 * (0.75 + mass[i, :n]))
+        assert (cache.mass[i, n:] == 3.0).all()
+
+
+@pytest.mark.parametrize("b,heads,top", [(330, 16, 700), (50, 128, 400), (301, 1, 129)])
+def test_more_rows_than_ctas(b, heads, top):
+    """More non-empty (sequence, head tile) rows than CTAs run at once: a CTA takes several, whole, one
+    after the other, of other lengths each."""
+    lens = [(97 * i) % (top + 1) for i in range(b)]
+    lens[3], lens[-1] = 0, top
+    cache, st = random_cache(b, top, lens, b)
+    q = torch.randn(b, heads, 576, generator=torch.Generator().manual_seed(b)).to(bf16)
+    ref, tol, mass, mtol = attend64(st, q, lens)
+    out = ds_kernels.mla_decode_attention4(q.cuda(), cache, SCALE)
+    check(out, ref, tol)
+    cache.mass.fill_(float("nan"))
+    assert torch.equal(ds_kernels.mla_decode_attention4(q.cuda(), cache, SCALE, mass_decay=0.0), out)
+    for i, n in enumerate(lens):
+        check(cache.mass[i, :n], mass[i, :n], mtol[i, :n])
+        assert torch.isnan(cache.mass[i, n:]).all()
+    assert ds_kernels.device_status() == ds_kernels.DS_OK
+
+
+@pytest.mark.parametrize("kind", ["random", "equal", "odd"])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_by_the_largest_clusters(kind, in_place):
+    """131073 to 262144 slots: eight blocks a sequence, 32 keys a thread."""
+    lens, budget, recent = [200000, 262144, 131073, 7], 30000, 77
+    b = len(lens)
+    cache = LatentKVCache4(b, max(lens))
+    cache.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    cache.next_pos.copy_(cache.lens)
+    cache._bound = cache._seen = max(lens)
+    g = torch.Generator().manual_seed(9)
+    mass = masses(kind, b, cache.slots, budget)
+    pos = torch.stack([torch.cat([torch.randperm(n, generator=g), torch.full((cache.slots - n,), -1)]) for n in lens])
+    cache.mass.copy_(mass)
+    cache.pos.copy_(pos)
+    cache.codes[:, :, 0] = (pos % 251).to(torch.uint8).cuda()       # rows that tell where they came from
+    cache.codes[:, :, 287] = (pos % 253).to(torch.uint8).cuda()
+    out = ds_kernels.mla_cache4_evict(cache, budget, recent, None if in_place else LatentKVCache4(b, budget))
+    assert out.lens.tolist() == [min(n, budget) for n in lens] and out.next_pos.tolist() == lens
+    for i, n in enumerate(lens):
+        src = evict_ref_long(mass[i], pos[i], n, n, budget, recent)
+        assert torch.equal(out.pos[i, :len(src)].cpu().long(), pos[i][src])
+        assert torch.equal(out.mass[i, :len(src)].cpu().nan_to_num(-5), mass[i][src].nan_to_num(-5))
+        assert torch.equal(out.codes[i, :len(src), 0].cpu().long(), pos[i][src] % 251)
+        assert torch.equal(out.codes[i, :len(src), 287].cpu().long(), pos[i][src] % 253)

@@ -182,3 +182,19 @@ def test_custom_operators():
 
     for got, want in zip(torch.compile(f, fullgraph=True)(x), f(x)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,k,n", [(8200, 272, 2072), (4500, 912, 4616)])
+def test_linear_with_several_tiles_for_each_pair_of_ctas(m, k, n):
+    """297 and 342 tiles of 256 x 256 for at most 74 pairs, ragged at every edge: accumulators, ring and
+    channel scales go on from tile to tile.  More tiles than the ring has stages, and fewer."""
+    x, (w, ws) = rows(m, k, m), weights(n, k, n)
+    check(ds_kernels.int8_linear(x.cuda(), w.cuda(), ws.cuda()), linear64(x, w, ws))
+
+
+@pytest.mark.parametrize("k", [1136, 1152, 2160, 2304, 2560, 3136, 5248])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 16, 17, 33, 64, 100, 128])
+def test_linear_with_parts_of_k_for_clusters_of_3_6_and_7(m, k):
+    for n in (8, 264):
+        x, (w, ws) = rows(m, k, m), weights(n, k, n)
+        check(ds_kernels.int8_linear(x.cuda(), w.cuda(), ws.cuda()), linear64(x, w, ws))
