@@ -686,8 +686,8 @@ int set_attrs(const DeviceInfo& di) {
   return DS_OK;
 }
 
-// K in parts: enough CTAs for the SMs to stream (up to 1.6 a SM; two fit), four k-blocks each at
-// least, clusters of at most 8.  None is empty.
+// K in parts: enough CTAs for the SMs to stream (up to 1.6 a SM; two fit), two k-blocks each or more (the
+// last part may have fewer, and none is empty), clusters of at most 8: of 1 to 4 or 6 to 8 as it comes out.
 void few_splits(int64_t tiles, int k_blocks, int num_sms, int* splits, int* per) {
   int n = 1;
   while (n < 8 && tiles * n * 10 <= num_sms * 8 && k_blocks >= 4 * n) n *= 2;

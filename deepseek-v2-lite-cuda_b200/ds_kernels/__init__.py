@@ -837,7 +837,8 @@ def _rows_2d(x: torch.Tensor) -> torch.Tensor:
 
 def int8_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
                 workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """x bf16 [..., K] @ (w_q int8 [N, K] * w_scale f32 [N, 1])^T -> bf16 [..., N] (additive).
+    """x bf16 [..., K] @ (w_q int8 [N, K] * w_scale[:, None])^T -> bf16 [..., N], w_scale f32 [N]
+    (additive).
 
     The rows of x are quantised as int8_quantize does, the product of the integers is exact
     (32 bits) and scaled once: bf16(acc * (scale_row * w_scale)).  K: a multiple of 16, at most

@@ -124,7 +124,8 @@ class FusedMLA(nn.Module):
                 prompt_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """forward() over a prompt at positions 0 .. seq-1 that also fills the (empty) cache.
         A 4-bit cache takes prompt_lens (int32 [bsz], on the device) for padded prompts: only the
-        first prompt_lens[b] tokens of sequence b enter it."""
+        first prompt_lens[b] tokens of sequence b enter it.  Tokens enter with weight 0: the prompt's
+        own attention is not accumulated, decode steps with mass_decay are."""
         x = hidden_states.to(torch.bfloat16)
         B, S, _ = x.shape
         if isinstance(cache, LatentKVCache4):

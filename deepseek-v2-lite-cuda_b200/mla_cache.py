@@ -172,7 +172,8 @@ class LatentKVCache4:
                                          bf16(max |v| / 7)
         rstd    f32   [bsz, slots]       rsqrt(mean(latent^2) + eps) of the exact latent
         pos     int32 [bsz, slots]       position of the token in the slot
-        mass    f32   [bsz, slots]       accumulated attention weight
+        mass    f32   [bsz, slots]       accumulated attention weight: 0 for a token that is
+                                         appended (prompts too), moved by decode steps alone
 
     The host knows only a bound on the lengths (`current_len`: exact for batches that are not
     ragged), which it advances with every call; no call synchronises.  A call recorded into a

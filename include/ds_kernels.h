@@ -486,7 +486,8 @@ DS_API int ds_ep_layer_forward(const void* x_bf16, int num_tokens,
  * / a) (ties to even), scale = a / 127 with a = max |x|; a = 0 gives zeros, a row with an
  * infinity or a NaN gives zeros and scale NaN.  ds_int8_linear quantises the rows of x so and
  * writes out[m, n] = bf16((sum_k q[m,k] w[n,k]) * (scale[m] * w_scale[n])), the sum exact.
- * cols / in_features: a multiple of 16, at most 131072; out_features: a multiple of 8. */
+ * cols: a multiple of 16; in_features: a multiple of 16, at most 131072 (the sums are 32-bit);
+ * out_features: a multiple of 8. */
 DS_API int ds_int8_quantize(const void* x_bf16, int64_t row_stride, int rows, int cols,
                             void* q_int8, float* scale, void* stream);
 DS_API size_t ds_int8_linear_workspace_size(int rows, int out_features, int in_features);
