@@ -157,3 +157,51 @@ def test_replays_stop_at_the_end_of_the_rope_tables(stack):
     caches[0]._seen = 3
     with pytest.raises(RuntimeError, match="empty"):
         stack.layers[0].attn.prefill(torch.randn(1, 4, 256, device="cuda").to(bf16), caches[0])
+
+
+def test_steps_of_two_caches_captured_on_forked_streams():
+    """Kernels that are set up under their predecessors, behind forks and joins of a capture."""
+    b, heads, hidden = 4, 16, 256
+    attn = attn_weights(hidden, heads, 512, 11)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(2, b, hidden, generator=g, device="cuda").to(bf16)
+    lat = torch.randn(b, 200, 512, generator=g, device="cuda").to(bf16)
+    kpe = torch.randn(b, 200, 64, generator=g, device="cuda").to(bf16)
+    w, s = attn.quantized_decode_weights()[2:]
+    w2, s2 = ds_kernels.int8_quantize(torch.randn(hidden, hidden, generator=g, device="cuda").to(bf16))
+
+    def caches():
+        out = [LatentKVCache4(b, 400) for _ in range(2)]
+        for c in out:
+            ds_kernels.mla_cache4_append(lat, kpe, c, attn.cos, attn.sin)
+        return out
+
+    def both(cs, side):
+        main = torch.cuda.current_stream()
+        if side is not None:
+            side.wait_stream(main)
+        y0 = attn.decode(x[0], cs[0], mass_decay=1.0)
+        with torch.cuda.stream(side if side is not None else main):
+            cs[1].evict(150, 10)
+            if side is None:    # a recorded call is cut for all slots: so is the eager one here
+                cs[0]._bound = cs[1]._bound = 399
+            y1 = attn.decode(x[1], cs[1], mass_decay=1.0)
+        if side is not None:
+            main.wait_stream(side)
+        return ds_kernels.int8_linear(y0 + y1, w2, s2), y0, y1
+
+    plain, forked = caches(), caches()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = both(forked, side)
+    for _ in range(4):
+        graph.replay()
+        plain[0]._bound = 399
+        for a, c in zip(got, both(plain, None)):
+            assert torch.isfinite(a).all() and torch.equal(a, c)
+        assert torch.equal(forked[0].state, plain[0].state) and torch.equal(forked[1].state, plain[1].state)
+        assert torch.equal(forked[0].codes, plain[0].codes)
+    assert forked[0].lens.tolist() == [204] * b and forked[1].lens.tolist() == [151] * b
+    assert ds_kernels.device_status() == ds_kernels.DS_OK
