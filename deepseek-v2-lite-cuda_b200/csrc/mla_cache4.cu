@@ -1808,9 +1808,9 @@ int launch_append(const Cache& c, const void* lat, int64_t lat_ld, const void* k
 int launch_evict(const Cache& s, const Cache& d, int budget, int recent, bool in_place,
                  int32_t* src_of, int32_t* holes, cudaStream_t st) {
   // One block a sequence up to 8192 slots, whatever the batch: clusters of two or more (four keys a thread)
-  // meet over the SMs in every round and need the second launch, 8192 slots to 256: 17.6 us against 14.5 (1 sequence),
-  // 18.7 against 14.7 (32), 31.2 against 19.2 (148); 2048 slots to 1024: 16.6 against 12.2, 20.4 against
-  // 15.6, 41.0 against 30.7.
+  // meet over the SMs in every round and need the second launch, 8192 slots to 256: 17.6 us against 14.5
+  // (1 sequence), 18.7 against 14.7 (32), 31.2 against 19.2 (148); 2048 slots to 1024: 16.6 against 12.2,
+  // 20.4 against 15.6, 41.0 against 30.7.
   // Few rows: the planning block moves them (no second launch); many: all SMs do.
   const bool one = s.slots <= 8192, here = one && budget <= kRowsHere;
   if (one) {

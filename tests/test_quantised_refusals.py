@@ -309,6 +309,8 @@ def test_a_recorded_eviction_into_another_cache_bounds_whatever_its_source_holds
         d.reset()
         d.note_replay(0, 800)
         assert d.current_len == 0 and d._seen == 0
+    dst.note_replay(0, 5000)                     # more than there are slots
+    assert dst.current_len == 1000
     del src                                      # the graph's memory is gone, the bounds stay usable
     dst.note_replay(0, 800)
     assert dst.current_len == 800
