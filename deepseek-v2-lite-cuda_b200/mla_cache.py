@@ -289,7 +289,7 @@ class LatentKVCache4:
             elif self._source is not None:
                 other = self._source()
                 bound, seen = budget, max(seen, other._now()[1] if other is not None else 0)
-            self._bound, self._seen, self._held = min(bound, budget, self.max_seq), seen, None
+            self._bound, self._seen, self._held = min(bound, budget), seen, None
         self._advance(tokens)
 
     # ---- saving and restoring ------------------------------------------------------------
